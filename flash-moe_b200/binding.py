@@ -16,6 +16,8 @@ LIB_PATH = HERE / "libfm_b200.so"
 FM_OK, FM_ERR_INVALID, FM_ERR_CAPACITY, FM_ERR_NOMEM, FM_ERR_CUDA, FM_ERR_TIMEOUT, FM_ERR_UNSUPPORTED = range(7)
 FM_PTR_DEVICE, FM_PTR_HOST = 0, 1
 FM_KV_BF16, FM_KV_FP8_E4M3 = 0, 1
+FM_W_Q4_AFFINE = 0
+FM_SCORE_SOFTMAX, FM_SCORE_SIGMOID = 0, 1
 
 EXPORTS = [
     "fm_default_config", "fm_create", "fm_destroy", "fm_last_error", "fm_set_stream",
@@ -26,6 +28,7 @@ EXPORTS = [
     "fm_attn_decode_static", "fm_exchange_bytes", "fm_exchange_attach", "fm_attn_decode_exchange_push",
     "fm_attn_decode_exchange_merge", "fm_attn_decode_exchange", "fm_attn_decode_layers",
     "fm_kv_export_fp8", "fm_kv_import_fp8", "fm_h2o_export", "fm_proj_upload", "fm_proj_free", "fm_out_proj_norm",
+    "fm_proj_forward", "fm_default_route_config", "fm_moe_route", "fm_moe_experts",
 ]
 
 
@@ -61,6 +64,19 @@ class FmProjWeights(C.Structure):
                 ("w", C.c_void_p), ("scales", C.c_void_p), ("biases", C.c_void_p)]
 
 
+class FmRouteConfig(C.Structure):
+    _fields_ = [("num_experts", C.c_int), ("top_k", C.c_int), ("score", C.c_int), ("num_groups", C.c_int), ("top_groups", C.c_int),
+                ("group_best", C.c_int), ("renormalize", C.c_int), ("scale", C.c_float), ("shared_expert", C.c_int)]
+
+
+class FmExpertWeights(C.Structure):
+    _fields_ = [("format", C.c_int), ("num_experts", C.c_int), ("first_expert", C.c_int), ("hidden", C.c_int), ("inter", C.c_int),
+                ("group_size", C.c_int), ("expert_stride", C.c_int64),
+                ("gate_w", C.c_void_p), ("gate_scales", C.c_void_p), ("gate_biases", C.c_void_p),
+                ("up_w", C.c_void_p), ("up_scales", C.c_void_p), ("up_biases", C.c_void_p),
+                ("down_w", C.c_void_p), ("down_scales", C.c_void_p), ("down_biases", C.c_void_p)]
+
+
 class FmError(RuntimeError):
     def __init__(self, status: int, text: str):
         super().__init__(f"fm status {status}: {text}")
@@ -85,6 +101,7 @@ def load_library() -> C.CDLL:
     lib.fm_exchange_bytes.restype = C.c_size_t
     lib.fm_exchange_bytes.argtypes = [C.c_void_p, C.c_int]
     lib.fm_proj_free.restype = None
+    lib.fm_default_route_config.restype = None
     return lib
 
 
@@ -114,6 +131,38 @@ def default_config(**kw) -> FmConfig:
             raise AttributeError(k)
         setattr(cfg, k, v)
     return cfg
+
+
+def route_config(**kw) -> FmRouteConfig:
+    """fm_default_route_config with the given fields changed."""
+    rc = FmRouteConfig()
+    load_library().fm_default_route_config(C.byref(rc))
+    for k, v in kw.items():
+        if not hasattr(rc, k):
+            raise AttributeError(k)
+        setattr(rc, k, v)
+    return rc
+
+
+def proj_weights(w, scales, biases) -> FmProjWeights:
+    """A 4-bit affine matrix that lies in device memory already: w int32 [out][in/8], scales and biases bf16 [out][in/64]
+    (CUDA tensors, kept alive by the result)."""
+    out_dim, in_dim = w.shape[-2], w.shape[-1] * 8
+    assert scales.shape == biases.shape == (out_dim, in_dim // 64)
+    r = FmProjWeights(FM_W_Q4_AFFINE, out_dim, in_dim, 64, _ptr(w), _ptr(scales), _ptr(biases))
+    r.keep = (w, scales, biases)
+    return r
+
+
+def expert_weights(gate, up, down, first_expert: int = 0) -> FmExpertWeights:
+    """Stacks of 4-bit affine matrices in device memory, each a (w, scales, biases) of CUDA tensors: gate and up
+    [experts][inter][hidden / 8], down [experts][hidden][inter / 8] int32 words, [..][in / 64] bf16 scales and biases."""
+    experts, inter, hidden = gate[0].shape[0], gate[0].shape[1], down[0].shape[1]
+    for (w, s, b), (rows, cols) in ((gate, (inter, hidden)), (up, (inter, hidden)), (down, (hidden, inter))):
+        assert w.shape == (experts, rows, cols // 8) and s.shape == b.shape == (experts, rows, cols // 64)
+    r = FmExpertWeights(FM_W_Q4_AFFINE, experts, first_expert, hidden, inter, 64, 0, *(_ptr(t) for m in (gate, up, down) for t in m))
+    r.keep = (gate, up, down)
+    return r
 
 
 class Context:
@@ -325,6 +374,38 @@ class Context:
 
     def out_proj_norm(self, dev, n, x, residual, norm_w, h_mid, h_post):
         self._check(self.lib.fm_out_proj_norm(self.h, C.byref(dev), C.c_int(n), _ptr(x), _ptr(residual), _ptr(norm_w), _ptr(h_mid), _ptr(h_post)))
+
+    def _bound(self, fn, *args, keep=()):
+        """A zero-argument callable for fn(ctx, *args) with converted arguments (like `prepared`)."""
+        h, check = self.h, self._check
+
+        def call(_keep=keep):
+            check(fn(h, *args))
+        return call
+
+    def prepared_proj_forward(self, weights, n, x, ys):
+        """fm_proj_forward as a callable: weights a list of FmProjWeights that share their input, ys one output each."""
+        w = (FmProjWeights * len(weights))(*weights)
+        y = (C.c_void_p * len(ys))(*[_ptr(t) for t in ys])
+        return self._bound(self.lib.fm_proj_forward, C.c_int(len(weights)), w, C.c_int(n), _ptr(x), y, keep=(list(weights), x, list(ys)))
+
+    def proj_forward(self, weights, n, x, ys):
+        self.prepared_proj_forward(weights, n, x, ys)()
+
+    def prepared_moe_route(self, rc, n, logits, bias, expert_ids, weights):
+        return self._bound(self.lib.fm_moe_route, C.byref(rc), C.c_int(n), _ptr(logits), _ptr(bias), _ptr(expert_ids), _ptr(weights),
+                           keep=(rc, logits, bias, expert_ids, weights))
+
+    def moe_route(self, rc, n, logits, bias, expert_ids, weights):
+        self.prepared_moe_route(rc, n, logits, bias, expert_ids, weights)()
+
+    def prepared_moe_experts(self, w, n, top_k, x, expert_ids, weights, residual, norm_w, h_out, h_norm):
+        return self._bound(self.lib.fm_moe_experts, C.byref(w), C.c_int(n), C.c_int(top_k), _ptr(x), _ptr(expert_ids), _ptr(weights),
+                           _ptr(residual), _ptr(norm_w), _ptr(h_out), _ptr(h_norm),
+                           keep=(w, x, expert_ids, weights, residual, norm_w, h_out, h_norm))
+
+    def moe_experts(self, w, n, top_k, x, expert_ids, weights, residual, norm_w, h_out, h_norm):
+        self.prepared_moe_experts(w, n, top_k, x, expert_ids, weights, residual, norm_w, h_out, h_norm)()
 
     def state_export(self, li, seq, conv, ssm):
         self._check(self.lib.fm_state_export(self.h, C.c_int(li), C.c_int(seq), _ptr(conv), _ptr(ssm)))

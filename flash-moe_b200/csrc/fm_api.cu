@@ -270,6 +270,8 @@ extern "C" void fm_destroy(FmCtx *ctx) {
     cudaFree(ctx->d_h2o_accum); cudaFree(ctx->d_h2o_order); cudaFree(ctx->d_h2o_tokpos); cudaFree(ctx->d_h2o_slot);
     cudaFree(ctx->d_h2o_counter); cudaFree(ctx->d_h2o_ml); cudaFree(ctx->d_h2o_w); cudaFree(ctx->d_h2o_mref); cudaFree(ctx->d_h2o_cand);
     cudaFree(ctx->d_proj_ssq);
+    cudaFree(ctx->d_moe_ws);
+    for (int i = 0; i < ctx->moe_ws_nold; i++) cudaFree(ctx->moe_ws_old[i]);
     cudaFree(ctx->d_gdn_scratch);
     cudaFree(ctx->d_stage);
     cudaFree(ctx->d_lstage);
@@ -1011,6 +1013,200 @@ extern "C" fm_status fm_out_proj_norm(FmCtx *ctx, const FmProjWeights *w, int n,
         FM_CUDA(ctx, sg.pull(h_mid + t0 * out, w_mid, m * out));
         if (sg.host && h_post) memcpy(h_post + t0 * out, ctx->h_stage + w_post, m * out * 4);
     }
+    return FM_OK;
+}
+
+// ---- 4-bit projections, routing, experts -------------------------------------------------------
+// Workspace of at least `bytes`.  An outgrown block is kept until the context goes: a captured graph may hold its address.
+static fm_status moe_workspace(FmCtx *ctx, const char *fn, size_t bytes, char **out) {
+    if (bytes > ctx->moe_ws_bytes) {
+        cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+        FM_CUDA(ctx, cudaStreamIsCapturing(ctx->stream, &cs));
+        if (cs != cudaStreamCaptureStatusNone)
+            return fail(ctx, FM_ERR_CAPACITY, "%s: the workspace has to grow to %zu bytes: make one call of this size before the capture", fn, bytes);
+        bytes = std::max(bytes, ctx->moe_ws_bytes + ctx->moe_ws_bytes / 4);  // few blocks, however the sizes creep up
+        if (ctx->d_moe_ws && ctx->moe_ws_nold == 64) return fail(ctx, FM_ERR_NOMEM, "%s: the workspace has grown too often", fn);
+        char *p = nullptr;
+        const cudaError_t e = cudaMalloc(&p, bytes);
+        if (e != cudaSuccess) {
+            cudaGetLastError();
+            return fail(ctx, FM_ERR_NOMEM, "%s: %zu bytes of workspace: %s", fn, bytes, cudaGetErrorString(e));
+        }
+        if (ctx->d_moe_ws) ctx->moe_ws_old[ctx->moe_ws_nold++] = ctx->d_moe_ws;
+        ctx->d_moe_ws = p;
+        ctx->moe_ws_bytes = bytes;
+    }
+    *out = ctx->d_moe_ws;
+    return FM_OK;
+}
+struct Carver {  // pieces of a block, 256-byte aligned; base null: only counts
+    char *base;
+    size_t off = 0;
+    template <typename T>
+    T *take(size_t count) {
+        T *p = reinterpret_cast<T *>(base + off);
+        off += (count * sizeof(T) + 255) & ~(size_t)255;
+        return p;
+    }
+};
+
+static bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+extern "C" fm_status fm_proj_forward(FmCtx *ctx, int count, const FmProjWeights *w, int n, const float *x, float *const *y) {
+    if (!ctx) return FM_ERR_INVALID;
+    if (!w || !x || !y || count < 1 || count > kMaxProj) return fail(ctx, FM_ERR_INVALID, "fm_proj_forward: null argument or %d matrices (1..%d)", count, kMaxProj);
+    if (n < 0 || n > ctx->cfg.max_batch_tokens) return fail(ctx, FM_ERR_INVALID, "fm_proj_forward: n=%d exceeds max_batch_tokens=%d", n, ctx->cfg.max_batch_tokens);
+    for (int i = 0; i < count; i++) {
+        if (!w[i].w || !w[i].scales || !w[i].biases || !y[i]) return fail(ctx, FM_ERR_INVALID, "fm_proj_forward: null argument (matrix %d)", i);
+        if (w[i].format != FM_W_Q4_AFFINE || w[i].group_size != 64 || w[i].out_dim < 1 || w[i].in_dim < 64 || w[i].in_dim % 64 || w[i].in_dim > 65536)
+            return fail(ctx, FM_ERR_UNSUPPORTED, "fm_proj_forward: matrix %d: format %d, group size %d, %d x %d (in a multiple of 64 up to 65536)", i,
+                        w[i].format, w[i].group_size, w[i].out_dim, w[i].in_dim);
+        if (w[i].in_dim != w[0].in_dim) return fail(ctx, FM_ERR_INVALID, "fm_proj_forward: matrix %d reads %d inputs, matrix 0 reads %d", i, w[i].in_dim, w[0].in_dim);
+        if (!aligned16(w[i].w)) return fail(ctx, FM_ERR_INVALID, "fm_proj_forward: the words of matrix %d are not 16-byte aligned", i);
+    }
+    if (n == 0) return FM_OK;
+    FM_CUDA(ctx, cudaSetDevice(ctx->cfg.device));
+    const size_t K = (size_t)w[0].in_dim;
+    Stager sg(ctx);
+    bool ok = true;
+    Q4Params p = {};
+    p.in_dim = w[0].in_dim; p.n = n; p.top_k = 1; p.nmat = count;
+    p.x = sg.in(x, n * K, &ok);
+    size_t where[kMaxProj] = {};
+    for (int i = 0; i < count; i++) {
+        p.out[i] = sg.out(y[i], (size_t)n * w[i].out_dim, &ok, &where[i]);
+        p.mat[i] = Q4View{(const unsigned char *)w[i].w, (const unsigned char *)w[i].scales, (const unsigned char *)w[i].biases, 0, 0, w[i].out_dim};
+    }
+    if (!ok) return fail(ctx, FM_ERR_INVALID, "fm_proj_forward: staging buffer too small (raise max_batch_tokens)");
+    if (!aligned16(p.x)) return fail(ctx, FM_ERR_INVALID, "fm_proj_forward: x is not 16-byte aligned");
+    FM_CUDA(ctx, sg.push());
+    fm_status st;
+    {
+        ProfScope prof(ctx);
+        st = launched(ctx, launch_q4_stream(kProj, p, ctx->sm_count, ctx->stream), "proj_forward");
+    }
+    if (st) return st;
+    for (int i = 0; i < count; i++) FM_CUDA(ctx, sg.pull(y[i], where[i], (size_t)n * w[i].out_dim));
+    return FM_OK;
+}
+
+extern "C" void fm_default_route_config(FmRouteConfig *rc) {
+    memset(rc, 0, sizeof *rc);
+    rc->num_experts = 512; rc->top_k = 10; rc->score = FM_SCORE_SOFTMAX;
+    rc->num_groups = 1; rc->top_groups = 1; rc->group_best = 1;
+    rc->renormalize = 1; rc->scale = 1.0f;
+}
+
+extern "C" fm_status fm_moe_route(FmCtx *ctx, const FmRouteConfig *rc, int n, const float *logits, const float *bias, int *expert_ids,
+                                  float *weights) {
+    if (!ctx) return FM_ERR_INVALID;
+    if (!rc || !logits || !expert_ids || !weights) return fail(ctx, FM_ERR_INVALID, "fm_moe_route: null argument");
+    if (rc->score != FM_SCORE_SOFTMAX && rc->score != FM_SCORE_SIGMOID) return fail(ctx, FM_ERR_INVALID, "fm_moe_route: score %d", rc->score);
+    if (rc->num_experts < 1 || rc->num_experts > 1024 || rc->top_k < 1 || rc->top_k > 32 || rc->num_groups < 1 || rc->num_groups > 32)
+        return fail(ctx, FM_ERR_UNSUPPORTED, "fm_moe_route: %d experts (1..1024), top_k %d (1..32), %d groups (1..32)", rc->num_experts, rc->top_k, rc->num_groups);
+    if (rc->num_experts % rc->num_groups || rc->top_groups < 1 || rc->top_groups > rc->num_groups || rc->group_best < 1 || rc->group_best > 2 ||
+        rc->top_k > rc->num_experts / rc->num_groups * rc->top_groups || (rc->shared_expert != 0 && rc->shared_expert != 1))
+        return fail(ctx, FM_ERR_INVALID, "fm_moe_route: %d experts in %d groups, the best %d by %d experts each, top_k %d, shared_expert %d", rc->num_experts,
+                    rc->num_groups, rc->top_groups, rc->group_best, rc->top_k, rc->shared_expert);
+    if (n < 0 || n > ctx->cfg.max_batch_tokens) return fail(ctx, FM_ERR_INVALID, "fm_moe_route: n=%d exceeds max_batch_tokens=%d", n, ctx->cfg.max_batch_tokens);
+    if (n == 0) return FM_OK;
+    FM_CUDA(ctx, cudaSetDevice(ctx->cfg.device));
+    const size_t cols = (size_t)rc->num_experts + rc->shared_expert, slots = (size_t)rc->top_k + rc->shared_expert;
+    Stager sg(ctx);
+    bool ok = true;
+    size_t w_ids = 0, w_w = 0;
+    RouteParams p = {};
+    p.logits = sg.in(logits, n * cols, &ok);
+    p.bias = sg.in(bias, (size_t)rc->num_experts, &ok);
+    p.ids = sg.out(expert_ids, n * slots, &ok, &w_ids);
+    p.weights = sg.out(weights, n * slots, &ok, &w_w);
+    if (!ok) return fail(ctx, FM_ERR_INVALID, "fm_moe_route: staging buffer too small (raise max_batch_tokens)");
+    p.n = n; p.experts = rc->num_experts; p.top_k = rc->top_k; p.score = rc->score; p.groups = rc->num_groups; p.top_groups = rc->top_groups;
+    p.group_best = rc->group_best; p.renormalize = rc->renormalize; p.shared = rc->shared_expert; p.scale = rc->scale;
+    FM_CUDA(ctx, sg.push());
+    fm_status st = launched(ctx, launch_moe_route(p, ctx->stream), "moe_route");
+    if (st) return st;
+    FM_CUDA(ctx, sg.pull(expert_ids, w_ids, n * slots));
+    FM_CUDA(ctx, sg.pull(weights, w_w, n * slots));
+    return FM_OK;
+}
+
+extern "C" fm_status fm_moe_experts(FmCtx *ctx, const FmExpertWeights *w, int n, int top_k, const float *x, const int *expert_ids,
+                                    const float *weights, const float *residual, const uint16_t *norm_w, float *h_out, float *h_norm) {
+    if (!ctx) return FM_ERR_INVALID;
+    if (!w || !w->gate_w || !w->gate_scales || !w->gate_biases || !w->up_w || !w->up_scales || !w->up_biases || !w->down_w || !w->down_scales ||
+        !w->down_biases || !x || !expert_ids || !weights || !h_out)
+        return fail(ctx, FM_ERR_INVALID, "fm_moe_experts: null argument");
+    if (w->format != FM_W_Q4_AFFINE || w->group_size != 64 || w->hidden < 64 || w->hidden % 64 || w->hidden > 65536 || w->inter < 64 || w->inter % 64 ||
+        w->inter > 65536 || w->num_experts < 1 || w->num_experts > 1024 || top_k < 1 || top_k > 32)
+        return fail(ctx, FM_ERR_UNSUPPORTED, "fm_moe_experts: format %d, group size %d, %d experts (1..1024) of %d x %d (multiples of 64 up to 65536), top_k %d (1..32)",
+                    w->format, w->group_size, w->num_experts, w->hidden, w->inter, top_k);
+    if (w->first_expert < 0 || w->expert_stride < 0 || w->expert_stride % 16)
+        return fail(ctx, FM_ERR_INVALID, "fm_moe_experts: first_expert %d, expert_stride %lld (0 or a multiple of 16)", w->first_expert, (long long)w->expert_stride);
+    if (n < 0 || n > ctx->cfg.max_batch_tokens) return fail(ctx, FM_ERR_INVALID, "fm_moe_experts: n=%d exceeds max_batch_tokens=%d", n, ctx->cfg.max_batch_tokens);
+    if (!aligned16(w->gate_w) || !aligned16(w->up_w) || !aligned16(w->down_w)) return fail(ctx, FM_ERR_INVALID, "fm_moe_experts: weight words are not 16-byte aligned");
+    if ((long long)n * top_k > (1 << 24)) return fail(ctx, FM_ERR_UNSUPPORTED, "fm_moe_experts: %d tokens with %d slots each", n, top_k);
+    if (n == 0) return FM_OK;
+    FM_CUDA(ctx, cudaSetDevice(ctx->cfg.device));
+    const size_t H = (size_t)w->hidden, I = (size_t)w->inter, pairs = (size_t)n * top_k;
+    Stager sg(ctx);
+    bool ok = true;
+    size_t w_out = 0, w_norm = 0;
+    const float *d_x = sg.in(x, n * H, &ok);
+    const int *d_ids = sg.in(expert_ids, pairs, &ok);
+    const float *d_w = sg.in(weights, pairs, &ok), *d_res = sg.in(residual, n * H, &ok);
+    const uint16_t *d_nw = sg.in(h_norm ? norm_w : nullptr, H, &ok);
+    float *d_out = sg.out(h_out, n * H, &ok, &w_out), *d_norm = sg.out(h_norm, n * H, &ok, &w_norm);
+    if (!ok) return fail(ctx, FM_ERR_INVALID, "fm_moe_experts: staging buffer too small (raise max_batch_tokens)");
+    if (!aligned16(d_x) || !aligned16(d_res) || !aligned16(d_out) || !aligned16(d_norm) || ((uintptr_t)d_nw & 7))
+        return fail(ctx, FM_ERR_INVALID, "fm_moe_experts: x, residual, h_out and h_norm have to be 16-byte aligned, norm_w 8-byte");
+
+    MoePlan plan = {};
+    float *hbuf = nullptr, *ybuf = nullptr;
+    auto carve = [&](Carver cv) {
+        plan.njobs = cv.take<int>(1);
+        plan.jobs = cv.take<int4>(pairs);
+        plan.pair_of = cv.take<int>(pairs);
+        hbuf = cv.take<float>(pairs * I);
+        ybuf = cv.take<float>(pairs * H);
+        return cv.off;
+    };
+    char *ws = nullptr;
+    fm_status st = moe_workspace(ctx, "fm_moe_experts", carve(Carver{nullptr}), &ws);
+    if (st) return st;
+    carve(Carver{ws});
+    FM_CUDA(ctx, sg.push());
+
+    auto view = [&](const uint32_t *words, const uint16_t *s, const uint16_t *b, size_t rows, size_t cols) {
+        return Q4View{(const unsigned char *)words, (const unsigned char *)s, (const unsigned char *)b,
+                      w->expert_stride ? (long long)w->expert_stride : (long long)(rows * cols / 2), w->expert_stride ? (long long)w->expert_stride : (long long)(rows * cols / 32), (int)rows};
+    };
+    Q4Params gu = {}, dn = {};
+    gu.n = dn.n = n; gu.top_k = dn.top_k = top_k;
+    gu.first_expert = dn.first_expert = w->first_expert; gu.num_experts = dn.num_experts = w->num_experts;
+    gu.ids = dn.ids = d_ids;
+    gu.in_dim = w->hidden; gu.x = d_x; gu.nmat = 2; gu.out[0] = hbuf;
+    gu.mat[0] = view(w->gate_w, w->gate_scales, w->gate_biases, I, H);
+    gu.mat[1] = view(w->up_w, w->up_scales, w->up_biases, I, H);
+    dn.in_dim = w->inter; dn.x = hbuf; dn.nmat = 1; dn.out[0] = ybuf;
+    dn.mat[0] = view(w->down_w, w->down_scales, w->down_biases, H, I);
+    if (pairs > 16) {  // fewer: one job per pair, straight from the ids
+        st = launched(ctx, launch_moe_plan(d_ids, (int)pairs, w->first_expert, w->num_experts, 4, plan, ctx->stream), "moe_plan");
+        if (st) return st;
+        gu.plan = dn.plan = plan;
+    }
+    {
+        ProfScope prof(ctx);
+        st = launched(ctx, launch_q4_stream(kGateUp, gu, ctx->sm_count, ctx->stream), "moe gate_up");
+        if (st) return st;
+        st = launched(ctx, launch_q4_stream(kDown, dn, ctx->sm_count, ctx->stream), "moe down");
+    }
+    if (st) return st;
+    st = launched(ctx, launch_moe_combine(ybuf, d_ids, d_w, n, top_k, w->first_expert, w->num_experts, w->hidden, d_res, d_nw, ctx->cfg.rms_norm_eps, d_out,
+                                          d_norm, ctx->stream), "moe_combine");
+    if (st) return st;
+    FM_CUDA(ctx, sg.pull(h_out, w_out, n * H));
+    FM_CUDA(ctx, sg.pull(h_norm, w_norm, n * H));
     return FM_OK;
 }
 

@@ -180,6 +180,13 @@ struct FmCtx {
     float *d_proj_ssq = nullptr;  // per-token sums of squares of the output projection's epilogue, two sets used alternately
     int proj_parity = 0;
 
+    // workspace of the 4-bit products and the experts, grown on demand; outgrown blocks live until the context goes, so
+    // that a captured graph that holds their addresses stays valid
+    char *d_moe_ws = nullptr;
+    size_t moe_ws_bytes = 0;
+    void *moe_ws_old[64] = {};
+    int moe_ws_nold = 0;
+
     // cross-GPU exchange of partial results (fm_exchange_attach)
     fm::XchgView xchg = {};
     uint32_t xchg_step = 0;
@@ -267,6 +274,55 @@ int launch_out_proj_q4(const uint32_t *w, const uint16_t *scales, const uint16_t
                        const float *residual, const uint16_t *norm_w, float eps, float *h_mid, float *h_post, float *ssq, int *parity,
                        cudaStream_t st);
 
+// Routing (moe_route.cu): one launch, a warp per token.
+struct RouteParams {
+    const float *logits;  // [n][experts + shared]
+    const float *bias;    // [experts] or null
+    int *ids;             // [n][top_k + shared]
+    float *weights;
+    int n, experts, top_k, score, groups, top_groups, group_best, renormalize, shared;
+    float scale;
+};
+int launch_moe_route(const RouteParams &p, cudaStream_t st);
+
+// A stack of 4-bit affine matrices as a kernel sees it: matrix e at the base pointers + e * stride bytes.
+struct Q4View {
+    const unsigned char *w, *scales, *biases;  // words, bf16 scales, bf16 biases of matrix 0
+    long long w_stride, s_stride;              // bytes between consecutive matrices
+    int rows;                                  // outputs
+};
+
+// What the products of one call work on.
+//   kProj    y_i = W_i x for up to kMaxProj matrices that share x
+//   kGateUp  h[pair] = silu(gate_e x[token]) * (up_e x[token])
+//   kDown    y[pair] = down_e h[pair]
+// pair p = token * top_k + slot; a job is a run of pairs of one expert, pair_of[] their numbers, sorted by expert.
+enum Q4Mode { kProj = 0, kGateUp = 1, kDown = 2 };
+constexpr int kMaxProj = 8;
+struct MoePlan {        // device memory, written by moe_plan_kernel
+    int *njobs;         // [1]
+    int4 *jobs;         // (expert, first position in pair_of, pairs, -)
+    int *pair_of;       // [n * top_k]
+};
+struct Q4Params {
+    int in_dim;             // K, a multiple of 64
+    const float *x;         // kProj [n][K], kGateUp [n][K], kDown [n * top_k][K] by pair number
+    int nmat;               // kProj: matrices; experts: 1 (kDown) or 2 (kGateUp: gate, up)
+    Q4View mat[kMaxProj];
+    float *out[kMaxProj];   // kProj [n][rows_i]; experts: out[0] [n * top_k][rows] by pair number
+    int n, top_k;           // tokens, slots per token (kProj: 1)
+    int first_expert, num_experts;
+    const int *ids;         // [n][top_k]
+    MoePlan plan;           // njobs null: one job per pair, read from ids directly
+};
+// Few tokens per matrix: the weights stream past the activations once per job of up to 2 * ntl tokens (q4_stream.cu).
+int launch_q4_stream(Q4Mode mode, const Q4Params &p, int sm_count, cudaStream_t st);
+// Which pairs go to which expert, in runs of `tile` (moe_plan.cu)
+int launch_moe_plan(const int *ids, int pairs, int first_expert, int num_experts, int tile, const MoePlan &plan, cudaStream_t st);
+// h = residual + sum over the slots of weight * y[pair]; h_norm = rms-norm(h) * norm_w (moe_plan.cu)
+int launch_moe_combine(const float *y, const int *ids, const float *weights, int n, int top_k, int first_expert, int num_experts, int hidden,
+                       const float *residual, const uint16_t *norm_w, float eps, float *h_out, float *h_norm, cudaStream_t st);
+
 struct PrefillWork {
     void *q16, *k16, *v16;
     int *err;
@@ -299,6 +355,19 @@ int launch_gdn_prefill(const GdnDims &g, int n, int chunk, int step0, float *con
                        const uint16_t *norm_w, float *out, void *work, size_t work_bytes, int *err,
                        cudaStream_t st);
 size_t gdn_prefill_work_bytes(const GdnDims &g, int max_tokens, int chunk);
+
+// Launch as a programmatic dependent of whatever precedes it in the stream: the kernel waits (griddepcontrol.wait)
+// before it touches memory, so only its start-up overlaps the previous kernel's tail.
+template <typename... P, typename... A>
+inline cudaError_t launch_dependent(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A &&...args) {
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = grid; lc.blockDim = block; lc.dynamicSmemBytes = smem; lc.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    lc.attrs = at; lc.numAttrs = 1;
+    return cudaLaunchKernelEx(&lc, kernel, static_cast<P>(args)...);
+}
 
 // True the first time it is called for the current device with a given per-call-site flag word: function
 // attributes (dynamic shared memory limits) are per device, and one process may hold contexts on several.

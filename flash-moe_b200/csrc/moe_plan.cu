@@ -1,0 +1,135 @@
+// Around the experts' products: which pairs (token, slot) go to which expert, and the weighted sum behind them.
+#include <math.h>
+
+#include "fm_device.cuh"
+#include "fm_internal.h"
+
+namespace fm {
+
+namespace {
+
+constexpr int kPlanThreads = 1024;  // one thread per expert in the scan: at most 1024 experts held
+
+// inclusive sums of two counts over the block
+__device__ __forceinline__ void block_scan2(int &a, int &b, int *s_a, int *s_b) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, b, o);
+        if (lane >= o) { a += x; b += y; }
+    }
+    if (lane == 31) { s_a[warp] = a; s_b[warp] = b; }
+    __syncthreads();
+    if (warp == 0) {
+        int x = s_a[lane], y = s_b[lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, x, o), v = __shfl_up_sync(0xffffffffu, y, o);
+            if (lane >= o) { x += u; y += v; }
+        }
+        s_a[lane] = x; s_b[lane] = y;
+    }
+    __syncthreads();
+    if (warp > 0) { a += s_a[warp - 1]; b += s_b[warp - 1]; }
+}
+
+// A counting sort of the pairs by expert, in one CTA.  Within an expert the order is that of the atomics and changes from
+// run to run; nothing depends on it, since a pair's products do not depend on its neighbours.
+__global__ void __launch_bounds__(kPlanThreads)
+moe_plan_kernel(const int *__restrict__ ids, int pairs, int first_expert, int num_experts, int tile, MoePlan plan) {
+    __shared__ int s_count[kPlanThreads], s_a[32], s_b[32];
+    const int tid = threadIdx.x;
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    s_count[tid] = 0;
+    __syncthreads();
+    for (int p = tid; p < pairs; p += kPlanThreads) {
+        const int e = __ldg(ids + p) - first_expert;
+        if (e >= 0 && e < num_experts) atomicAdd(s_count + e, 1);
+    }
+    __syncthreads();
+    const int count = s_count[tid], tiles = (count + tile - 1) / tile;
+    int end = count, tend = tiles;
+    block_scan2(end, tend, s_a, s_b);
+    const int start = end - count, tstart = tend - tiles;
+    s_count[tid] = start;  // from here on the next free position
+    for (int i = 0; i < tiles; i++) plan.jobs[tstart + i] = make_int4(tid, start + i * tile, min(tile, count - i * tile), 0);
+    if (tid == kPlanThreads - 1) *plan.njobs = tend;
+    __syncthreads();
+    for (int p = tid; p < pairs; p += kPlanThreads) {
+        const int e = __ldg(ids + p) - first_expert;
+        if (e >= 0 && e < num_experts) plan.pair_of[atomicAdd(s_count + e, 1)] = p;
+    }
+}
+
+// One CTA per token.  The slots are summed in their order, so the result does not depend on the launch.
+__global__ void __launch_bounds__(256)
+moe_combine_kernel(const float *__restrict__ y, const int *__restrict__ ids, const float *__restrict__ weights, int top_k, int first_expert,
+                   int num_experts, int hidden, const float *residual, const uint16_t *__restrict__ norm_w, float eps, float *h_out, float *h_norm) {
+    __shared__ float s_w[32];
+    __shared__ int s_slot[32];
+    __shared__ int s_n;
+    __shared__ float s_sq[8];
+    const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    if (warp == 0) {  // the slots that have an expert here
+        const int e = lane < top_k ? ids[(size_t)t * top_k + lane] - first_expert : -1;
+        const bool here = e >= 0 && e < num_experts;
+        const unsigned m = __ballot_sync(0xffffffffu, here);
+        if (here) {
+            const int at = __popc(m & ((1u << lane) - 1));
+            s_slot[at] = lane;
+            s_w[at] = weights[(size_t)t * top_k + lane];
+        }
+        if (lane == 0) s_n = __popc(m);
+    }
+    __syncthreads();
+    const int ns = s_n;
+    const float *yt = y + (size_t)t * top_k * hidden;
+    float sq = 0.f;
+    for (int i = tid * 4; i < hidden; i += 1024) {
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int s = 0; s < ns; s++) {
+            const float4 v = *reinterpret_cast<const float4 *>(yt + (size_t)s_slot[s] * hidden + i);
+            const float w = s_w[s];
+            a.x = fmaf(w, v.x, a.x); a.y = fmaf(w, v.y, a.y); a.z = fmaf(w, v.z, a.z); a.w = fmaf(w, v.w, a.w);
+        }
+        if (residual != nullptr) {
+            const float4 r = *reinterpret_cast<const float4 *>(residual + (size_t)t * hidden + i);
+            a.x += r.x; a.y += r.y; a.z += r.z; a.w += r.w;
+        }
+        *reinterpret_cast<float4 *>(h_out + (size_t)t * hidden + i) = a;
+        sq += (a.x * a.x + a.y * a.y) + (a.z * a.z + a.w * a.w);
+    }
+    if (h_norm == nullptr) return;
+    sq = warp_sum(sq);
+    if (lane == 0) s_sq[warp] = sq;
+    __syncthreads();
+    float tot = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; w++) tot += s_sq[w];
+    const float inv = 1.0f / sqrtf(tot / hidden + eps);
+    for (int i = tid * 4; i < hidden; i += 1024) {
+        const float4 h = *reinterpret_cast<const float4 *>(h_out + (size_t)t * hidden + i);
+        uint2 wb = make_uint2(0x3f803f80u, 0x3f803f80u);
+        if (norm_w != nullptr) wb = __ldg(reinterpret_cast<const uint2 *>(norm_w + i));
+        *reinterpret_cast<float4 *>(h_norm + (size_t)t * hidden + i) =
+            make_float4(h.x * inv * __uint_as_float(wb.x << 16), h.y * inv * __uint_as_float(wb.x & 0xffff0000u),
+                        h.z * inv * __uint_as_float(wb.y << 16), h.w * inv * __uint_as_float(wb.y & 0xffff0000u));
+    }
+}
+
+}  // namespace
+
+int launch_moe_plan(const int *ids, int pairs, int first_expert, int num_experts, int tile, const MoePlan &plan, cudaStream_t st) {
+    return launch_dependent(moe_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, ids, pairs, first_expert, num_experts, tile, plan) == cudaSuccess ? 1 : -1;
+}
+
+int launch_moe_combine(const float *y, const int *ids, const float *weights, int n, int top_k, int first_expert, int num_experts, int hidden,
+                       const float *residual, const uint16_t *norm_w, float eps, float *h_out, float *h_norm, cudaStream_t st) {
+    return launch_dependent(moe_combine_kernel, dim3(n), dim3(256), 0, st, y, ids, weights, top_k, first_expert, num_experts, hidden, residual, norm_w, eps,
+                            h_out, h_norm) == cudaSuccess ? 1 : -1;
+}
+
+}  // namespace fm

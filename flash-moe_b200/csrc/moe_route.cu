@@ -1,0 +1,288 @@
+// Routing of tokens to experts: scores, balance bias, groups, top-k, renormalised weights.
+//
+// Reference: cpu_softmax over the gate's logits, cpu_topk and the renormalisation of the selected weights between the
+// post-attention norm and the experts of fused_layer_forward (metal_infer/layer_forward.h, metal_infer/cpu_kernels.h).
+// Per token, over E logits x (include/fm_attn.h has the contract):
+//     s_e = softmax(x)_e or 1 / (1 + exp(-x_e));   c_e = s_e + bias_e
+//     groups: G runs of E / G experts; a group counts with the sum of its one or two best c; the best ones survive
+//     ids = the top_k largest c, ties to the lowest index;   w = s, divided by the selected ones' sum, times a factor
+//
+// One warp per token, expert j * 32 + lane in register j: the row is read once, coalesced, and nothing leaves the
+// registers.  Selection works on order-preserving 32-bit keys, one redux for the value and one for the lowest index that
+// holds it; a slot's result stays in the lane of its number.  What bounds it is that chain (two redux and a pass over
+// the lane's keys per slot), not the bytes.
+//
+// Borders.  Which expert is the k-th best is a whole number, so a rounding must not decide it.  Softmax without a bias
+// is ordered by the logits themselves (exact).  Otherwise the 32-bit choices carry an error of a few units in the last
+// place; where two neighbours in the order, or two groups at the border, are nearer than a bound on that error, the warp
+// takes the row again in 64 bits (rare: about one row in a thousand of random logits).
+#include <math.h>
+
+#include "fm_device.cuh"
+#include "fm_internal.h"
+
+namespace fm {
+
+namespace {
+
+constexpr int kRtWarps = 4;
+constexpr unsigned kFull = 0xffffffffu;
+
+// order-preserving map of non-NaN floats to unsigned; 0 is below every value (it stands for "not available")
+__device__ __forceinline__ uint32_t key_of(float f) {
+    const uint32_t u = __float_as_uint(f);
+    return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k); }
+
+__device__ __forceinline__ double warp_max_d(double v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmax(v, __shfl_xor_sync(kFull, v, o));
+    return v;
+}
+
+// Lane g holds group g's total; returns the bit mask of the `top` best groups (ties: lowest index).  *border: the last
+// total kept; *gap: its distance from the first one dropped.
+template <typename T>
+__device__ uint32_t best_groups(T total, int groups, int top, int lane, T *gap, T *border) {
+    int rank = 0;
+    T last = -INFINITY, next = -INFINITY;
+    for (int g = 0; g < groups; g++) {
+        const T o = __shfl_sync(kFull, total, g);
+        rank += (o > total || (o == total && g < lane)) ? 1 : 0;
+    }
+    const uint32_t keep = __ballot_sync(kFull, lane < groups && rank < top);
+    const uint32_t at_last = __ballot_sync(kFull, lane < groups && rank == top - 1), at_next = __ballot_sync(kFull, lane < groups && rank == top);
+    if (at_last) last = __shfl_sync(kFull, total, __ffs(at_last) - 1);
+    if (at_next) next = __shfl_sync(kFull, total, __ffs(at_next) - 1);
+    *border = last;
+    *gap = next == -INFINITY ? (T)INFINITY : last - next;
+    return keep;
+}
+
+// The same row in 64 bits, taken where 32 cannot tell neighbours apart.  Returns the lane's slot's expert (-1: none).
+template <int VPL>
+__device__ __noinline__ int select_in_double(const RouteParams &p, const float *row, int lane) {
+    double c[VPL];
+    double m = -INFINITY, sum = 0.0;
+    for (int j = 0; j < VPL; j++) {
+        const int e = j * 32 + lane;
+        const float x = e < p.experts ? row[e] : -INFINITY;
+        const float b = p.bias != nullptr && e < p.experts ? p.bias[e] : 0.f;
+        c[j] = (x > -INFINITY && b > -INFINITY) ? (double)x : -INFINITY;
+        m = fmax(m, c[j]);
+    }
+    m = warp_max_d(m);
+    for (int j = 0; j < VPL; j++) {
+        if (c[j] == -INFINITY) continue;
+        c[j] = p.score == FM_SCORE_SOFTMAX ? (c[j] == m ? 1.0 : exp(c[j] - m)) : 1.0 / (1.0 + exp(-c[j]));
+        sum += c[j];
+    }
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+    for (int j = 0; j < VPL; j++) {
+        if (c[j] == -INFINITY) continue;
+        if (p.score == FM_SCORE_SOFTMAX) c[j] /= sum;
+        if (p.bias != nullptr) c[j] += (double)p.bias[j * 32 + lane];
+    }
+    if (p.groups > 1) {
+        const int size = p.experts / p.groups;
+        double mine = -INFINITY;
+        for (int g = 0; g < p.groups; g++) {
+            double m1 = -INFINITY, m2 = -INFINITY;
+            for (int j = 0; j < VPL; j++) {
+                if ((j * 32 + lane) / size != g) continue;
+                if (c[j] > m1) { m2 = m1; m1 = c[j]; } else if (c[j] > m2) m2 = c[j];
+            }
+            const double a = warp_max_d(m1);
+            double t = a;
+            if (p.group_best == 2) {
+                const uint32_t at = __ballot_sync(kFull, m1 == a);
+                const double b = __popc(at) > 1 ? a : warp_max_d(m1 == a ? m2 : m1);
+                if (b > -INFINITY) t += b;
+            }
+            if (lane == g) mine = t;
+        }
+        double gap, border;
+        const uint32_t keep = best_groups<double>(mine, p.groups, p.top_groups, lane, &gap, &border);
+        for (int j = 0; j < VPL; j++)
+            if (j * 32 + lane < p.experts && !((keep >> ((j * 32 + lane) / size)) & 1)) c[j] = -INFINITY;
+        if (p.score == FM_SCORE_SOFTMAX && p.bias == nullptr)  // within the groups the logits decide, as in the kernel
+            for (int j = 0; j < VPL; j++)
+                if (c[j] > -INFINITY) c[j] = (double)row[j * 32 + lane];
+    }
+    int id = -1;
+    for (int s = 0; s < p.top_k; s++) {
+        double best = -INFINITY;
+        for (int j = 0; j < VPL; j++) best = fmax(best, c[j]);
+        best = warp_max_d(best);
+        if (best == -INFINITY) break;
+        int at = 0x7fffffff;
+        for (int j = VPL - 1; j >= 0; j--)
+            if (c[j] == best) at = j * 32 + lane;
+        at = __reduce_min_sync(kFull, at);
+        for (int j = 0; j < VPL; j++)
+            if (j * 32 + lane == at) c[j] = -INFINITY;
+        if (lane == s) id = at;
+    }
+    return id;
+}
+
+template <int VPL>
+__global__ void __launch_bounds__(32 * kRtWarps)
+moe_route_kernel(RouteParams p) {
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    const int lane = threadIdx.x & 31, t = blockIdx.x * kRtWarps + (threadIdx.x >> 5);
+    if (t >= p.n) return;
+    const float *row = p.logits + (size_t)t * (p.experts + p.shared);
+    const bool softmax = p.score == FM_SCORE_SOFTMAX;
+
+    // logits; -inf where the expert cannot be chosen (its logit or bias is NaN or -inf)
+    float x[VPL];
+    float m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < VPL; j++) {
+        const int e = j * 32 + lane;
+        x[j] = e < p.experts ? __ldg(row + e) : -INFINITY;
+        if (!(x[j] > -INFINITY)) x[j] = -INFINITY;
+        if (p.bias != nullptr && e < p.experts && !(__ldg(p.bias + e) > -INFINITY)) x[j] = -INFINITY;
+        m = fmaxf(m, x[j]);
+    }
+    m = warp_max(m);
+    // scores' denominator (softmax); +inf logits share the weight equally
+    float sum = 0.f, inv = 0.f;
+    const bool by_logit = softmax && p.bias == nullptr;  // order of the logits = order of the scores, without rounding
+    uint32_t key[VPL];
+    float top_score = 0.f;
+#pragma unroll
+    for (int j = 0; j < VPL; j++) {
+        float s = 0.f;
+        if (x[j] > -INFINITY) s = softmax ? (x[j] == m ? 1.f : expf(x[j] - m)) : 1.f / (1.f + expf(-x[j]));
+        sum += s;
+        key[j] = by_logit ? (x[j] > -INFINITY ? key_of(x[j]) : 0u) : __float_as_uint(s);  // scores for now: the choice follows below
+        top_score = fmaxf(top_score, s);
+    }
+    if (softmax) {
+        sum = warp_sum(sum);
+        inv = sum > 0.f ? 1.f / sum : 0.f;
+    }
+    if (!by_logit) {
+        top_score = warp_max(top_score) * (softmax ? inv : 1.f);
+#pragma unroll
+        for (int j = 0; j < VPL; j++) {
+            const float s = __uint_as_float(key[j]) * (softmax ? inv : 1.f);
+            key[j] = x[j] > -INFINITY ? key_of(p.bias != nullptr ? s + __ldg(p.bias + j * 32 + lane) : s) : 0u;
+        }
+    }
+    // error bound of a choice: the score's (softmax: the exponent's rounding grows with its size) and the sum's
+    const float tol_score = (softmax ? 8e-6f : 1e-6f) * top_score;
+    bool unsure = false;
+
+    if (p.groups > 1) {
+        const int size = p.experts / p.groups;
+        float mine = -INFINITY;
+        for (int g = 0; g < p.groups; g++) {
+            uint32_t m1 = 0, m2 = 0;
+#pragma unroll
+            for (int j = 0; j < VPL; j++) {
+                if (j * 32 + 31 < g * size || j * 32 >= (g + 1) * size) continue;  // uniform: no expert of the group in register j
+                const int e = j * 32 + lane;
+                const uint32_t k = e >= g * size && e < (g + 1) * size ? key[j] : 0u;
+                m2 = max(m2, min(m1, k));
+                m1 = max(m1, k);
+            }
+            const uint32_t a = __reduce_max_sync(kFull, m1);
+            float total = -INFINITY;
+            if (a != 0u) {
+                // by_logit: the group's best scores are those of its best logits
+                const float va = value_of(a);
+                total = by_logit ? (va == m ? 1.f : expf(va - m)) * inv : va;
+                if (by_logit && p.group_best == 1) total = va;  // one best: compare the logits themselves
+                if (p.group_best == 2) {
+                    const uint32_t at = __ballot_sync(kFull, m1 == a);
+                    const uint32_t b = __popc(at) > 1 ? a : __reduce_max_sync(kFull, m1 == a ? m2 : m1);
+                    if (b != 0u) {
+                        const float vb = value_of(b);
+                        total += by_logit ? (vb == m ? 1.f : expf(vb - m)) * inv : vb;
+                    }
+                }
+            }
+            if (lane == g) mine = total;
+        }
+        float gap, border;
+        const uint32_t keep = best_groups<float>(mine, p.groups, p.top_groups, lane, &gap, &border);
+        if (!(by_logit && p.group_best == 1))
+            unsure = !(gap > (by_logit ? 1.6e-5f * border : 4.f * tol_score + 4.8e-7f * fabsf(border)));
+#pragma unroll
+        for (int j = 0; j < VPL; j++) {
+            const int e = j * 32 + lane;
+            if (e < p.experts && !((keep >> (e / size)) & 1)) key[j] = 0u;
+        }
+    }
+
+    int id = -1;
+    uint32_t prev = 0;
+    const int rounds = p.top_k + (by_logit ? 0 : 1);  // one more than asked for: the border needs its other side
+    for (int s = 0; s < rounds; s++) {
+        uint32_t best = 0;
+#pragma unroll
+        for (int j = 0; j < VPL; j++) best = max(best, key[j]);
+        best = __reduce_max_sync(kFull, best);
+        if (best == 0u) break;
+        int at = 0x7fffffff;
+#pragma unroll
+        for (int j = VPL - 1; j >= 0; j--)
+            if (key[j] == best) at = j * 32 + lane;
+        at = __reduce_min_sync(kFull, at);
+#pragma unroll
+        for (int j = 0; j < VPL; j++)
+            if (j * 32 + lane == at) key[j] = 0u;
+        if (s < p.top_k && lane == s) id = at;
+        if (!by_logit) {
+            const float v = value_of(best);
+            if (s > 0 && !(value_of(prev) - v > 2.f * tol_score + 2.4e-7f * fabsf(v))) unsure = true;
+            prev = best;
+        }
+    }
+    if (unsure) id = select_in_double<VPL>(p, row, lane);
+
+    const int slots = p.top_k + p.shared;
+    const float v = id >= 0 ? __ldg(row + id) : -INFINITY;
+    float w = 0.f;
+    if (!p.renormalize) {
+        if (id >= 0) w = softmax ? (v == m ? 1.f : expf(v - m)) * inv : 1.f / (1.f + expf(-v));
+    } else {
+        // a common factor drops out: the scores relative to the largest selected one, so that small ones do not underflow
+        const float vm = warp_max(v);
+        if (id >= 0) {
+            const float rel = v == vm ? 1.f : expf(v - vm);
+            w = softmax ? rel : vm > 0.f ? 1.f / (1.f + expf(-v)) : rel / (1.f + expf(v));
+        }
+        const float tot = warp_sum(w);
+        w = tot > 0.f ? w / tot : 0.f;
+    }
+    if (lane < p.top_k) {
+        p.ids[(size_t)t * slots + lane] = id;
+        p.weights[(size_t)t * slots + lane] = w * p.scale;
+    }
+    if (p.shared && lane == 0) {
+        p.ids[(size_t)t * slots + p.top_k] = p.experts;
+        p.weights[(size_t)t * slots + p.top_k] = 1.f / (1.f + expf(-__ldg(row + p.experts)));
+    }
+}
+
+}  // namespace
+
+int launch_moe_route(const RouteParams &p, cudaStream_t st) {
+    const dim3 grid((p.n + kRtWarps - 1) / kRtWarps), block(32 * kRtWarps);
+    cudaError_t e;
+    if (p.experts <= 32) e = launch_dependent(moe_route_kernel<1>, grid, block, 0, st, p);
+    else if (p.experts <= 64) e = launch_dependent(moe_route_kernel<2>, grid, block, 0, st, p);
+    else if (p.experts <= 128) e = launch_dependent(moe_route_kernel<4>, grid, block, 0, st, p);
+    else if (p.experts <= 256) e = launch_dependent(moe_route_kernel<8>, grid, block, 0, st, p);
+    else if (p.experts <= 512) e = launch_dependent(moe_route_kernel<16>, grid, block, 0, st, p);
+    else e = launch_dependent(moe_route_kernel<32>, grid, block, 0, st, p);
+    return e == cudaSuccess ? 1 : -1;
+}
+
+}  // namespace fm

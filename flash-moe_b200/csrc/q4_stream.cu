@@ -1,0 +1,318 @@
+// Products of 4-bit affine matrices with a few tokens each: projections at decode, and the routed experts while an
+// expert sees a handful of tokens.
+//
+// Reference: cpu_dequant_matvec (metal_infer/cpu_kernels.h:199-232; Metal dequant_matvec_4bit*), batched over matrices
+// that share their input by gpu_encode_batch_matvec (metal_infer/gpu_dispatch.h), and the experts' gate / up / SwiGLU /
+// down chain of the same file.
+//     y[r] = sum over groups g of 64 inputs:  s[r][g] * sum_k nibble[r][k] x[k]  +  b[r][g] * X[g],   X[g] = sum_k x[k]
+//
+// Bound by the weights' stream, 0.5625 bytes per weight, and close behind it by the instructions that widen them.  So
+// the nibbles are never turned into floating point: they are multiplied as they are, unsigned bytes, on the integer
+// tensor cores (mma.sync m16n8k32, measured at twice the fp16 rate), which takes 3 instructions per word of eight.  The
+// activations are the other factor, as 32-bit fixed point relative to the largest of their group of 64, cut into four
+// signed bytes, which are four of the eight columns of the product: two tokens per instruction.  The integer sums are
+// exact; what is left of fp32's accuracy is 2^-30 of a group's largest input.  Scale and bias meet the group's sum in
+// fp32, once per row and group.
+//
+// A unit is 16 rows of one matrix pair (kGateUp: the same rows of gate and up; else 32 rows of one matrix) for one job.
+// The 8 warps of a CTA split the groups of a row among themselves and meet in shared memory at the unit's end; every
+// lane fetches 8 bytes of a row group straight into registers, several groups ahead.  CTAs are persistent and take a
+// contiguous range of units, so that a job's activations are widened once per CTA and not once per unit.
+#include <math.h>
+
+#include <algorithm>
+
+#include "fm_device.cuh"
+#include "fm_internal.h"
+
+namespace fm {
+
+namespace {
+
+constexpr int kWarps = 8;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kDepth = 4;        // weight groups a warp has in flight
+constexpr int kTiles = 2;        // 16-row tiles per unit
+constexpr int kTokBytes = 256;   // a token's group as bytes: 64 inputs x 4
+constexpr int kFactorBytes = 32; // per group and pair of tokens: (factor, input sum) for each of the four lanes of a quad
+
+__device__ __forceinline__ void mma_u8s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Row sources of a unit: where its two tiles start.
+struct Rows {
+    const unsigned char *w[kTiles], *s[kTiles], *b[kTiles];  // first row of the tile
+    int rows[kTiles];                                        // rows of the tile that exist (0..16)
+};
+
+// Eight inputs (those of one weight word) of a token -> fixed point bytes in the order of the B fragments.
+// The eight threads of a group of 64 inputs sit in consecutive lanes.
+__device__ __forceinline__ void widen8(const float *x, bool valid, unsigned char *tok_group, float2 *factor, int wi) {
+    float v[8];
+    if (valid) {
+        const float4 a = __ldg(reinterpret_cast<const float4 *>(x)), b = __ldg(reinterpret_cast<const float4 *>(x) + 1);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = 0.f;
+    }
+    float am = 0.f, sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) am = fmaxf(am, fabsf(v[i]));
+    sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+        am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, o));
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    }
+    if (!valid) return;
+    // am in [2^e, 2^(e+1)): inputs as integers of 2^(e-29), so that |q| < 2^30; groups below 2^-97 keep a fixed step.
+    // A group with an infinity or a NaN (the maximum passes NaN by, the sum does not) makes its token's results NaN.
+    int e = (int)(__float_as_uint(am) >> 23) - 127;
+    e = max(e, -97);
+    const bool bad = !(fabsf(sum) <= 3.4028235e38f) || e > 127;
+    const float up = __uint_as_float((uint32_t)(127 + 29 - e) << 23), down = bad ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)(127 - 29 + e) << 23);
+    uint32_t q[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int k = bad ? 0 : __float2int_rn(v[i] * up);
+        // four signed digits of 8 bits: adding 0x80 to the lower three bytes carries into the next, flipping their top bit
+        // takes it off again
+        q[i] = ((uint32_t)k + 0x00808080u) ^ 0x00808080u;
+    }
+    // digit planes: plane p (0 = most significant) of the even inputs and of the odd ones
+    unsigned char *o = tok_group + (wi >> 1) * 16 + (wi & 1) * 8;
+#pragma unroll
+    for (int half = 0; half < 2; half++) {
+        const uint32_t a = q[half], b = q[2 + half], c = q[4 + half], d = q[6 + half];
+        const uint32_t ab_hi = __byte_perm(a, b, 0x7362), cd_hi = __byte_perm(c, d, 0x7362);  // a2 b2 a3 b3
+        const uint32_t ab_lo = __byte_perm(a, b, 0x5140), cd_lo = __byte_perm(c, d, 0x5140);  // a0 b0 a1 b1
+        *reinterpret_cast<uint32_t *>(o + 0 * 64 + half * 4) = __byte_perm(ab_hi, cd_hi, 0x7632);  // a3 b3 c3 d3
+        *reinterpret_cast<uint32_t *>(o + 1 * 64 + half * 4) = __byte_perm(ab_hi, cd_hi, 0x5410);  // a2 b2 c2 d2
+        *reinterpret_cast<uint32_t *>(o + 2 * 64 + half * 4) = __byte_perm(ab_lo, cd_lo, 0x7632);  // a1 b1 c1 d1
+        *reinterpret_cast<uint32_t *>(o + 3 * 64 + half * 4) = __byte_perm(ab_lo, cd_lo, 0x5410);  // a0 b0 c0 d0
+    }
+    // the pair of upper digits counts 2^16, the pair of lower ones 1; the input sum goes with either (see the loop)
+    if (wi < 2) factor[wi] = make_float2(wi == 0 ? down * 65536.f : down, sum);
+}
+
+template <Q4Mode MODE, int NTL>
+__global__ void __launch_bounds__(kThreads, NTL == 4 ? 1 : 2)
+q4_stream_kernel(Q4Params p, int chunk_groups, int units_per_job, int fixed_jobs) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    constexpr int kTok = 2 * NTL;
+    unsigned char *s_b = smem;                                                                      // [NTL][2 tokens][chunk][256]
+    float2 *s_f = reinterpret_cast<float2 *>(smem + (size_t)kTok * chunk_groups * kTokBytes);       // [NTL][chunk][4]
+    float *s_red = reinterpret_cast<float *>(reinterpret_cast<unsigned char *>(s_f) + (size_t)NTL * chunk_groups * kFactorBytes);  // [2][warp][tok][32 rows]
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int G = p.in_dim / 64;
+    const size_t w_pitch = (size_t)G * 32, s_pitch = (size_t)G * 2;
+    const int nchunks = (G + chunk_groups - 1) / chunk_groups;
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    const int njobs = p.plan.njobs != nullptr ? *p.plan.njobs : fixed_jobs;
+    const long long units = (long long)njobs * units_per_job;
+    const long long u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1) / gridDim.x;
+
+    auto job_of = [&](int job, int &expert, int &start, int &cnt) {
+        if constexpr (MODE == kProj) {
+            expert = 0; start = job * kTok; cnt = min(kTok, p.n - start);
+        } else if (p.plan.njobs != nullptr) {
+            const int4 j = p.plan.jobs[job];
+            expert = j.x; start = j.y; cnt = j.z;
+        } else {
+            expert = p.ids[job] - p.first_expert; start = job; cnt = expert >= 0 && expert < p.num_experts ? 1 : 0;
+        }
+    };
+    auto pair_at = [&](int start, int i) { return MODE == kProj ? start + i : p.plan.njobs != nullptr ? p.plan.pair_of[start + i] : start; };
+    // the unit's matrix (kProj) and first row in it
+    auto where = [&](int rb, int &mat, int &row0) {
+        mat = 0;
+        if constexpr (MODE == kGateUp) {
+            row0 = rb * 16;
+        } else {
+            if constexpr (MODE == kProj)
+                while (rb >= (p.mat[mat].rows + 31) / 32) rb -= (p.mat[mat++].rows + 31) / 32;
+            row0 = rb * 32;
+        }
+    };
+    auto rows_of = [&](int expert, int mat, int row0) {
+        Rows r;
+#pragma unroll
+        for (int i = 0; i < kTiles; i++) {
+            const Q4View &m = p.mat[MODE == kGateUp ? i : mat];
+            const int first = MODE == kGateUp ? row0 : row0 + 16 * i;
+            r.rows[i] = max(0, min(16, m.rows - first));
+            const size_t at = r.rows[i] > 0 ? first : 0;
+            r.w[i] = m.w + (size_t)expert * m.w_stride + at * w_pitch;
+            r.s[i] = m.scales + (size_t)expert * m.s_stride + at * s_pitch;
+            r.b[i] = m.biases + (size_t)expert * m.s_stride + at * s_pitch;
+        }
+        return r;
+    };
+
+    uint2 wq[kDepth][kTiles][2];
+    uint32_t sc[kDepth][kTiles];  // scales of rows g | g + 8
+    uint16_t bi[kDepth][kTiles];  // bias of row g (even lanes) or g + 8 (odd lanes)
+    auto fetch = [&](const Rows &r, int grp, int slot) {
+#pragma unroll
+        for (int i = 0; i < kTiles; i++) {
+            const int l0 = min(g, max(r.rows[i] - 1, 0)), l1 = min(g + 8, max(r.rows[i] - 1, 0));  // rows without a place read the last one
+            wq[slot][i][0] = __ldg(reinterpret_cast<const uint2 *>(r.w[i] + l0 * w_pitch + (size_t)grp * 32) + t);
+            wq[slot][i][1] = __ldg(reinterpret_cast<const uint2 *>(r.w[i] + l1 * w_pitch + (size_t)grp * 32) + t);
+            sc[slot][i] = (uint32_t)__ldg(reinterpret_cast<const uint16_t *>(r.s[i] + l0 * s_pitch) + grp) |
+                          ((uint32_t)__ldg(reinterpret_cast<const uint16_t *>(r.s[i] + l1 * s_pitch) + grp) << 16);
+            bi[slot][i] = __ldg(reinterpret_cast<const uint16_t *>(r.b[i] + (t & 1 ? l1 : l0) * s_pitch) + grp);
+        }
+    };
+
+    int held_start = -1, held_job = -1;  // whose activations shared memory holds
+    int half = 0;                        // of s_red: units alternate
+    for (long long u = u0; u < u1; u++) {
+        const int job = (int)(u / units_per_job), rb = (int)(u - (long long)job * units_per_job);
+        int expert, start, cnt, mat, row0;
+        job_of(job, expert, start, cnt);
+        if (cnt == 0) continue;  // an expert of another rank, or a slot without one
+        where(rb, mat, row0);
+        const Rows r = rows_of(expert, mat, row0);
+        const int ntl = (cnt + 1) / 2;
+        float acc[kTiles][2][NTL] = {}, accb[kTiles][NTL] = {};
+        for (int c = 0; c < nchunks; c++) {
+            const int cg0 = c * chunk_groups, cgn = min(chunk_groups, G - cg0);
+            const int ga = cg0 + cgn * warp / kWarps, gb = cg0 + cgn * (warp + 1) / kWarps;  // this warp's groups
+#pragma unroll
+            for (int s = 0; s < kDepth; s++)
+                if (ga + s < gb) fetch(r, ga + s, s);
+            // activations of the job: of one token the source is the token, so consecutive single-token jobs share them
+            int source = start;
+            if (MODE == kGateUp && cnt == 1) source = pair_at(start, 0) / p.top_k;
+            const int kind = MODE == kGateUp && cnt == 1 ? -2 : job;
+            if (nchunks > 1 || kind != held_job || source != held_start) {
+                __syncthreads();  // everyone is done with the previous activations
+                const int words = cgn * 8, total = cnt * words;
+                for (int i0 = 0; i0 < total; i0 += kThreads) {
+                    const int i = i0 + tid;
+                    const bool valid = i < total;
+                    const int tok = valid ? i / words : 0, w8 = valid ? i - tok * words : 0;
+                    int row = pair_at(start, tok);
+                    if (MODE == kGateUp) row /= p.top_k;
+                    unsigned char *tb = s_b + ((size_t)tok * chunk_groups + (w8 >> 3)) * kTokBytes;
+                    float2 *f = s_f + ((size_t)(tok >> 1) * chunk_groups + (w8 >> 3)) * 4 + (tok & 1) * 2;
+                    widen8(p.x + (size_t)row * p.in_dim + (size_t)cg0 * 64 + (size_t)w8 * 8, valid, tb, f, w8 & 7);
+                }
+                held_start = source; held_job = kind;
+                __syncthreads();
+            }
+            for (int grp0 = ga; grp0 < gb; grp0 += kDepth) {
+#pragma unroll
+                for (int s = 0; s < kDepth; s++) {
+                    const int grp = grp0 + s;
+                    if (grp >= gb) break;
+                    uint32_t a[kTiles][2][4];  // nibbles as bytes: [tile][word of the lane's two][fragment register]
+                    float s0[kTiles], s1[kTiles], sb[kTiles];
+#pragma unroll
+                    for (int i = 0; i < kTiles; i++) {
+                        const uint2 w0 = wq[s][i][0], w1 = wq[s][i][1];
+                        a[i][0][0] = w0.x & 0x0F0F0F0Fu; a[i][0][1] = w1.x & 0x0F0F0F0Fu;
+                        a[i][0][2] = (w0.x >> 4) & 0x0F0F0F0Fu; a[i][0][3] = (w1.x >> 4) & 0x0F0F0F0Fu;
+                        a[i][1][0] = w0.y & 0x0F0F0F0Fu; a[i][1][1] = w1.y & 0x0F0F0F0Fu;
+                        a[i][1][2] = (w0.y >> 4) & 0x0F0F0F0Fu; a[i][1][3] = (w1.y >> 4) & 0x0F0F0F0Fu;
+                        s0[i] = __uint_as_float(sc[s][i] << 16);
+                        s1[i] = __uint_as_float(sc[s][i] & 0xffff0000u);
+                        sb[i] = __uint_as_float((uint32_t)bi[s][i] << 16);
+                    }
+                    if (grp + kDepth < gb) fetch(r, grp + kDepth, s);
+#pragma unroll
+                    for (int nt = 0; nt < NTL; nt++) {
+                        if (nt >= ntl) break;
+                        const uint4 bf = *reinterpret_cast<const uint4 *>(s_b + ((size_t)(nt * 2 + (g >> 2)) * chunk_groups + (grp - cg0)) * kTokBytes +
+                                                                          ((g & 3) * 4 + t) * 16);
+                        const float2 f = s_f[((size_t)nt * chunk_groups + (grp - cg0)) * 4 + t];
+#pragma unroll
+                        for (int i = 0; i < kTiles; i++) {
+                            int d[4] = {0, 0, 0, 0};
+                            mma_u8s8(d, a[i][0][0], a[i][0][1], a[i][0][2], a[i][0][3], bf.x, bf.y);
+                            mma_u8s8(d, a[i][1][0], a[i][1][1], a[i][1][2], a[i][1][3], bf.z, bf.w);
+                            // |d| <= 64 * 15 * 128, so two digits still fit an int; lane t holds the digit pair t & 1 of token t / 2
+                            acc[i][0][nt] = fmaf(s0[i] * f.x, (float)(d[0] * 256 + d[1]), acc[i][0][nt]);
+                            acc[i][1][nt] = fmaf(s1[i] * f.x, (float)(d[2] * 256 + d[3]), acc[i][1][nt]);
+                            accb[i][nt] = fmaf(sb[i], f.y, accb[i][nt]);
+                        }
+                    }
+                }
+            }
+        }
+        // ---- the digit pairs of a row meet, then the eight warps ----
+        float *red = s_red + (size_t)half * kWarps * kTok * 32;
+        half ^= 1;
+#pragma unroll
+        for (int i = 0; i < kTiles; i++)
+#pragma unroll
+            for (int nt = 0; nt < NTL; nt++) {
+                float v0 = acc[i][0][nt] + (t & 1 ? 0.f : accb[i][nt]), v1 = acc[i][1][nt] + (t & 1 ? accb[i][nt] : 0.f);
+                v0 += __shfl_xor_sync(0xffffffffu, v0, 1);
+                v1 += __shfl_xor_sync(0xffffffffu, v1, 1);
+                red[((size_t)warp * kTok + nt * 2 + (t >> 1)) * 32 + i * 16 + g + (t & 1) * 8] = t & 1 ? v1 : v0;
+            }
+        __syncthreads();  // (the other half of s_red is free again once everyone is here)
+        for (int e = tid; e < cnt * 32; e += kThreads) {
+            const int tok = e >> 5, row = e & 31;
+            float v = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; w++) v += red[((size_t)w * kTok + tok) * 32 + row];
+            const size_t pr = (size_t)pair_at(start, tok);
+            if constexpr (MODE == kGateUp) {
+                const float up = __shfl_down_sync(0xffffffffu, v, 16);
+                if (row < 16 && row0 + row < p.mat[0].rows) p.out[0][pr * p.mat[0].rows + row0 + row] = v / (1.f + expf(-v)) * up;
+            } else {
+                if (row0 + row < p.mat[mat].rows) p.out[mat][pr * p.mat[mat].rows + row0 + row] = v;
+            }
+        }
+    }
+}
+
+constexpr int kMaxSmem = 200 * 1024;
+
+size_t smem_bytes(int ntl, int chunk) {
+    return (size_t)2 * ntl * chunk * kTokBytes + (size_t)ntl * chunk * kFactorBytes + (size_t)2 * kWarps * 2 * ntl * 32 * 4;
+}
+
+template <Q4Mode MODE, int NTL>
+int launch_one(const Q4Params &p, int jobs, int sm_count, cudaStream_t st) {
+    const int G = p.in_dim / 64;
+    int chunk = G;
+    while (smem_bytes(NTL, chunk) > kMaxSmem) chunk = (chunk + 1) / 2;
+    const size_t smem = smem_bytes(NTL, chunk);
+    static unsigned long long configured = 0;
+    if (first_use_on_device(&configured) &&
+        cudaFuncSetAttribute(q4_stream_kernel<MODE, NTL>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem) != cudaSuccess)
+        return -1;
+    int per_job = 0;
+    if (MODE == kGateUp) per_job = (p.mat[0].rows + 15) / 16;
+    else
+        for (int i = 0; i < p.nmat; i++) per_job += (p.mat[i].rows + 31) / 32;
+    const int per_sm = std::max(1, std::min(NTL == 4 ? 1 : 2, (int)((220 * 1024) / (smem + 1024))));
+    const long long units = (long long)jobs * per_job;
+    const int grid = (int)std::min<long long>(units, (long long)sm_count * per_sm);
+    return launch_dependent(q4_stream_kernel<MODE, NTL>, dim3(grid), dim3(kThreads), smem, st, p, chunk, per_job, jobs) == cudaSuccess ? 1 : -1;
+}
+
+}  // namespace
+
+int launch_q4_stream(Q4Mode mode, const Q4Params &p, int sm_count, cudaStream_t st) {
+    if (mode == kProj) {
+        // tokens per pass over the weights: as many as there are, up to 8; more take more passes, which find the weights in L2
+        if (p.n <= 2) return launch_one<kProj, 1>(p, 1, sm_count, st);
+        if (p.n <= 4) return launch_one<kProj, 2>(p, 1, sm_count, st);
+        return launch_one<kProj, 4>(p, (p.n + 7) / 8, sm_count, st);
+    }
+    const int pairs = p.n * p.top_k;  // an upper bound of the jobs; with a plan the device knows how many there are
+    if (p.plan.njobs == nullptr) return mode == kGateUp ? launch_one<kGateUp, 1>(p, pairs, sm_count, st) : launch_one<kDown, 1>(p, pairs, sm_count, st);
+    return mode == kGateUp ? launch_one<kGateUp, 2>(p, pairs, sm_count, st) : launch_one<kDown, 2>(p, pairs, sm_count, st);
+}
+
+}  // namespace fm

@@ -300,6 +300,83 @@ void fm_proj_free(FmCtx *ctx, FmProjWeights *device);
 fm_status fm_out_proj_norm(FmCtx *ctx, const FmProjWeights *w, int n, const float *x, const float *residual,
                            const uint16_t *norm_w, float *h_mid, float *h_post);
 
+/* Projections from 4-bit affine weights, several at a time: y[i] = W_i x for `count` (1..8) matrices that read the same
+ * input -- q | gate, k and v of a full-attention layer; qkv, z, beta and alpha of a GatedDeltaNet layer; the router and the
+ * shared expert's gate.  Replaces gpu_encode_batch_matvec / BatchMatvecSpec (metal_infer/gpu_dispatch.h) and, at prompt
+ * size, dequant_gemm_4bit_batch (metal_infer/shaders.metal); CPU cpu_dequant_matvec (metal_infer/cpu_kernels.h:199-232).
+ * x [n][in_dim], y[i] [n][out_dim_i] follow the pointer mode; the array y itself is a host array; weights are device
+ * pointers in either mode, 16-byte aligned words.  in_dim a multiple of 64 (up to 65536) and the same for all, out_dim any;
+ * n up to max_batch_tokens.
+ * Accuracy is fp32's: the nibbles are exact on the tensor cores, an activation enters them as 22 bits or more, the scale and
+ * bias of a group meet its sum in fp32.  A token with an infinity or a NaN among its inputs gets NaN outputs.
+ * The outputs must not overlap each other or the inputs. */
+fm_status fm_proj_forward(FmCtx *ctx, int count, const FmProjWeights *w, int n, const float *x, float *const *y);
+
+/* Routing: which experts a token goes to, and with what weights.  The reference takes the softmax of the gate's logits, the
+ * top_k largest and divides them by their sum (cpu_softmax, cpu_topk: metal_infer/cpu_kernels.h; order of use in
+ * fused_layer_forward).  Per token, over the logits x[0..num_experts):
+ *     s = softmax(x) or 1 / (1 + exp(-x));   c = s + bias   (bias may be NULL; it moves the choice, not the weight)
+ *     num_groups > 1: the experts are num_groups equal runs; a run counts with the sum of its group_best (1 or 2) largest c,
+ *     and only the top_groups best runs remain
+ *     ids = the top_k largest c among what remains, largest first, ties to the lowest index (softmax without a bias: the
+ *     largest logits, which is the same order and has no ties by underflow)
+ *     weights = s of those, divided by their sum if renormalize, times scale
+ * An expert whose logit or bias is NaN or -infinity is not available (an expert that is switched off); where fewer than
+ * top_k are, the remaining slots get id -1 and weight 0.  Comparisons that fp32 cannot decide are taken in fp64.
+ * shared_expert = 1: the logits have one more column, the shared expert's gate; each token gets one more slot, with id
+ * num_experts and weight sigmoid(that logit), so that a shared expert stacked behind the routed ones runs with them.
+ * logits [n][num_experts + shared_expert], bias [num_experts], expert_ids and weights [n][top_k + shared_expert] follow the
+ * pointer mode.  num_experts <= 1024, top_k <= 32, num_groups <= 32. */
+enum { FM_SCORE_SOFTMAX = 0, FM_SCORE_SIGMOID = 1 };
+typedef struct FmRouteConfig {
+    int num_experts;     /* 512 */
+    int top_k;           /* 10 */
+    int score;           /* FM_SCORE_SOFTMAX */
+    int num_groups;      /* 1 */
+    int top_groups;      /* 1 */
+    int group_best;      /* 1 */
+    int renormalize;     /* 1 */
+    float scale;         /* 1.0 */
+    int shared_expert;   /* 0 */
+} FmRouteConfig;
+void fm_default_route_config(FmRouteConfig *rc);
+fm_status fm_moe_route(FmCtx *ctx, const FmRouteConfig *rc, int n, const float *logits, const float *bias, int *expert_ids,
+                       float *weights);
+
+/* The experts behind the router, and the end of the layer:
+ *     a_j    = silu(gate_e x) * (up_e x),  e = expert_ids[t][j]
+ *     h_out  = residual + sum_j weights[t][j] * down_e a_j          (slots in order; residual may be NULL)
+ *     h_norm = h_out * rsqrt(mean(h_out^2) + rms_norm_eps) * norm_w (may be NULL; norm_w bf16 [hidden] or NULL: the next
+ *                                                                    layer's input norm)
+ * Replaces the expert encoders of metal_infer/gpu_dispatch.h (gate, up, swiglu, down per expert) and moe_combine_residual +
+ * rms_norm (metal_infer/shaders.metal).  Weights are stacks of 4-bit affine matrices in device memory, in either pointer mode:
+ * gate and up [num_experts][inter][hidden], down [num_experts][hidden][inter], each as words, scales and biases like
+ * FmProjWeights.  expert_stride = 0: each of the nine arrays is packed by itself; else it is the distance in bytes (a multiple
+ * of 16) from one expert to the next in all nine (one blob per expert).
+ * Experts [first_expert, first_expert + num_experts) are the ones held here; slots with any other id (-1, another rank's) add
+ * nothing, so the ranks of an expert-sharded model sum their h_out (with the residual on one of them).
+ * An expert that several slots or tokens name is read once for all of them, as far as that pays; the same id twice in a
+ * token counts twice.  x [n][hidden], expert_ids and weights [n][top_k] (top_k <= 32), residual, h_out and h_norm [n][hidden]
+ * follow the pointer mode; h_out may be the residual itself, and x may be h_out or h_norm.  hidden and inter multiples of 64
+ * (up to 65536), num_experts <= 1024, n up to max_batch_tokens.  Accuracy as for fm_proj_forward.
+ * The first call of a size allocates workspace (so make it before a stream capture: FM_ERR_CAPACITY otherwise); graphs
+ * captured on one context share that workspace and must not run at the same time. */
+typedef struct FmExpertWeights {
+    int format;                  /* FM_W_Q4_AFFINE */
+    int num_experts, first_expert;
+    int hidden, inter;           /* 4096, 1024 */
+    int group_size;              /* 64 */
+    int64_t expert_stride;       /* bytes; 0 = packed */
+    const uint32_t *gate_w;
+    const uint16_t *gate_scales, *gate_biases;
+    const uint32_t *up_w;
+    const uint16_t *up_scales, *up_biases;
+    const uint32_t *down_w;
+    const uint16_t *down_scales, *down_biases;
+} FmExpertWeights;
+fm_status fm_moe_experts(FmCtx *ctx, const FmExpertWeights *w, int n, int top_k, const float *x, const int *expert_ids,
+                         const float *weights, const float *residual, const uint16_t *norm_w, float *h_out, float *h_norm);
+
 /* Off by default.  On: the caller vouches that the launch that precedes a fm_gdn_decode call in the stream does not
  * touch the state of the layer that call steps (in a model loop it never does: the previous launch belongs to another
  * layer or to a projection).  The step is then launched as a programmatic dependent of whatever precedes it: it

@@ -1,0 +1,126 @@
+"""fm_moe_route against its definition in 64 bits: ids exactly, weights to fp32."""
+import numpy as np
+import pytest
+import torch
+
+import moe_ref
+from test_gpu_proj_forward import context
+
+pytestmark = pytest.mark.gpu
+BASE = dict(num_experts=64, top_k=4, score=0, num_groups=1, top_groups=1, group_best=1, renormalize=1, scale=1.0, shared_expert=0)
+
+
+def run(pkg, c, rc, logits, bias=None):
+    n, slots = len(logits), rc["top_k"] + rc["shared_expert"]
+    dev = lambda a: None if a is None else torch.from_numpy(np.ascontiguousarray(a, np.float32)).cuda()  # noqa: E731
+    ids = torch.full((n + 1, slots), 77, device="cuda", dtype=torch.int32)
+    w = torch.full((n + 1, slots), 77.0, device="cuda")
+    c.moe_route(pkg.route_config(**rc), n, dev(logits), dev(bias), ids, w)
+    c.synchronize()
+    assert torch.all(ids[n:] == 77) and torch.all(w[n:] == 77.0)
+    return ids[:n].cpu().numpy(), w[:n].cpu().numpy()
+
+
+def check(got, want):
+    """Weights: exp and the sigmoid to 2 ulp and the exponent's own rounding (2^-24 of it, exponents up to 40 here), the sum
+    over the experts, two divisions, the factor: 128 half steps cover them."""
+    assert np.array_equal(got[0], want[0])
+    assert np.all(np.abs(got[1] - want[1]) <= 128 * moe_ref.EPS * np.abs(want[1]) + 1e-37)
+
+
+CASES = [dict(), dict(num_experts=512, top_k=10), dict(num_experts=512, top_k=10, shared_expert=1), dict(num_experts=1, top_k=1),
+         dict(num_experts=33, top_k=32), dict(num_experts=32, top_k=32, renormalize=0), dict(num_experts=1000, top_k=3, scale=2.5), dict(num_experts=1024, top_k=17, score=1),
+         dict(num_experts=256, top_k=8, score=1, num_groups=8, top_groups=4, group_best=2, scale=2.5), dict(num_experts=100, top_k=6, num_groups=5, top_groups=2, renormalize=0),
+         dict(num_experts=60, top_k=7, num_groups=4, top_groups=2, group_best=2), dict(num_experts=32, top_k=3, num_groups=32, top_groups=3, group_best=2),
+         dict(num_experts=96, top_k=9, score=1, num_groups=3, top_groups=3, group_best=1, renormalize=0, shared_expert=1)]
+
+
+@pytest.mark.parametrize("with_bias", [False, True])
+@pytest.mark.parametrize("case", CASES)
+def test_random_logits(pkg, case, with_bias):
+    rc = {**BASE, **case}
+    rng = np.random.default_rng(rc["num_experts"] + rc["top_k"])
+    c = context(pkg, max_batch=512)
+    for n in (1, 3, 130):
+        logits = (2.0 * rng.standard_normal((n, rc["num_experts"] + rc["shared_expert"]))).astype(np.float32)
+        bias = (0.1 * rng.standard_normal(rc["num_experts"])).astype(np.float32) if with_bias else None
+        check(run(pkg, c, rc, logits, bias), moe_ref.route(logits, bias, rc))
+    c.close()
+
+
+@pytest.mark.parametrize("score", [0, 1])
+def test_borders_that_fp32_cannot_decide(pkg, score):
+    """Scores that differ by less than fp32's rounding of them, and equal ones: 64 bits decide, ties go to the lowest index."""
+    rc = {**BASE, "num_experts": 128, "top_k": 8, "score": score}
+    rng = np.random.default_rng(4)
+    logits = (3.0 + 1e-6 * rng.integers(-3, 4, size=(64, 128))).astype(np.float32)
+    logits[:, ::5] -= 9.0
+    logits[32:, 7] = logits[32:, 90]
+    bias = (1e-8 * rng.integers(-2, 3, size=128)).astype(np.float32)
+    grouped = {**rc, "num_groups": 8, "top_groups": 3, "group_best": 2}
+    c = context(pkg)
+    for r in (rc, grouped):
+        for b in (None, bias):
+            check(run(pkg, c, r, logits, b), moe_ref.route(logits, b, r))
+    same = np.zeros((3, 128), np.float32)
+    for r in (rc, grouped):
+        ids, w = run(pkg, c, r, same)
+        assert np.array_equal(ids, np.tile(np.arange(8, dtype=np.int32), (3, 1))) and np.allclose(w, 1 / 8, rtol=1e-6, atol=0)
+    c.close()
+
+
+@pytest.mark.parametrize("score", [0, 1])
+@pytest.mark.parametrize("groups", [1, 4])
+def test_experts_that_are_not_available(pkg, score, groups):
+    rc = {**BASE, "num_experts": 40, "top_k": 6, "score": score, "num_groups": groups, "top_groups": min(groups, 2), "group_best": 2, "shared_expert": 1}
+    rng = np.random.default_rng(6)
+    logits = rng.standard_normal((12, 41)).astype(np.float32)
+    logits[0, :40] = -np.inf                       # nothing is left
+    logits[1, :40] = -np.inf; logits[1, [5, 33]] = 0.5, 0.25
+    logits[2, 3:37] = np.nan
+    logits[3, :40] = np.finfo(np.float32).min      # the lowest finite value is a logit like any other
+    logits[4, 1:40] = np.finfo(np.float32).min
+    logits[5, [4, 9]] = np.inf
+    logits[6, 40] = -np.inf
+    logits[7, :40] = -200.0 + 0.5 * rng.standard_normal(40)
+    logits[8, 10:30] = -np.inf
+    bias = (0.1 * rng.standard_normal(40)).astype(np.float32)
+    bias[[2, 11]] = -np.inf, np.nan
+    c = context(pkg)
+    for b in (None, bias):
+        for renorm in (0, 1):
+            r = {**rc, "renormalize": renorm}
+            check(run(pkg, c, r, logits, b), moe_ref.route(logits, b, r))
+    c.close()
+
+
+def test_host_pointers(pkg):
+    rc = {**BASE, "shared_expert": 1}
+    rng = np.random.default_rng(1)
+    logits = rng.standard_normal((9, 65)).astype(np.float32)
+    c = context(pkg, host=True)
+    ids, w = np.empty((9, 5), np.int32), np.empty((9, 5), np.float32)
+    c.moe_route(pkg.route_config(**rc), 9, logits, None, ids, w)
+    check((ids, w), moe_ref.route(logits, None, rc))
+    c.close()
+
+
+def test_refusals(pkg):
+    c = context(pkg, max_batch=4)
+    x = torch.zeros((8, 64), device="cuda")
+    ids, w = torch.zeros((8, 4), device="cuda", dtype=torch.int32), torch.zeros((8, 4), device="cuda")
+    B = pkg.binding
+
+    def status(n=1, args=(x, None, ids, w), **kw):
+        with pytest.raises(pkg.FmError) as e:
+            c.moe_route(pkg.route_config(**{**BASE, **kw}), n, *args)
+        assert e.value.text.startswith("fm_moe_route")
+        return e.value.status
+    for bad in (dict(num_experts=0), dict(num_experts=1025), dict(top_k=0), dict(top_k=33), dict(num_groups=0), dict(num_groups=64)):
+        assert status(**bad) == B.FM_ERR_UNSUPPORTED
+    for bad in (dict(score=2), dict(top_k=5, num_groups=16, top_groups=1), dict(num_groups=3), dict(top_groups=2), dict(top_groups=0),
+                dict(num_groups=8, top_groups=2, group_best=3), dict(shared_expert=2), dict(n=5), dict(n=-1)):
+        assert status(**bad) == B.FM_ERR_INVALID
+    assert status(args=(None, None, ids, w)) == B.FM_ERR_INVALID and status(args=(x, None, None, w)) == B.FM_ERR_INVALID
+    c.moe_route(pkg.route_config(**BASE), 0, x, None, ids, w)
+    c.close()

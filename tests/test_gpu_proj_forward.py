@@ -1,0 +1,143 @@
+"""fm_proj_forward: 4-bit projections that share their input, against the product in 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+import moe_ref
+
+pytestmark = pytest.mark.gpu
+
+
+def context(pkg, host=False, max_batch=64, **kw):
+    cfg = pkg.default_config(num_full_layers=0, num_linear_layers=0, max_batch_tokens=max_batch, **kw)
+    c = pkg.Context(cfg, host_pointers=host)
+    if not host:
+        c.set_stream(torch.cuda.current_stream().cuda_stream)
+    return c
+
+
+def on_device(pkg, mat):
+    w, s, b = mat
+    cuda = lambda a, t: torch.from_numpy(a.view(t)).cuda()  # noqa: E731
+    return pkg.proj_weights(cuda(w, np.int32), cuda(s, np.int16).view(torch.bfloat16), cuda(b, np.int16).view(torch.bfloat16))
+
+
+def run(pkg, c, mats, x):
+    xd = torch.from_numpy(np.asarray(x, np.float32)).cuda()
+    ys = [torch.full((len(x) + 1, m[0].shape[0]), 7.0, device="cuda") for m in mats]
+    c.proj_forward([on_device(pkg, m) for m in mats], len(x), xd, ys)
+    c.synchronize()
+    for y in ys:
+        assert torch.all(y[len(x):] == 7.0)  # rows behind the last token stay as they were
+    return [y[: len(x)].cpu().numpy() for y in ys]
+
+
+SHAPES = [  # tokens, inputs, outputs
+    (1, 64, [1]), (1, 4096, [512, 33, 1]), (2, 128, [16]), (2, 1088, [100, 1]), (3, 576, [31, 32, 33]), (4, 1024, [130]), (5, 640, [17, 1, 1, 5]),
+    (8, 4096, [96]), (9, 192, [40]), (17, 2048, [64, 64, 3]), (40, 1088, [257]), (1, 32768, [5]), (3, 24640, [18]), (11, 8192, [33]),
+    (2, 512, [1, 2, 3, 4, 5, 6, 7, 8])]
+
+
+@pytest.mark.parametrize("n,k,outs", SHAPES)
+def test_products(pkg, n, k, outs):
+    rng = np.random.default_rng(1000 + n * 7 + k)
+    c = context(pkg)
+    mats = [moe_ref.weights(rng, o, k) for o in outs]
+    x = rng.standard_normal((n, k)).astype(np.float32)
+    for got, m in zip(run(pkg, c, mats, x), mats):
+        moe_ref.close(got, *moe_ref.product(x, m))
+    c.close()
+
+
+@pytest.mark.parametrize("n", [1, 4, 13, 40])
+def test_inputs_of_every_size(pkg, n):
+    """Outliers beside small values, groups of zeros, values at both ends of fp32's range: no group loses its own."""
+    rng = np.random.default_rng(5 + n)
+    c = context(pkg)
+    k = 64 * 12
+    m = moe_ref.weights(rng, 48, k)
+    x = rng.standard_normal((n, k))
+    x[:, 64:128] = 0.0
+    x[:, 128] = 3.0e4
+    x[:, 192:256] *= 1e-6
+    x[-1, :] = 0.0
+    for scale in (1.0, 1e-30, 1e30):
+        xs = (x * scale).astype(np.float32)
+        want, bound = moe_ref.product(xs, m)
+        moe_ref.close(run(pkg, c, [m], xs)[0], want, bound + 1e-300)
+    c.close()
+
+
+def test_non_finite_inputs_stay_in_their_token(pkg):
+    rng = np.random.default_rng(3)
+    for n in (4, 24):
+        c = context(pkg)
+        m = moe_ref.weights(rng, 40, 256)
+        x = rng.standard_normal((n, 256)).astype(np.float32)
+        want, bound = moe_ref.product(x, m)
+        x[1, 3], x[3, 200] = np.inf, np.nan
+        got = run(pkg, c, [m], x)[0]
+        assert np.isnan(got[[1, 3]]).all()
+        keep = [t for t in range(n) if t not in (1, 3)]
+        moe_ref.close(got[keep], want[keep], bound[keep])
+        c.close()
+
+
+def test_host_pointers_and_uploaded_weights(pkg):
+    rng = np.random.default_rng(8)
+    c = context(pkg, host=True)
+    mats = [moe_ref.weights(rng, o, 512) for o in (70, 9)]
+    dev = [c.proj_upload(*m) for m in mats]
+    for n in (1, 6, 64):
+        x = rng.standard_normal((n, 512)).astype(np.float32)
+        ys = [np.empty((n, 70), np.float32), np.empty((n, 9), np.float32)]
+        c.proj_forward(dev, n, x, ys)
+        for y, m in zip(ys, mats):
+            moe_ref.close(y, *moe_ref.product(x, m))
+    for d in dev:
+        c.proj_free(d)
+    c.close()
+
+
+def test_same_token_gives_the_same_bits_wherever_it_stands(pkg):
+    rng = np.random.default_rng(9)
+    c = context(pkg)
+    m = moe_ref.weights(rng, 65, 1024)
+    x = rng.standard_normal((1, 1024)).astype(np.float32)
+    for n in (2, 7, 8):
+        got = run(pkg, c, [m], np.repeat(x, n, 0))[0]
+        assert np.all(got == got[0])
+    c.close()
+
+
+def test_refusals(pkg):
+    rng = np.random.default_rng(2)
+    c = context(pkg, max_batch=8)
+    a, b = on_device(pkg, moe_ref.weights(rng, 16, 128)), on_device(pkg, moe_ref.weights(rng, 16, 192))
+    x, y = torch.zeros((9, 192), device="cuda"), torch.full((9, 16), 7.0, device="cuda")
+    B = pkg.binding
+
+    def status(ws, n, x_=x, ys=(y,)):
+        with pytest.raises(pkg.FmError) as e:
+            c.proj_forward(list(ws), n, x_, list(ys))
+        assert e.value.text.startswith("fm_proj_forward")
+        return e.value.status
+
+    def changed(mat, **kw):
+        r = B.FmProjWeights.from_buffer_copy(mat)
+        for k, v in kw.items():
+            setattr(r, k, v)
+        return r
+    assert status([a, b], 1, ys=(y, y)) == B.FM_ERR_INVALID                    # inputs of different length
+    assert status([a], 9) == B.FM_ERR_INVALID and status([a], -1) == B.FM_ERR_INVALID
+    assert status([a] * 9, 1, ys=[y] * 9) == B.FM_ERR_INVALID and status([], 1, ys=[]) == B.FM_ERR_INVALID
+    assert status([a], 1, x_=None) == B.FM_ERR_INVALID and status([a], 1, ys=[None]) == B.FM_ERR_INVALID
+    for bad in (dict(group_size=32), dict(in_dim=96), dict(in_dim=0), dict(out_dim=0), dict(format=1), dict(in_dim=65600)):
+        assert status([changed(a, **bad)], 1) == B.FM_ERR_UNSUPPORTED
+    assert status([changed(a, scales=None)], 1) == B.FM_ERR_INVALID
+    assert status([changed(a, w=a.w + 4)], 1) == B.FM_ERR_INVALID
+    assert status([a], 1, x_=x.view(-1)[1:129]) == B.FM_ERR_INVALID            # x off its 16-byte boundary
+    c.proj_forward([a], 0, x, [y])                                             # no tokens: nothing to do
+    c.synchronize()
+    assert torch.all(y == 7.0)
+    c.close()
