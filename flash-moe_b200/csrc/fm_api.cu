@@ -1050,6 +1050,11 @@ struct Carver {  // pieces of a block, 256-byte aligned; base null: only counts
     }
 };
 
+// Up to this many tokens (projections) or pairs per expert held (experts) the weights stream past the activations on the
+// integer tensor cores; beyond, the prompt form takes over.
+constexpr int kProjStreamTokens = 16;
+constexpr int kExpertStreamPairs = 3;
+
 static bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 extern "C" fm_status fm_proj_forward(FmCtx *ctx, int count, const FmProjWeights *w, int n, const float *x, float *const *y) {
@@ -1079,14 +1084,35 @@ extern "C" fm_status fm_proj_forward(FmCtx *ctx, int count, const FmProjWeights 
     }
     if (!ok) return fail(ctx, FM_ERR_INVALID, "fm_proj_forward: staging buffer too small (raise max_batch_tokens)");
     if (!aligned16(p.x)) return fail(ctx, FM_ERR_INVALID, "fm_proj_forward: x is not 16-byte aligned");
-    FM_CUDA(ctx, sg.push());
+    const bool gemm = n > kProjStreamTokens;
+    void *xs = nullptr;
+    float *tscale = nullptr;
     fm_status st;
+    if (gemm) {
+        auto carve = [&](Carver cv) {
+            xs = cv.take<uint16_t>((size_t)n * 2 * q4_split_columns(p.in_dim));
+            tscale = cv.take<float>((size_t)n);
+            return cv.off;
+        };
+        char *ws = nullptr;
+        st = moe_workspace(ctx, "fm_proj_forward", carve(Carver{nullptr}), &ws);
+        if (st) return st;
+        carve(Carver{ws});
+    }
+    FM_CUDA(ctx, sg.push());
     {
         ProfScope prof(ctx);
-        st = launched(ctx, launch_q4_stream(kProj, p, ctx->sm_count, ctx->stream), "proj_forward");
+        if (!gemm) {
+            st = launched(ctx, launch_q4_stream(kProj, p, ctx->sm_count, ctx->stream), "proj_forward");
+        } else {
+            st = launched(ctx, launch_q4_split(p.x, n, p.in_dim, nullptr, xs, tscale, ctx->stream), "proj_forward split");
+            if (st == FM_OK) st = launched(ctx, launch_q4_gemm(kProj, p, xs, n, tscale, ctx->d_err, ctx->sm_count, ctx->stream), "proj_forward");
+        }
     }
     if (st) return st;
+    if (sg.host && gemm) FM_CUDA(ctx, cudaMemcpyAsync(ctx->h_err, ctx->d_err, sizeof(int), cudaMemcpyDeviceToHost, ctx->stream));
     for (int i = 0; i < count; i++) FM_CUDA(ctx, sg.pull(y[i], where[i], (size_t)n * w[i].out_dim));
+    if (sg.host && gemm) return check_device_error(ctx);
     return FM_OK;
 }
 
@@ -1162,13 +1188,21 @@ extern "C" fm_status fm_moe_experts(FmCtx *ctx, const FmExpertWeights *w, int n,
         return fail(ctx, FM_ERR_INVALID, "fm_moe_experts: x, residual, h_out and h_norm have to be 16-byte aligned, norm_w 8-byte");
 
     MoePlan plan = {};
-    float *hbuf = nullptr, *ybuf = nullptr;
+    const bool gemm = pairs > (size_t)kExpertStreamPairs * w->num_experts && pairs > 16;
+    float *hbuf = nullptr, *ybuf = nullptr, *xscale = nullptr, *hscale = nullptr;
+    void *xs = nullptr, *hs = nullptr;
     auto carve = [&](Carver cv) {
-        plan.njobs = cv.take<int>(1);
+        plan.njobs = cv.take<int>(2);
         plan.jobs = cv.take<int4>(pairs);
         plan.pair_of = cv.take<int>(pairs);
         hbuf = cv.take<float>(pairs * I);
         ybuf = cv.take<float>(pairs * H);
+        if (gemm) {
+            xs = cv.take<uint16_t>((size_t)n * 2 * q4_split_columns(w->hidden));
+            xscale = cv.take<float>((size_t)n);
+            hs = cv.take<uint16_t>(pairs * 2 * q4_split_columns(w->inter));
+            hscale = cv.take<float>(pairs);
+        }
         return cv.off;
     };
     char *ws = nullptr;
@@ -1191,22 +1225,34 @@ extern "C" fm_status fm_moe_experts(FmCtx *ctx, const FmExpertWeights *w, int n,
     dn.in_dim = w->inter; dn.x = hbuf; dn.nmat = 1; dn.out[0] = ybuf;
     dn.mat[0] = view(w->down_w, w->down_scales, w->down_biases, H, I);
     if (pairs > 16) {  // fewer: one job per pair, straight from the ids
-        st = launched(ctx, launch_moe_plan(d_ids, (int)pairs, w->first_expert, w->num_experts, 4, plan, ctx->stream), "moe_plan");
+        st = launched(ctx, launch_moe_plan(d_ids, (int)pairs, w->first_expert, w->num_experts, gemm ? kGemmTokens : 4, plan, ctx->stream), "moe_plan");
         if (st) return st;
         gu.plan = dn.plan = plan;
     }
     {
         ProfScope prof(ctx);
-        st = launched(ctx, launch_q4_stream(kGateUp, gu, ctx->sm_count, ctx->stream), "moe gate_up");
-        if (st) return st;
-        st = launched(ctx, launch_q4_stream(kDown, dn, ctx->sm_count, ctx->stream), "moe down");
+        if (!gemm) {
+            st = launched(ctx, launch_q4_stream(kGateUp, gu, ctx->sm_count, ctx->stream), "moe gate_up");
+            if (st) return st;
+            st = launched(ctx, launch_q4_stream(kDown, dn, ctx->sm_count, ctx->stream), "moe down");
+        } else {
+            st = launched(ctx, launch_q4_split(d_x, n, w->hidden, nullptr, xs, xscale, ctx->stream), "moe split");
+            if (st) return st;
+            st = launched(ctx, launch_q4_gemm(kGateUp, gu, xs, n, xscale, ctx->d_err, ctx->sm_count, ctx->stream), "moe gate_up");
+            if (st) return st;
+            st = launched(ctx, launch_q4_split(hbuf, (int)pairs, w->inter, plan.njobs + 1, hs, hscale, ctx->stream), "moe split");
+            if (st) return st;
+            st = launched(ctx, launch_q4_gemm(kDown, dn, hs, (int)pairs, hscale, ctx->d_err, ctx->sm_count, ctx->stream), "moe down");
+        }
     }
     if (st) return st;
     st = launched(ctx, launch_moe_combine(ybuf, d_ids, d_w, n, top_k, w->first_expert, w->num_experts, w->hidden, d_res, d_nw, ctx->cfg.rms_norm_eps, d_out,
                                           d_norm, ctx->stream), "moe_combine");
     if (st) return st;
+    if (sg.host && gemm) FM_CUDA(ctx, cudaMemcpyAsync(ctx->h_err, ctx->d_err, sizeof(int), cudaMemcpyDeviceToHost, ctx->stream));
     FM_CUDA(ctx, sg.pull(h_out, w_out, n * H));
     FM_CUDA(ctx, sg.pull(h_norm, w_norm, n * H));
+    if (sg.host && gemm) return check_device_error(ctx);
     return FM_OK;
 }
 

@@ -299,6 +299,8 @@ struct Q4View {
 // pair p = token * top_k + slot; a job is a run of pairs of one expert, pair_of[] their numbers, sorted by expert.
 enum Q4Mode { kProj = 0, kGateUp = 1, kDown = 2 };
 constexpr int kMaxProj = 8;
+// index of an expert among those held, -1 for any other id
+__host__ __device__ inline int local_expert(int id, int first, int count) { return id >= first && id - first < count ? id - first : -1; }
 struct MoePlan {        // device memory, written by moe_plan_kernel
     int *njobs;         // [1]
     int4 *jobs;         // (expert, first position in pair_of, pairs, -)
@@ -317,6 +319,13 @@ struct Q4Params {
 };
 // Few tokens per matrix: the weights stream past the activations once per job of up to 2 * ntl tokens (q4_stream.cu).
 int launch_q4_stream(Q4Mode mode, const Q4Params &p, int sm_count, cudaStream_t st);
+// Many tokens per matrix: tcgen05 (q4_gemm.cu).  xs, tscale: what launch_q4_split left of the activations -- of p.x for
+// kProj and kGateUp (by token), of the h rows for kDown (sorted, like pair_of); with experts h comes out sorted and y by pair
+// number.  plan.jobs hold up to 64 pairs.  err: the context's error word.
+constexpr int kGemmTokens = 64;
+int q4_split_columns(int in_dim);  // fp16 numbers per term and row
+int launch_q4_split(const float *x, int rows, int in_dim, const int *count, void *xs, float *tscale, cudaStream_t st);
+int launch_q4_gemm(Q4Mode mode, const Q4Params &p, const void *xs, int xs_rows, const float *tscale, int *err, int sm_count, cudaStream_t st);
 // Which pairs go to which expert, in runs of `tile` (moe_plan.cu)
 int launch_moe_plan(const int *ids, int pairs, int first_expert, int num_experts, int tile, const MoePlan &plan, cudaStream_t st);
 // h = residual + sum over the slots of weight * y[pair]; h_norm = rms-norm(h) * norm_w (moe_plan.cu)

@@ -44,8 +44,8 @@ moe_plan_kernel(const int *__restrict__ ids, int pairs, int first_expert, int nu
     s_count[tid] = 0;
     __syncthreads();
     for (int p = tid; p < pairs; p += kPlanThreads) {
-        const int e = __ldg(ids + p) - first_expert;
-        if (e >= 0 && e < num_experts) atomicAdd(s_count + e, 1);
+        const int e = local_expert(__ldg(ids + p), first_expert, num_experts);
+        if (e >= 0) atomicAdd(s_count + e, 1);
     }
     __syncthreads();
     const int count = s_count[tid], tiles = (count + tile - 1) / tile;
@@ -54,11 +54,11 @@ moe_plan_kernel(const int *__restrict__ ids, int pairs, int first_expert, int nu
     const int start = end - count, tstart = tend - tiles;
     s_count[tid] = start;  // from here on the next free position
     for (int i = 0; i < tiles; i++) plan.jobs[tstart + i] = make_int4(tid, start + i * tile, min(tile, count - i * tile), 0);
-    if (tid == kPlanThreads - 1) *plan.njobs = tend;
+    if (tid == kPlanThreads - 1) { plan.njobs[0] = tend; plan.njobs[1] = end; }
     __syncthreads();
     for (int p = tid; p < pairs; p += kPlanThreads) {
-        const int e = __ldg(ids + p) - first_expert;
-        if (e >= 0 && e < num_experts) plan.pair_of[atomicAdd(s_count + e, 1)] = p;
+        const int e = local_expert(__ldg(ids + p), first_expert, num_experts);
+        if (e >= 0) plan.pair_of[atomicAdd(s_count + e, 1)] = p;
     }
 }
 
@@ -74,8 +74,7 @@ moe_combine_kernel(const float *__restrict__ y, const int *__restrict__ ids, con
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     if (warp == 0) {  // the slots that have an expert here
-        const int e = lane < top_k ? ids[(size_t)t * top_k + lane] - first_expert : -1;
-        const bool here = e >= 0 && e < num_experts;
+        const bool here = lane < top_k && local_expert(ids[(size_t)t * top_k + lane], first_expert, num_experts) >= 0;
         const unsigned m = __ballot_sync(0xffffffffu, here);
         if (here) {
             const int at = __popc(m & ((1u << lane) - 1));

@@ -1,0 +1,660 @@
+// Products of 4-bit affine matrices with many tokens: projections of a prompt, and the routed experts once an expert sees
+// more than a handful of tokens.  tcgen05 / TMEM / TMA.
+//
+// Reference: dequant_gemm_4bit_batch (metal_infer/shaders.metal) and, per expert, the chain of metal_infer/gpu_dispatch.h.
+//     y[r][t] = sum_g sum_{k in g} s[r][g] (nibble[r][k] - 8) x[t][k]  +  sum_g (b[r][g] + 8 s[r][g]) X[t][g]
+// with X[t][g] the sum of the group's 64 inputs.
+//
+// Exactness.  A scale is bf16 (8 bits) and |nibble - 8| is 8 or has 3 bits, so s * (nibble - 8) has 11 bits at most: it
+// IS an fp16 number, once a power of two per row and 256 inputs has brought the scales into range.  An activation enters
+// as two fp16 terms, hi + lo (22 bits, a power of two per token).  The second sum is one more block of 64 columns, per 64
+// groups, with both factors in two terms.  The tensor cores add into fp32 by truncation, which shrinks a long sum by a
+// few 2^-24 per addition; so TMEM accumulates over 256 inputs only, and the parts are added in fp32 by the epilogue
+// warps, which apply the row's power of two in the same fused multiply-add.
+//
+// Organisation (persistent, one CTA per SM).  A unit is T row tiles of 128 rows and up to 64 tokens; a step is one tile
+// over one chunk of 4 groups.  kGateUp: the tiles alternate between gate and up, so that SwiGLU needs no exchange.
+//   warps 0-7    widen: a thread owns a row; two 16-byte reads from the TMA-filled weight tile, 13 instructions per word of
+//                eight nibbles, 32 TMEM columns (one group) per store.  Operand A lives in TMEM: written row by row where
+//                the MMA wants it, and half of the shared-memory traffic of an A tile there.
+//   warps 8-15   epilogue: running sums in TMEM, added up per step; the last step of a tile writes the results, 128
+//                consecutive features per token and store
+//   warp 16      TMA producer: weight tiles [128 rows][128 bytes], token tiles hi | lo (kGateUp: gathered by token, 4 rows per
+//                instruction)
+//   warp 17      issues the MMAs (M128, N = the unit's tokens rounded up to 16, K16)
+// TMEM columns: T * 64 running sums, 2 * 64 of steps in flight, the rest operand A in slots of 32.
+// With two terms the tensor work is twice the product's; what bounds a long prompt is that, a short one the weights' stream.
+// Every wait is bounded; on expiry the CTA records an error code and winds down.
+#include <cuda.h>
+#include <cuda_fp16.h>
+
+#include <string.h>
+
+#include <algorithm>
+
+#include "fm_device.cuh"
+#include "fm_internal.h"
+#include "fm_tc.cuh"
+
+namespace fm {
+
+namespace {
+
+constexpr int kTok = 64;                    // tokens per unit
+constexpr int kChunk = 4;                   // groups per step
+constexpr int kBSlot = 2 * kTok * 128;      // bytes of a token tile: one group, hi then lo
+constexpr int kBSlots = 8;
+constexpr int kWSlot = 128 * 128;           // bytes of a weight tile: 128 rows, 4 groups
+constexpr int kWSlots = 5;
+constexpr int kGemmThreads = 18 * 32;
+constexpr int kDBufs = 2;
+// Steps whose row factors are kept: the widening warps are at most the operand slots (8, one to a step at the least), the
+// steps in flight and their own step ahead of the epilogue.
+constexpr int kFSteps = 16;
+constexpr uint32_t kColStep = 0, kColSum = kDBufs * kTok;  // TMEM columns; operand A behind the sums
+
+template <int T>
+struct Layout {
+    static constexpr uint32_t colA = kColSum + T * kTok;
+    static constexpr int aslots = (512 - (int)colA) / 32;
+};
+
+enum Bar { BAR_W_FULL = 0, BAR_W_EMPTY = BAR_W_FULL + kWSlots, BAR_B_FULL = BAR_W_EMPTY + kWSlots, BAR_B_EMPTY = BAR_B_FULL + kBSlots,
+           BAR_D_FULL = BAR_B_EMPTY + kBSlots, BAR_D_EMPTY = BAR_D_FULL + kDBufs, BAR_A_FULL = BAR_D_EMPTY + kDBufs,
+           BAR_A_EMPTY = BAR_A_FULL + 8, BAR_END = BAR_A_EMPTY + 8, BAR_COUNT };
+constexpr int kGemmSmem = kBSlots * kBSlot + kWSlots * kWSlot + kFSteps * 128 * 4 + BAR_COUNT * 8 + 1024;
+
+struct GemmMaps {
+    CUtensorMap w[kMaxProj];  // words: [matrix][rows][K / 8] (kGateUp: 0 gate, 1 up)
+    CUtensorMap s[kMaxProj], b[kMaxProj];  // scales and biases [matrix][rows][K / 64], where GemmParams.wide
+    CUtensorMap x;            // fp16 [rows][hi | lo]
+};
+struct GemmParams {
+    Q4Params p;
+    int G, pseudo, units_per_job, kp;  // groups, blocks of 64 groups, row units, columns of one term of x
+    int m_units[kMaxProj];             // kProj: row units of each matrix
+    int wide;                          // groups a multiple of 8, scales and biases 16-byte aligned
+    const float *tscale;               // what a row of x has to be multiplied with
+    int *err;
+};
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(dst),
+                 "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+                 : "memory");
+}
+// four rows of a 2-D tensor, one 128-byte piece of each
+__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap *map, int x, int4 rows, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];\n" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(rows.x), "r"(rows.y), "r"(rows.z), "r"(rows.w), "r"(bar)
+        : "memory");
+}
+
+// A ring position: slot and the parity its next phase completes with.
+template <int N>
+struct Ring {
+    int slot = 0;
+    uint32_t phase = 0;
+    __device__ void next() {
+        if (++slot == N) { slot = 0; phase ^= 1; }
+    }
+};
+
+// One unit, as every role works it out for itself.
+struct Unit {
+    int mat, row0, rows;   // matrix, first row, rows of the matrix
+    int expert;
+    int tiles;             // row tiles that hold rows
+    int start, cnt, ncols; // tokens (kProj) or positions in pair_of; columns of the MMA
+};
+
+template <Q4Mode MODE, int T>
+__device__ __forceinline__ Unit unit_at(const GemmParams &g, int u) {
+    Unit r;
+    const int job = u / g.units_per_job;
+    int mu = u - job * g.units_per_job;
+    r.mat = 0; r.expert = 0;
+    if constexpr (MODE == kProj) {
+        while (mu >= g.m_units[r.mat]) mu -= g.m_units[r.mat++];
+        r.start = job * kTok;
+        r.cnt = min(kTok, g.p.n - r.start);
+    } else {
+        const int4 j = g.p.plan.jobs[job];
+        r.expert = j.x; r.start = j.y; r.cnt = j.z;
+    }
+    constexpr int kRows = MODE == kGateUp ? T * 64 : T * 128;
+    r.row0 = mu * kRows;
+    r.rows = g.p.mat[r.mat].rows;
+    const int t = (min(kRows, r.rows - r.row0) + 127) / 128;
+    r.tiles = MODE == kGateUp ? 2 * t : t;
+    r.ncols = (r.cnt + 15) / 16 * 16;
+    return r;
+}
+template <Q4Mode MODE>
+__device__ __forceinline__ int tile_row(const Unit &u, int tile) {
+    return u.row0 + 128 * (MODE == kGateUp ? tile >> 1 : tile);
+}
+template <Q4Mode MODE>
+__device__ __forceinline__ int tile_mat(const Unit &u, int tile) {
+    return MODE == kGateUp ? tile & 1 : u.mat;
+}
+
+// The four scales of a row's chunk as bf16 bits (zero beyond the last group).
+__device__ __forceinline__ uint2 chunk_scales(const unsigned char *row, int c, int G, bool wide) {
+    if (wide) return __ldg(reinterpret_cast<const uint2 *>(row) + c);
+    const uint16_t *s = reinterpret_cast<const uint16_t *>(row) + c * kChunk;
+    const int left = G - c * kChunk;
+    uint2 v;
+    v.x = (uint32_t)__ldg(s) | (left > 1 ? (uint32_t)__ldg(s + 1) << 16 : 0u);
+    v.y = (left > 2 ? (uint32_t)__ldg(s + 2) : 0u) | (left > 3 ? (uint32_t)__ldg(s + 3) << 16 : 0u);
+    return v;
+}
+// Exponent field of the largest of them, kept where both 2^(135 - e) and 2^(e - 135) are normal numbers.
+__device__ __forceinline__ int chunk_exponent(uint2 v) {
+    const uint32_t a = max(v.x & 0x7fff0000u, v.x << 16 & 0x7fff0000u), b = max(v.y & 0x7fff0000u, v.y << 16 & 0x7fff0000u);
+    return max((int)(max(a, b) >> 23), 16);
+}
+__device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ float pow2(int biased) { return __uint_as_float((uint32_t)biased << 23); }
+__device__ __forceinline__ uint32_t h2_bits(__half2 v) { return *reinterpret_cast<const uint32_t *>(&v); }
+
+// (n_q - 8, n_{q+4} - 8) * s for q = 0..3 of a weight word; every step exact (see the head of the file)
+__device__ __forceinline__ void widen_word(uint32_t w, __half2 s, uint32_t *out) {
+    const __half2 k1032 = __half2half2(__ushort_as_half(0x6408)), k16th = __half2half2(__ushort_as_half(0x2C00)), km72 = __half2half2(__ushort_as_half(0xD480));
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const uint32_t v = i ? w >> 8 : w;
+        const uint32_t even = (v & 0x000F000Fu) | 0x64006400u, odd = (v & 0x00F000F0u) | 0x64006400u;  // 1024 + n, 1024 + 16 n
+        out[2 * i] = h2_bits(__hmul2(__hsub2(*reinterpret_cast<const __half2 *>(&even), k1032), s));
+        out[2 * i + 1] = h2_bits(__hmul2(__hfma2(*reinterpret_cast<const __half2 *>(&odd), k16th, km72), s));
+    }
+}
+
+template <Q4Mode MODE, int T>
+__global__ void __launch_bounds__(kGemmThreads, 1)
+q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ GemmParams g) {
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_abort;
+    using L = Layout<T>;
+    constexpr int kA = L::aslots;
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t sB = base, sW = sB + kBSlots * kBSlot;
+    float *s_f = reinterpret_cast<float *>(smem_raw + (sW + kWSlots * kWSlot - smem_u32(smem_raw)));  // [steps][128 rows] power of two of the step
+    const uint32_t sBar = sW + kWSlots * kWSlot + kFSteps * 128 * 4;
+    auto bar = [&](int i) { return sBar + 8u * (uint32_t)i; };
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        s_abort = 0;
+        for (int i = 0; i < kWSlots; i++) { mbar_init(bar(BAR_W_FULL + i), 1); mbar_init(bar(BAR_W_EMPTY + i), 8); }
+        for (int i = 0; i < kBSlots; i++) { mbar_init(bar(BAR_B_FULL + i), 1); mbar_init(bar(BAR_B_EMPTY + i), 1); }
+        for (int i = 0; i < kDBufs; i++) { mbar_init(bar(BAR_D_FULL + i), 1); mbar_init(bar(BAR_D_EMPTY + i), 8); }
+        mbar_init(bar(BAR_END), 1);
+        for (int i = 0; i < 8; i++) { mbar_init(bar(BAR_A_FULL + i), 4); mbar_init(bar(BAR_A_EMPTY + i), 1); }
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    if (warp == 17) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&s_tmem)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    volatile int *abortp = &s_abort;
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+
+    const int G = g.G, nreal = (G + kChunk - 1) / kChunk, nchunks = nreal + g.pseudo;
+    const int njobs = MODE == kProj ? (g.p.n + kTok - 1) / kTok : *g.p.plan.njobs;
+    const int nunits = njobs * g.units_per_job;
+    const size_t s_pitch = (size_t)G * 2;
+    // one thread's row of a tile: its scales and biases (rows beyond the matrix read the last one; their results are dropped)
+    auto row_ptr = [&](const Unit &u, int tile, int r, bool biases) {
+        const Q4View &m = g.p.mat[tile_mat<MODE>(u, tile)];
+        const int row = min(tile_row<MODE>(u, tile) + r, m.rows - 1);
+        return (biases ? m.biases : m.scales) + (size_t)u.expert * m.s_stride + (size_t)row * s_pitch;
+    };
+
+    if (warp == 16) {
+        // ================= TMA producer =================
+        Ring<kWSlots> rw;
+        Ring<kBSlots> rb;
+        int wcount = 0, bcount = 0;
+        bool ok = true;
+        for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x) {
+            const Unit un = unit_at<MODE, T>(g, u);
+            int4 tok = make_int4(0, 0, 0, 0);
+            if constexpr (MODE == kGateUp) {  // lane l < 16: tokens of columns 4 l .. 4 l + 3 (columns without one repeat the first)
+                auto token = [&](int c) { return g.p.plan.pair_of[un.start + (c < un.cnt ? c : 0)] / g.p.top_k; };
+                if (lane < 16) tok = make_int4(token(4 * lane), token(4 * lane + 1), token(4 * lane + 2), token(4 * lane + 3));
+            }
+            for (int c = 0; c < nchunks && ok; c++) {
+                const int ng = c < nreal ? min(kChunk, G - c * kChunk) : 1;
+                auto load_b = [&](int grp) {  // grp: 64 columns of x
+                    if (lane == 0) ok = bcount < kBSlots || mbar_wait(bar(BAR_B_EMPTY + rb.slot), rb.phase ^ 1, abortp);
+                    ok = __shfl_sync(0xffffffffu, ok, 0);
+                    if (!ok) return;
+                    const uint32_t full = bar(BAR_B_FULL + rb.slot), dst = sB + (uint32_t)rb.slot * kBSlot;
+                    if (lane == 0) mbar_expect_tx(full, (uint32_t)un.ncols * 256u);
+                    __syncwarp();
+                    if constexpr (MODE == kGateUp) {
+                        if (lane * 4 < un.ncols) {
+                            tma_gather4(dst + (uint32_t)lane * 512u, &maps.x, grp * 64, tok, full);
+                            tma_gather4(dst + kTok * 128u + (uint32_t)lane * 512u, &maps.x, g.kp + grp * 64, tok, full);
+                        }
+                    } else {
+                        if (lane * 16 < un.ncols) {
+                            tma_load_2d(dst + (uint32_t)lane * 2048u, &maps.x, grp * 64, un.start + lane * 16, full);
+                            tma_load_2d(dst + kTok * 128u + (uint32_t)lane * 2048u, &maps.x, g.kp + grp * 64, un.start + lane * 16, full);
+                        }
+                    }
+                    rb.next(); bcount = min(bcount + 1, kBSlots);
+                };
+                auto load_w = [&](const CUtensorMap *map, int x, int tile) {  // 128 bytes of each of the tile's rows
+                    if (lane == 0) ok = wcount < kWSlots || mbar_wait(bar(BAR_W_EMPTY + rw.slot), rw.phase ^ 1, abortp);
+                    ok = __shfl_sync(0xffffffffu, ok, 0);
+                    if (!ok) return;
+                    if (lane == 0) {
+                        mbar_expect_tx(bar(BAR_W_FULL + rw.slot), kWSlot);
+                        tma_load_3d(sW + (uint32_t)rw.slot * kWSlot, map, x, tile_row<MODE>(un, tile), un.expert, bar(BAR_W_FULL + rw.slot));
+                    }
+                    rw.next(); wcount = min(wcount + 1, kWSlots);
+                };
+                auto load_tile = [&](int tile) {
+                    const int m = tile_mat<MODE>(un, tile);
+                    if (c < nreal) load_w(&maps.w[m], c * 32, tile);
+                    else if (g.wide) {
+                        load_w(&maps.s[m], (c - nreal) * 64, tile);
+                        if (ok) load_w(&maps.b[m], (c - nreal) * 64, tile);
+                    }
+                };
+                // in the order they are wanted: the first tile, the chunk's tokens, the other tiles
+                load_tile(0);
+                for (int j = 0; j < ng && ok; j++) load_b(c < nreal ? c * kChunk + j : G + c - nreal);
+                for (int i = 1; i < un.tiles && ok; i++) load_tile(i);
+            }
+        }
+        // the copies in flight land before the CTA goes (they have, unless a wait ran out)
+        if (lane == 0 && *abortp) {
+            const long long t0 = clock64();
+            auto drain = [&](int first, int n, auto r, int count) {
+                for (int i = 0; i < count; i++) {
+                    if (r.slot == 0) { r.slot = n; r.phase ^= 1; }
+                    r.slot--;
+                    while (!mbar_try(bar(first + r.slot), r.phase) && clock64() - t0 < 200000000LL) {}
+                }
+            };
+            drain(BAR_W_FULL, kWSlots, rw, wcount);
+            drain(BAR_B_FULL, kBSlots, rb, bcount);
+        }
+    } else if (warp == 17) {
+        // ================= MMA issuer =================
+        if (lane == 0) {
+            Ring<kBSlots> rb;
+            Ring<kA> ra;
+            Ring<kDBufs> rd;
+            int dcount = 0;
+            bool ok = true;
+            for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x) {
+                const Unit un = unit_at<MODE, T>(g, u);
+                const uint32_t idesc = idesc_dense(128, un.ncols, false, 0);
+                for (int c = 0; c < nchunks && ok; c++) {
+                    const bool real = c < nreal;
+                    const int na = real ? min(kChunk, G - c * kChunk) : 2, nb = real ? na : 1;
+                    for (int i = 0; i < un.tiles && ok; i++) {
+                        ok = dcount < kDBufs || mbar_wait(bar(BAR_D_EMPTY + rd.slot), rd.phase ^ 1, abortp);
+                        if (!ok) break;
+                        const uint32_t d = tmem + kColStep + (uint32_t)rd.slot * kTok;
+                        Ring<kBSlots> rt = rb;
+                        for (int j = 0; j < na && ok; j++) {
+                            ok = mbar_wait(bar(BAR_B_FULL + rt.slot), rt.phase, abortp) && mbar_wait(bar(BAR_A_FULL + ra.slot), ra.phase, abortp);
+                            if (!ok) break;
+                            tc_fence_after();
+                            const uint32_t a = tmem + L::colA + (uint32_t)ra.slot * 32, b = sB + (uint32_t)rt.slot * kBSlot;
+                            const uint64_t hi = smem_desc(b, 0, 1024), lo = smem_desc(b + kTok * 128, 0, 1024);
+#pragma unroll
+                            for (int k = 0; k < 4; k++) tc_mma_f16_ta(d, a + k * 8, lo + k * 2, idesc, j > 0 || k > 0);
+#pragma unroll
+                            for (int k = 0; k < 4; k++) tc_mma_f16_ta(d, a + k * 8, hi + k * 2, idesc, 1);
+                            tc_commit(bar(BAR_A_EMPTY + ra.slot));
+                            if (i == un.tiles - 1 && (real || j == na - 1)) tc_commit(bar(BAR_B_EMPTY + rt.slot));
+                            ra.next();
+                            if (real) rt.next();
+                        }
+                        if (!ok) break;
+                        tc_commit(bar(BAR_D_FULL + rd.slot));
+                        rd.next(); dcount = min(dcount + 1, kDBufs);
+                    }
+                    for (int j = 0; j < nb; j++) rb.next();
+                }
+            }
+            if (!ok) {  // a wait ran out: let what was issued finish before tensor memory is given back
+                tc_commit(bar(BAR_END));
+                const long long t0 = clock64();
+                while (!mbar_try(bar(BAR_END), 0) && clock64() - t0 < 200000000LL) {}
+            }
+        }
+        __syncwarp();
+    } else if (warp < 8) {
+        // ================= widen: weight tiles -> operand A =================
+        const int wg = warp >> 2, r = (warp & 3) * 32 + lane;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // TMEM lane of the warp's first row, in bits 16+
+        Ring<kWSlots> rw;
+        Ring<kA> ra;
+        Ring<kFSteps> rf;
+        int acount = 0, turn = 0;  // operand slots alternate between the two groups of four warps
+        bool ok = true;
+        // the steps in order; the scales of a step are fetched while the one before it is worked on
+        Unit un;
+        int u = blockIdx.x, c = 0, i = 0;
+        uint2 sc = make_uint2(0, 0);
+        if (u < nunits) {
+            un = unit_at<MODE, T>(g, u);
+            sc = chunk_scales(row_ptr(un, 0, r, false), 0, G, g.wide);
+        }
+        while (u < nunits && ok) {
+            Unit un2 = un;
+            int u2 = u, c2 = c, i2 = i + 1;
+            if (i2 == un.tiles) { i2 = 0; c2++; }
+            if (c2 == nchunks) {
+                c2 = 0; u2 = u + gridDim.x;
+                if (u2 < nunits) un2 = unit_at<MODE, T>(g, u2);
+            }
+            uint2 sc2 = make_uint2(0, 0);
+            if (u2 < nunits && c2 < nreal) sc2 = chunk_scales(row_ptr(un2, i2, r, false), c2, G, g.wide);
+
+            const bool real = c < nreal;
+            const int na = real ? min(kChunk, G - c * kChunk) : 2;
+            int e = 0;
+            uint32_t pw[32];  // bias block: this thread's term of its row, as fp16 pairs
+            if (real) {
+                e = chunk_exponent(sc);
+                ok = __all_sync(0xffffffffu, mbar_wait(bar(BAR_W_FULL + rw.slot), rw.phase, abortp));
+            } else {
+                // b + 8 s of the row's groups; slot `turn` is the first term, the other the second
+                float v[64];
+                const int g0 = (c - nreal) * 64, gn = min(64, G - g0);
+                if (g.wide) {  // both tiles came like weight tiles, 64 bf16 to a row
+                    Ring<kWSlots> rs = rw;
+                    ok = __all_sync(0xffffffffu, mbar_wait(bar(BAR_W_FULL + rs.slot), rs.phase, abortp));
+                    const uint32_t srow = sW + (uint32_t)rs.slot * kWSlot + (uint32_t)r * 128u;
+                    rs.next();
+                    ok = ok && __all_sync(0xffffffffu, mbar_wait(bar(BAR_W_FULL + rs.slot), rs.phase, abortp));
+                    const uint32_t brow = sW + (uint32_t)rs.slot * kWSlot + (uint32_t)r * 128u;
+                    if (!ok) break;
+#pragma unroll
+                    for (int q = 0; q < 8; q++) {
+                        const uint4 s4 = ld_shared16(srow + (uint32_t)((q ^ (r & 7)) << 4)), b4 = ld_shared16(brow + (uint32_t)((q ^ (r & 7)) << 4));
+                        const uint32_t sw[4] = {s4.x, s4.y, s4.z, s4.w}, bw[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            v[8 * q + 2 * k] = fmaf(8.f, __uint_as_float(sw[k] << 16), __uint_as_float(bw[k] << 16));
+                            v[8 * q + 2 * k + 1] = fmaf(8.f, __uint_as_float(sw[k] & 0xffff0000u), __uint_as_float(bw[k] & 0xffff0000u));
+                        }
+                    }
+                } else {
+                    const uint16_t *ps = reinterpret_cast<const uint16_t *>(row_ptr(un, i, r, false)) + g0;
+                    const uint16_t *pb = reinterpret_cast<const uint16_t *>(row_ptr(un, i, r, true)) + g0;
+#pragma unroll
+                    for (int q = 0; q < 64; q++) v[q] = q < gn ? fmaf(8.f, bf16_bits_to_float(__ldg(ps + q)), bf16_bits_to_float(__ldg(pb + q))) : 0.f;
+                }
+                float m = 0.f;
+#pragma unroll
+                for (int q = 0; q < 64; q++) m = fmaxf(m, fabsf(v[q]));
+                e = max((int)(__float_as_uint(m) >> 23), 16);
+                const float up = pow2(127 + 135 - e);
+#pragma unroll
+                for (int q = 0; q < 32; q++) {
+                    const float a0 = v[2 * q] * up, a1 = v[2 * q + 1] * up;
+                    const __half2 h = __floats2half2_rn(a0, a1);
+                    const float2 hf = __half22float2(h);
+                    pw[q] = h2_bits(turn == wg ? h : __floats2half2_rn(a0 - hf.x, a1 - hf.y));
+                }
+            }
+            if (!ok) break;
+            if (turn == wg) s_f[rf.slot * 128 + r] = pow2(127 + e - 135);  // for the epilogue; seen through A_FULL, the MMAs and D_FULL
+            for (int j = 0; j < na && ok; j++, ra.next(), turn ^= 1) {
+                const bool first = acount < kA;
+                acount = min(acount + 1, kA);
+                if (turn != wg) continue;
+                uint32_t a[32];
+                if (real) {
+                    const __half2 s = __float2half2_rn(__uint_as_float(((j & 2 ? sc.y : sc.x) >> ((j & 1) * 16)) << 16) * pow2(127 + 135 - e));
+                    const uint32_t wrow = sW + (uint32_t)rw.slot * kWSlot + (uint32_t)r * 128u;
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const uint4 w4 = ld_shared16(wrow + (uint32_t)(((2 * j + h) ^ (r & 7)) << 4));
+                        widen_word(w4.x, s, a + h * 16);
+                        widen_word(w4.y, s, a + h * 16 + 4);
+                        widen_word(w4.z, s, a + h * 16 + 8);
+                        widen_word(w4.w, s, a + h * 16 + 12);
+                    }
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 32; q++) a[q] = pw[q];
+                }
+                ok = first || __all_sync(0xffffffffu, mbar_wait(bar(BAR_A_EMPTY + ra.slot), ra.phase ^ 1, abortp));
+                if (!ok) break;
+                tc_fence_after();
+                tc_st32(tmem + lanes + L::colA + (uint32_t)ra.slot * 32, a);
+                tc_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(BAR_A_FULL + ra.slot));
+            }
+            const int used = real ? 1 : g.wide ? 2 : 0;  // weight slots of the step
+            for (int k = 0; k < used; k++) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(BAR_W_EMPTY + rw.slot));
+                rw.next();
+            }
+            rf.next();
+            un = un2; u = u2; c = c2; i = i2; sc = sc2;
+        }
+    } else {
+        // ================= epilogue =================
+        const int r = (warp & 3) * 32 + lane, half = (warp - 8) >> 2;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+        Ring<kDBufs> rd;
+        Ring<kFSteps> rf;
+        bool ok = true;
+        for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x) {
+            const Unit un = unit_at<MODE, T>(g, u);
+            // column `half * 32 + lane`: the row of the output it goes to, and what takes its token's power of two off again
+            const int col = half * 32 + lane;
+            const bool there = col < un.cnt;
+            long long out_row = 0;
+            float ts = 0.f;
+            if (there) {
+                if constexpr (MODE == kProj) { out_row = un.start + col; ts = __ldg(g.tscale + un.start + col); }
+                if constexpr (MODE == kGateUp) { out_row = un.start + col; ts = __ldg(g.tscale + g.p.plan.pair_of[un.start + col] / g.p.top_k); }
+                if constexpr (MODE == kDown) { out_row = g.p.plan.pair_of[un.start + col]; ts = __ldg(g.tscale + un.start + col); }
+            }
+            const int live = min(32, un.cnt - half * 32);  // columns of this warp
+            for (int c = 0; c < nchunks && ok; c++) {
+                const bool last = c == nchunks - 1;
+                for (int i = 0; i < un.tiles && ok; i++) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(bar(BAR_D_FULL + rd.slot), rd.phase, abortp));
+                    if (!ok) break;
+                    tc_fence_after();
+                    const float f = s_f[rf.slot * 128 + r];
+                    rf.next();
+                    uint32_t d[32], s[32];
+                    const uint32_t tsum = tmem + lanes + kColSum + (uint32_t)i * kTok + (uint32_t)half * 32;
+                    if (live > 0) {
+                        tc_ld32(tmem + lanes + kColStep + (uint32_t)rd.slot * kTok + (uint32_t)half * 32, d);
+                        if (c > 0) tc_ld32(tsum, s);
+                        tc_wait_ld();
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(BAR_D_EMPTY + rd.slot));
+                    rd.next();
+                    if (live <= 0) continue;
+#pragma unroll
+                    for (int k = 0; k < 32; k++) d[k] = __float_as_uint(fmaf(__uint_as_float(d[k]), f, c > 0 ? __uint_as_float(s[k]) : 0.f));
+                    if (!last || (MODE == kGateUp && !(i & 1))) {
+                        tc_st32(tsum, d);
+                        tc_wait_st();
+                        continue;
+                    }
+                    if constexpr (MODE == kGateUp) {  // the gate's sums wait one tile to the left
+                        tc_ld32(tsum - kTok, s);
+                        tc_wait_ld();
+                    }
+                    const int row = tile_row<MODE>(un, i) + r;
+                    float *out = g.p.out[MODE == kProj ? un.mat : 0];
+#pragma unroll
+                    for (int k = 0; k < 32; k++) {
+                        const long long o = __shfl_sync(0xffffffffu, out_row, k);
+                        const float t = __shfl_sync(0xffffffffu, ts, k);
+                        float v = __uint_as_float(d[k]) * t;
+                        if constexpr (MODE == kGateUp) {
+                            const float a = __uint_as_float(s[k]) * t;
+                            v = a / (1.f + expf(-a)) * v;
+                        }
+                        if (k < live && row < un.rows) out[o * un.rows + row] = v;
+                    }
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 17) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512u) : "memory");
+    }
+    if (tid == 0 && s_abort) atomicExch(g.err, 0x60 + MODE);
+}
+
+// Rows of fp32 activations -> two fp16 terms each, brought into range by a power of two per row, in the order the widened
+// words have along K (0 4 1 5 2 6 3 7 of every eight); behind them the sums of every 64 inputs, likewise in two terms.
+// One CTA per row.
+__global__ void __launch_bounds__(256)
+q4_split_kernel(const float *__restrict__ x, int K, int kp, const int *count, __half *__restrict__ xs, float *__restrict__ tscale) {
+    __shared__ float s_red[8], s_sum[8];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    const size_t row = blockIdx.x;
+    if (count != nullptr && (int)row >= *count) return;
+    const float4 *src = reinterpret_cast<const float4 *>(x + row * K);
+    float am = 0.f, sum = 0.f;
+    for (int i = tid; i < K / 4; i += 256) {
+        const float4 v = __ldg(src + i);
+        am = fmaxf(fmaxf(am, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+        sum += (v.x - v.x) + (v.y - v.y) + (v.z - v.z) + (v.w - v.w);  // 0, or NaN where an input is not finite
+    }
+    am = warp_max(am);
+    sum = warp_sum(sum);
+    if (lane == 0) { s_red[warp] = am; s_sum[warp] = sum; }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; w++) { am = fmaxf(am, s_red[w]); sum += s_sum[w]; }
+    const bool bad = !(sum == 0.f);
+    // am in [2^e, 2^(e+1)) becomes [2^8, 2^9): the sum of 64 inputs stays below fp16's largest number
+    int e = max((int)(__float_as_uint(am) >> 23), 16);
+    if (bad) e = 135;
+    const float up = __uint_as_float((uint32_t)(127 + 135 - e) << 23);
+    if (tid == 0) tscale[row] = bad ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)(127 + e - 135) << 23);
+    __half *hi = xs + row * 2 * kp, *lo = hi + kp;
+    const int G = K / 64;
+    for (int i0 = 0; i0 < K / 8; i0 += 256) {  // eight inputs per thread; the eight threads of a group are neighbours
+        const int i = i0 + tid;
+        const bool valid = i < K / 8;
+        float v[8] = {};
+        if (valid && !bad) {
+            const float4 a = __ldg(src + 2 * i), b = __ldg(src + 2 * i + 1);
+            v[0] = a.x * up; v[1] = a.y * up; v[2] = a.z * up; v[3] = a.w * up; v[4] = b.x * up; v[5] = b.y * up; v[6] = b.z * up; v[7] = b.w * up;
+        }
+        uint32_t h[4], l[4];
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const __half2 p = __floats2half2_rn(v[q], v[q + 4]);
+            const float2 f = __half22float2(p);
+            h[q] = h2_bits(p);
+            l[q] = h2_bits(__floats2half2_rn(v[q] - f.x, v[q + 4] - f.y));
+        }
+        float s = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (valid) {
+            *reinterpret_cast<uint4 *>(hi + 8 * i) = make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4 *>(lo + 8 * i) = make_uint4(l[0], l[1], l[2], l[3]);
+            if ((i & 7) == 0) {
+                const __half sh = __float2half_rn(s);
+                hi[K + (i >> 3)] = sh;
+                lo[K + (i >> 3)] = __float2half_rn(s - __half2float(sh));
+            }
+        }
+    }
+    for (int i = G + tid; i < kp - K; i += 256) { hi[K + i] = __float2half_rn(0.f); lo[K + i] = __float2half_rn(0.f); }
+}
+
+// [matrices][rows][row_bytes], box [1][128 rows][128 bytes], 128-byte swizzle, zeros outside
+bool map_rows(CUtensorMap *m, const void *base, long long stride, int rows, int row_bytes, int matrices, bool words) {
+    EncodeTiledFn enc = get_encode();
+    if (!enc) return false;
+    const cuuint32_t esz = words ? 4 : 2;
+    const cuuint64_t dims[3] = {(cuuint64_t)row_bytes / esz, (cuuint64_t)rows, (cuuint64_t)matrices};
+    const cuuint64_t strides[2] = {(cuuint64_t)row_bytes, (cuuint64_t)(matrices > 1 ? stride : (long long)rows * row_bytes)};
+    const cuuint32_t box[3] = {128 / esz, 128, 1}, estr[3] = {1, 1, 1};
+    return enc(m, words ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void *>(base), dims, strides, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <Q4Mode MODE, int T>
+int launch_gemm(const GemmMaps &maps, GemmParams &g, long long jobs, int sm_count, cudaStream_t st) {
+    constexpr int kRows = MODE == kGateUp ? T * 64 : T * 128;
+    g.units_per_job = 0;
+    for (int i = 0; i < (MODE == kProj ? g.p.nmat : 1); i++) {
+        g.m_units[i] = (g.p.mat[i].rows + kRows - 1) / kRows;
+        g.units_per_job += g.m_units[i];
+    }
+    static unsigned long long configured = 0;
+    if (first_use_on_device(&configured) &&
+        cudaFuncSetAttribute(q4_gemm_kernel<MODE, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem) != cudaSuccess)
+        return -1;
+    const int grid = (int)std::min<long long>(jobs * g.units_per_job, sm_count);
+    return launch_dependent(q4_gemm_kernel<MODE, T>, dim3(grid), dim3(kGemmThreads), kGemmSmem, st, maps, g) == cudaSuccess ? 1 : -1;
+}
+
+}  // namespace
+
+int q4_split_columns(int in_dim) { return in_dim + (in_dim / 64 + 63) / 64 * 64; }
+
+int launch_q4_split(const float *x, int rows, int in_dim, const int *count, void *xs, float *tscale, cudaStream_t st) {
+    return launch_dependent(q4_split_kernel, dim3(rows), dim3(256), 0, st, x, in_dim, q4_split_columns(in_dim), count, reinterpret_cast<__half *>(xs), tscale) ==
+                   cudaSuccess ? 1 : -1;
+}
+
+int launch_q4_gemm(Q4Mode mode, const Q4Params &p, const void *xs, int xs_rows, const float *tscale, int *err, int sm_count, cudaStream_t st) {
+    GemmMaps maps;
+    memset(&maps, 0, sizeof maps);
+    GemmParams g = {};
+    g.p = p; g.G = p.in_dim / 64; g.pseudo = (g.G + 63) / 64; g.kp = q4_split_columns(p.in_dim); g.tscale = tscale; g.err = err;
+    const int matrices = mode == kProj ? 1 : p.num_experts;
+    g.wide = g.G % 8 == 0;
+    for (int i = 0; i < p.nmat; i++) g.wide = g.wide && (((uintptr_t)p.mat[i].scales | (uintptr_t)p.mat[i].biases) & 15) == 0;
+    for (int i = 0; i < p.nmat; i++) {
+        const Q4View &m = p.mat[i];
+        if (!map_rows(&maps.w[i], m.w, m.w_stride, m.rows, p.in_dim / 2, matrices, true)) return -1;
+        if (g.wide && (!map_rows(&maps.s[i], m.scales, m.s_stride, m.rows, g.G * 2, matrices, false) ||
+                       !map_rows(&maps.b[i], m.biases, m.s_stride, m.rows, g.G * 2, matrices, false)))
+            return -1;
+    }
+    if (!make_map_2d(&maps.x, xs, (uint64_t)xs_rows, (uint64_t)2 * g.kp, mode == kGateUp ? 1 : 16, false)) return -1;
+    const long long jobs = mode == kProj ? (p.n + kTok - 1) / kTok : (long long)p.n * p.top_k;
+    if (mode == kProj) return launch_gemm<kProj, 4>(maps, g, jobs, sm_count, st);
+    if (mode == kGateUp) return launch_gemm<kGateUp, 4>(maps, g, jobs, sm_count, st);
+    return launch_gemm<kDown, 4>(maps, g, jobs, sm_count, st);
+}
+
+}  // namespace fm

@@ -125,7 +125,7 @@ q4_stream_kernel(Q4Params p, int chunk_groups, int units_per_job, int fixed_jobs
             const int4 j = p.plan.jobs[job];
             expert = j.x; start = j.y; cnt = j.z;
         } else {
-            expert = p.ids[job] - p.first_expert; start = job; cnt = expert >= 0 && expert < p.num_experts ? 1 : 0;
+            expert = local_expert(p.ids[job], p.first_expert, p.num_experts); start = job; cnt = expert >= 0 ? 1 : 0;
         }
     };
     auto pair_at = [&](int start, int i) { return MODE == kProj ? start + i : p.plan.njobs != nullptr ? p.plan.pair_of[start + i] : start; };

@@ -118,7 +118,7 @@ def experts(gate, up, down, x, ids, weights, residual, norm_w, first=0, eps=1e-6
     bound = np.abs(h) * 4 * EPS
     for t in range(n):
         for j, e in enumerate(ids[t]):
-            e -= first
+            e = int(e) - first
             if not 0 <= e < held:
                 continue
             g, bg = product(x[t:t + 1], [m[e] for m in gate])

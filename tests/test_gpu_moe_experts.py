@@ -52,13 +52,14 @@ def check(got, m, x, ids, w, res, nw, first=0):
 
 SHAPES = [  # tokens, hidden, inter, experts, slots
     (1, 64, 64, 1, 1), (1, 256, 192, 8, 2), (1, 1024, 512, 16, 10), (3, 256, 192, 8, 2), (2, 128, 64, 5, 3), (5, 192, 320, 4, 4), (9, 576, 128, 40, 6),
-    (30, 128, 192, 6, 2), (64, 256, 64, 3, 1), (70, 128, 128, 100, 8), (33, 1088, 704, 5, 3), (150, 192, 128, 2, 2), (7, 64, 64, 40, 32)]
+    (30, 128, 192, 6, 2), (64, 256, 64, 3, 1), (70, 128, 128, 100, 8), (33, 1088, 704, 5, 3), (150, 192, 128, 2, 2), (7, 64, 64, 40, 32),
+    (260, 512, 320, 4, 2), (400, 256, 512, 3, 1)]
 
 
 @pytest.mark.parametrize("n,hidden,inter,experts,top", SHAPES)
 def test_against_64_bits(pkg, n, hidden, inter, experts, top):
     rng = np.random.default_rng(n * 31 + hidden + experts)
-    c = context(pkg, max_batch=256)
+    c = context(pkg, max_batch=512)
     m = stacks(rng, experts, hidden, inter)
     x, res, ids, w, nw = inputs(rng, n, hidden, experts, top)
     check(run(pkg, c, device_stacks(pkg, m), x, ids, w, res, nw), m, x, ids, w, res, nw)

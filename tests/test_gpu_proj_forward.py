@@ -35,13 +35,15 @@ def run(pkg, c, mats, x):
 SHAPES = [  # tokens, inputs, outputs
     (1, 64, [1]), (1, 4096, [512, 33, 1]), (2, 128, [16]), (2, 1088, [100, 1]), (3, 576, [31, 32, 33]), (4, 1024, [130]), (5, 640, [17, 1, 1, 5]),
     (8, 4096, [96]), (9, 192, [40]), (17, 2048, [64, 64, 3]), (40, 1088, [257]), (1, 32768, [5]), (3, 24640, [18]), (11, 8192, [33]),
-    (2, 512, [1, 2, 3, 4, 5, 6, 7, 8])]
+    (2, 512, [1, 2, 3, 4, 5, 6, 7, 8]),
+    (64, 64, [1]), (65, 128, [129, 1]), (63, 4096, [520]), (100, 192, [128, 513]), (200, 512, [300, 64, 64]), (33, 4160, [40]), (20, 8192, [130]),
+    (130, 1024, [1, 2, 600, 4, 5, 6, 7, 8]), (18, 12352, [33])]
 
 
 @pytest.mark.parametrize("n,k,outs", SHAPES)
 def test_products(pkg, n, k, outs):
     rng = np.random.default_rng(1000 + n * 7 + k)
-    c = context(pkg)
+    c = context(pkg, max_batch=256)
     mats = [moe_ref.weights(rng, o, k) for o in outs]
     x = rng.standard_normal((n, k)).astype(np.float32)
     for got, m in zip(run(pkg, c, mats, x), mats):
