@@ -6,7 +6,8 @@
 // with X[t][g] the sum of the group's 64 inputs.
 //
 // Exactness.  A scale is bf16 (8 bits) and |nibble - 8| is 8 or has 3 bits, so s * (nibble - 8) has 11 bits at most: it
-// IS an fp16 number, once a power of two per row and 256 inputs has brought the scales into range.  An activation enters
+// IS an fp16 number, once a power of two per row and 256 inputs has brought the scales into range (those below 1/256 of
+// the largest keep an absolute error of 2^-18 of its weights).  An activation enters
 // as two fp16 terms, hi + lo (22 bits, a power of two per token).  The second sum is one more block of 64 columns, per 64
 // groups, with both factors in two terms.  The tensor cores add into fp32 by truncation, which shrinks a long sum by a
 // few 2^-24 per addition; so TMEM accumulates over 256 inputs only, and the parts are added in fp32 by the epilogue
@@ -91,6 +92,16 @@ __device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap *map
         : "memory");
 }
 
+// True in one lane of the warp, the same one for every call.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(one));
+    return one != 0;
+}
+
+// The same value in every lane, and known to the compiler as such (values of at least 0).
+__device__ __forceinline__ int uniform(int v) { return __reduce_max_sync(0xffffffffu, v); }
+
 // A ring position: slot and the parity its next phase completes with.
 template <int N>
 struct Ring {
@@ -121,7 +132,7 @@ __device__ __forceinline__ Unit unit_at(const GemmParams &g, int u) {
         r.cnt = min(kTok, g.p.n - r.start);
     } else {
         const int4 j = g.p.plan.jobs[job];
-        r.expert = j.x; r.start = j.y; r.cnt = j.z;
+        r.expert = uniform(j.x); r.start = uniform(j.y); r.cnt = uniform(j.z);
     }
     constexpr int kRows = MODE == kGateUp ? T * 64 : T * 128;
     r.row0 = mu * kRows;
@@ -142,18 +153,21 @@ __device__ __forceinline__ int tile_mat(const Unit &u, int tile) {
 
 // The four scales of a row's chunk as bf16 bits (zero beyond the last group).
 __device__ __forceinline__ uint2 chunk_scales(const unsigned char *row, int c, int G, bool wide) {
-    if (wide) return __ldg(reinterpret_cast<const uint2 *>(row) + c);
+    uint2 v = make_uint2(0, 0);
+    if (wide) {  // volatile: the load stays where it is written, a step ahead of its use
+        asm volatile("ld.global.nc.v2.u32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "l"(reinterpret_cast<const uint2 *>(row) + c));
+        return v;
+    }
     const uint16_t *s = reinterpret_cast<const uint16_t *>(row) + c * kChunk;
     const int left = G - c * kChunk;
-    uint2 v;
     v.x = (uint32_t)__ldg(s) | (left > 1 ? (uint32_t)__ldg(s + 1) << 16 : 0u);
     v.y = (left > 2 ? (uint32_t)__ldg(s + 2) : 0u) | (left > 3 ? (uint32_t)__ldg(s + 3) << 16 : 0u);
     return v;
 }
-// Exponent field of the largest of them, kept where both 2^(135 - e) and 2^(e - 135) are normal numbers.
+// Exponent field of the largest of them, kept where the powers of two made of it are normal numbers.
 __device__ __forceinline__ int chunk_exponent(uint2 v) {
     const uint32_t a = max(v.x & 0x7fff0000u, v.x << 16 & 0x7fff0000u), b = max(v.y & 0x7fff0000u, v.y << 16 & 0x7fff0000u);
-    return max((int)(max(a, b) >> 23), 16);
+    return min(max((int)(max(a, b) >> 23), 16), 244);
 }
 __device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
     uint4 v;
@@ -163,18 +177,55 @@ __device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
 __device__ __forceinline__ float pow2(int biased) { return __uint_as_float((uint32_t)biased << 23); }
 __device__ __forceinline__ uint32_t h2_bits(__half2 v) { return *reinterpret_cast<const uint32_t *>(&v); }
 
-// (n_q - 8, n_{q+4} - 8) * s for q = 0..3 of a weight word; every step exact (see the head of the file)
-__device__ __forceinline__ void widen_word(uint32_t w, __half2 s, uint32_t *out) {
-    const __half2 k1032 = __half2half2(__ushort_as_half(0x6408)), k16th = __half2half2(__ushort_as_half(0x2C00)), km72 = __half2half2(__ushort_as_half(0xD480));
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const uint32_t v = i ? w >> 8 : w;
-        const uint32_t even = (v & 0x000F000Fu) | 0x64006400u, odd = (v & 0x00F000F0u) | 0x64006400u;  // 1024 + n, 1024 + 16 n
-        out[2 * i] = h2_bits(__hmul2(__hsub2(*reinterpret_cast<const __half2 *>(&even), k1032), s));
-        out[2 * i + 1] = h2_bits(__hmul2(__hfma2(*reinterpret_cast<const __half2 *>(&odd), k16th, km72), s));
-    }
+// (n_q - 8, n_{q+4} - 8) * m * 2^-24 for q = 0..3 of a weight word.  A nibble in the low bits of a half is the subnormal
+// fp16 number n * 2^-24 (16 n * 2^-24 one nibble up), so one fused multiply-add takes the 8 off and the scale on, exactly: m
+// is the scale as an integer below 2^15 with 8 bits.
+__device__ __forceinline__ uint32_t fma_h2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;\n" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+}
+__device__ __forceinline__ void widen_word(uint32_t w, uint32_t m, uint32_t m16, uint32_t c, uint32_t *out) {
+    const uint32_t v = w >> 8;
+    out[0] = fma_h2(w & 0x000F000Fu, m, c);
+    out[1] = fma_h2(w & 0x00F000F0u, m16, c);
+    out[2] = fma_h2(v & 0x000F000Fu, m, c);
+    out[3] = fma_h2(v & 0x00F000F0u, m16, c);
+}
+// x as fp16 in both halves
+__device__ __forceinline__ uint32_t dup_h2(float x) {
+    uint32_t d;
+    asm("cvt.rn.f16x2.f32 %0, %1, %1;\n" : "=r"(d) : "f"(x));
+    return d;
+}
+// (a0, a1) = (a0, a1) * f + (b0, b1) in one instruction
+__device__ __forceinline__ void fma_f32x2(uint32_t &a0, uint32_t &a1, uint64_t ff, uint32_t b0, uint32_t b1) {
+    uint64_t a, b, d;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(a) : "r"(a0), "r"(a1));
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(b) : "r"(b0), "r"(b1));
+    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(d) : "l"(a), "l"(ff), "l"(b));
+    asm("mov.b64 {%0, %1}, %2;\n" : "=r"(a0), "=r"(a1) : "l"(d));
 }
 
+// Bounded wait like mbar_wait, with the thread suspended meanwhile: polling warps take issue slots from the widening ones.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag) {
+    long long t0 = 0;
+    while (true) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+            : "=r"(done)
+            : "r"(bar), "r"(parity), "r"(1000000u)
+            : "memory");
+        if (done) return true;
+        if (*abort_flag) return false;
+        if (t0 == 0) t0 = clock64();
+        else if (clock64() - t0 > 1000000000LL) {
+            *abort_flag = 1;
+            return false;
+        }
+    }
+}
 template <Q4Mode MODE, int T>
 __global__ void __launch_bounds__(kGemmThreads, 1)
 q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ GemmParams g) {
@@ -188,7 +239,7 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
     float *s_f = reinterpret_cast<float *>(smem_raw + (sW + kWSlots * kWSlot - smem_u32(smem_raw)));  // [steps][128 rows] power of two of the step
     const uint32_t sBar = sW + kWSlots * kWSlot + kFSteps * 128 * 4;
     auto bar = [&](int i) { return sBar + 8u * (uint32_t)i; };
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
     if (tid == 0) {
         s_abort = 0;
         for (int i = 0; i < kWSlots; i++) { mbar_init(bar(BAR_W_FULL + i), 1); mbar_init(bar(BAR_W_EMPTY + i), 8); }
@@ -211,14 +262,15 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
 
     const int G = g.G, nreal = (G + kChunk - 1) / kChunk, nchunks = nreal + g.pseudo;
-    const int njobs = MODE == kProj ? (g.p.n + kTok - 1) / kTok : *g.p.plan.njobs;
+    const int njobs = MODE == kProj ? (g.p.n + kTok - 1) / kTok : uniform(*g.p.plan.njobs);
     const int nunits = njobs * g.units_per_job;
     const size_t s_pitch = (size_t)G * 2;
     // one thread's row of a tile: its scales and biases (rows beyond the matrix read the last one; their results are dropped)
     auto row_ptr = [&](const Unit &u, int tile, int r, bool biases) {
         const Q4View &m = g.p.mat[tile_mat<MODE>(u, tile)];
-        const int row = min(tile_row<MODE>(u, tile) + r, m.rows - 1);
-        return (biases ? m.biases : m.scales) + (size_t)u.expert * m.s_stride + (size_t)row * s_pitch;
+        const int first = tile_row<MODE>(u, tile);
+        const unsigned char *tile0 = (biases ? m.biases : m.scales) + (size_t)u.expert * m.s_stride + (size_t)first * s_pitch;  // uniform
+        return tile0 + (uint32_t)min(r, m.rows - 1 - first) * (uint32_t)s_pitch;
     };
 
     if (warp == 16) {
@@ -237,7 +289,7 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
             for (int c = 0; c < nchunks && ok; c++) {
                 const int ng = c < nreal ? min(kChunk, G - c * kChunk) : 1;
                 auto load_b = [&](int grp) {  // grp: 64 columns of x
-                    if (lane == 0) ok = bcount < kBSlots || mbar_wait(bar(BAR_B_EMPTY + rb.slot), rb.phase ^ 1, abortp);
+                    if (lane == 0) ok = bcount < kBSlots || bar_wait(bar(BAR_B_EMPTY + rb.slot), rb.phase ^ 1, abortp);
                     ok = __shfl_sync(0xffffffffu, ok, 0);
                     if (!ok) return;
                     const uint32_t full = bar(BAR_B_FULL + rb.slot), dst = sB + (uint32_t)rb.slot * kBSlot;
@@ -257,7 +309,7 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
                     rb.next(); bcount = min(bcount + 1, kBSlots);
                 };
                 auto load_w = [&](const CUtensorMap *map, int x, int tile) {  // 128 bytes of each of the tile's rows
-                    if (lane == 0) ok = wcount < kWSlots || mbar_wait(bar(BAR_W_EMPTY + rw.slot), rw.phase ^ 1, abortp);
+                    if (lane == 0) ok = wcount < kWSlots || bar_wait(bar(BAR_W_EMPTY + rw.slot), rw.phase ^ 1, abortp);
                     ok = __shfl_sync(0xffffffffu, ok, 0);
                     if (!ok) return;
                     if (lane == 0) {
@@ -295,50 +347,58 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
         }
     } else if (warp == 17) {
         // ================= MMA issuer =================
-        if (lane == 0) {
-            Ring<kBSlots> rb;
-            Ring<kA> ra;
-            Ring<kDBufs> rd;
-            int dcount = 0;
-            bool ok = true;
-            for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x) {
-                const Unit un = unit_at<MODE, T>(g, u);
-                const uint32_t idesc = idesc_dense(128, un.ncols, false, 0);
-                for (int c = 0; c < nchunks && ok; c++) {
-                    const bool real = c < nreal;
-                    const int na = real ? min(kChunk, G - c * kChunk) : 2, nb = real ? na : 1;
-                    for (int i = 0; i < un.tiles && ok; i++) {
-                        ok = dcount < kDBufs || mbar_wait(bar(BAR_D_EMPTY + rd.slot), rd.phase ^ 1, abortp);
+        // The whole warp walks the steps and one elected lane issues a slot's MMAs in one go: everything they read is then
+        // uniform across the warp (the reductions below say so to the compiler), and an MMA costs what the tensor core takes,
+        // 41 cycles at N = 64.  Issued by `lane == 0` in divergent code each took 120 to 190.
+        const uint32_t tm = uniform(tmem);
+        Ring<kBSlots> rb;
+        Ring<kA> ra;
+        Ring<kDBufs> rd;
+        int dcount = 0;
+        bool ok = true;
+        for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x) {
+            const Unit un = unit_at<MODE, T>(g, u);
+            const int tiles = un.tiles;
+            const uint32_t idesc = idesc_dense(128, un.ncols, false, 0);
+            for (int c = 0; c < nchunks && ok; c++) {
+                const bool real = c < nreal;
+                const int na = real ? min(kChunk, G - c * kChunk) : 2, nb = real ? na : 1;
+                for (int i = 0; i < tiles && ok; i++) {
+                    ok = dcount < kDBufs || __all_sync(0xffffffffu, bar_wait(bar(BAR_D_EMPTY + rd.slot), rd.phase ^ 1, abortp));
+                    if (!ok) break;
+                    const uint32_t d = tm + kColStep + (uint32_t)rd.slot * kTok;
+                    Ring<kBSlots> rt = rb;
+                    for (int j = 0; j < na && ok; j++) {
+                        ok = __all_sync(0xffffffffu, bar_wait(bar(BAR_B_FULL + rt.slot), rt.phase, abortp) &&
+                                                         bar_wait(bar(BAR_A_FULL + ra.slot), ra.phase, abortp));
                         if (!ok) break;
-                        const uint32_t d = tmem + kColStep + (uint32_t)rd.slot * kTok;
-                        Ring<kBSlots> rt = rb;
-                        for (int j = 0; j < na && ok; j++) {
-                            ok = mbar_wait(bar(BAR_B_FULL + rt.slot), rt.phase, abortp) && mbar_wait(bar(BAR_A_FULL + ra.slot), ra.phase, abortp);
-                            if (!ok) break;
-                            tc_fence_after();
-                            const uint32_t a = tmem + L::colA + (uint32_t)ra.slot * 32, b = sB + (uint32_t)rt.slot * kBSlot;
-                            const uint64_t hi = smem_desc(b, 0, 1024), lo = smem_desc(b + kTok * 128, 0, 1024);
+                        tc_fence_after();
+                        const uint32_t a = tm + L::colA + (uint32_t)ra.slot * 32, b = sB + (uint32_t)rt.slot * kBSlot;
+                        const uint64_t hi = smem_desc(b, 0, 1024), lo = smem_desc(b + kTok * 128, 0, 1024);
+                        const bool done_b = i == tiles - 1 && (real || j == na - 1);
+                        if (elect_one()) {
 #pragma unroll
                             for (int k = 0; k < 4; k++) tc_mma_f16_ta(d, a + k * 8, lo + k * 2, idesc, j > 0 || k > 0);
 #pragma unroll
                             for (int k = 0; k < 4; k++) tc_mma_f16_ta(d, a + k * 8, hi + k * 2, idesc, 1);
                             tc_commit(bar(BAR_A_EMPTY + ra.slot));
-                            if (i == un.tiles - 1 && (real || j == na - 1)) tc_commit(bar(BAR_B_EMPTY + rt.slot));
-                            ra.next();
-                            if (real) rt.next();
+                            if (done_b) tc_commit(bar(BAR_B_EMPTY + rt.slot));
+                            if (j == na - 1) tc_commit(bar(BAR_D_FULL + rd.slot));
                         }
-                        if (!ok) break;
-                        tc_commit(bar(BAR_D_FULL + rd.slot));
-                        rd.next(); dcount = min(dcount + 1, kDBufs);
+                        __syncwarp();
+                        ra.next();
+                        if (real) rt.next();
                     }
-                    for (int j = 0; j < nb; j++) rb.next();
+                    if (!ok) break;
+                    rd.next(); dcount = min(dcount + 1, kDBufs);
                 }
+                for (int j = 0; j < nb; j++) rb.next();
             }
-            if (!ok) {  // a wait ran out: let what was issued finish before tensor memory is given back
-                tc_commit(bar(BAR_END));
-                const long long t0 = clock64();
-                while (!mbar_try(bar(BAR_END), 0) && clock64() - t0 < 200000000LL) {}
-            }
+        }
+        if (!ok && elect_one()) {  // a wait ran out: let what was issued finish before tensor memory is given back
+            tc_commit(bar(BAR_END));
+            const long long t0 = clock64();
+            while (!mbar_try(bar(BAR_END), 0) && clock64() - t0 < 200000000LL) {}
         }
         __syncwarp();
     } else if (warp < 8) {
@@ -348,7 +408,7 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
         Ring<kWSlots> rw;
         Ring<kA> ra;
         Ring<kFSteps> rf;
-        int acount = 0, turn = 0;  // operand slots alternate between the two groups of four warps
+        int ahead = 0, turn = 0;  // operand slots used so far (up to all); they alternate between the two groups of four warps
         bool ok = true;
         // the steps in order; the scales of a step are fetched while the one before it is worked on
         Unit un;
@@ -375,17 +435,17 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
             uint32_t pw[32];  // bias block: this thread's term of its row, as fp16 pairs
             if (real) {
                 e = chunk_exponent(sc);
-                ok = __all_sync(0xffffffffu, mbar_wait(bar(BAR_W_FULL + rw.slot), rw.phase, abortp));
+                ok = __all_sync(0xffffffffu, bar_wait(bar(BAR_W_FULL + rw.slot), rw.phase, abortp));
             } else {
                 // b + 8 s of the row's groups; slot `turn` is the first term, the other the second
                 float v[64];
                 const int g0 = (c - nreal) * 64, gn = min(64, G - g0);
                 if (g.wide) {  // both tiles came like weight tiles, 64 bf16 to a row
                     Ring<kWSlots> rs = rw;
-                    ok = __all_sync(0xffffffffu, mbar_wait(bar(BAR_W_FULL + rs.slot), rs.phase, abortp));
+                    ok = __all_sync(0xffffffffu, bar_wait(bar(BAR_W_FULL + rs.slot), rs.phase, abortp));
                     const uint32_t srow = sW + (uint32_t)rs.slot * kWSlot + (uint32_t)r * 128u;
                     rs.next();
-                    ok = ok && __all_sync(0xffffffffu, mbar_wait(bar(BAR_W_FULL + rs.slot), rs.phase, abortp));
+                    ok = ok && __all_sync(0xffffffffu, bar_wait(bar(BAR_W_FULL + rs.slot), rs.phase, abortp));
                     const uint32_t brow = sW + (uint32_t)rs.slot * kWSlot + (uint32_t)r * 128u;
                     if (!ok) break;
 #pragma unroll
@@ -418,35 +478,40 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
                 }
             }
             if (!ok) break;
-            if (turn == wg) s_f[rf.slot * 128 + r] = pow2(127 + e - 135);  // for the epilogue; seen through A_FULL, the MMAs and D_FULL
-            for (int j = 0; j < na && ok; j++, ra.next(), turn ^= 1) {
-                const bool first = acount < kA;
-                acount = min(acount + 1, kA);
-                if (turn != wg) continue;
-                uint32_t a[32];
-                if (real) {
-                    const __half2 s = __float2half2_rn(__uint_as_float(((j & 2 ? sc.y : sc.x) >> ((j & 1) * 16)) << 16) * pow2(127 + 135 - e));
-                    const uint32_t wrow = sW + (uint32_t)rw.slot * kWSlot + (uint32_t)r * 128u;
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const uint4 w4 = ld_shared16(wrow + (uint32_t)(((2 * j + h) ^ (r & 7)) << 4));
-                        widen_word(w4.x, s, a + h * 16);
-                        widen_word(w4.y, s, a + h * 16 + 4);
-                        widen_word(w4.z, s, a + h * 16 + 8);
-                        widen_word(w4.w, s, a + h * 16 + 12);
-                    }
-                } else {
-#pragma unroll
-                    for (int q = 0; q < 32; q++) a[q] = pw[q];
-                }
-                ok = first || __all_sync(0xffffffffu, mbar_wait(bar(BAR_A_EMPTY + ra.slot), ra.phase ^ 1, abortp));
-                if (!ok) break;
+            // for the epilogue: what the step's sums have to be multiplied with (seen through A_FULL, the MMAs and D_FULL)
+            if (turn == wg) s_f[rf.slot * 128 + r] = real ? pow2(127 + e - 141 + 24) : pow2(127 + e - 135);
+            // one group's operand into the next slot of TMEM
+            auto put = [&](const uint32_t (&a)[32]) {
+                ok = __all_sync(0xffffffffu, ahead < kA || bar_wait(bar(BAR_A_EMPTY + ra.slot), ra.phase ^ 1, abortp));
+                if (!ok) return;
                 tc_fence_after();
                 tc_st32(tmem + lanes + L::colA + (uint32_t)ra.slot * 32, a);
                 tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(BAR_A_FULL + ra.slot));
+            };
+            if (real) {
+                const float up = pow2(127 + 141 - e);  // the largest scale comes to [2^14, 2^15)
+                const uint32_t wrow = sW + (uint32_t)rw.slot * kWSlot + (uint32_t)r * 128u;
+                for (int j = 0; j < na && ok; j++, ra.next(), turn ^= 1, ahead = min(ahead + 1, kA)) {
+                    if (turn != wg) continue;
+                    const float mf = __uint_as_float(((j & 2 ? sc.y : sc.x) >> ((j & 1) * 16)) << 16) * up;
+                    const uint32_t m = dup_h2(mf), m16 = dup_h2(mf * 0.0625f), mc = dup_h2(mf * -0x1p-21f);
+                    uint32_t a[32];
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const uint4 w4 = ld_shared16(wrow + (uint32_t)(((2 * j + h) ^ (r & 7)) << 4));
+                        widen_word(w4.x, m, m16, mc, a + h * 16);
+                        widen_word(w4.y, m, m16, mc, a + h * 16 + 4);
+                        widen_word(w4.z, m, m16, mc, a + h * 16 + 8);
+                        widen_word(w4.w, m, m16, mc, a + h * 16 + 12);
+                    }
+                    put(a);
+                }
+            } else {
+                for (int j = 0; j < 2 && ok; j++, ra.next(), turn ^= 1, ahead = min(ahead + 1, kA))
+                    if (turn == wg) put(pw);
             }
             const int used = real ? 1 : g.wide ? 2 : 0;  // weight slots of the step
             for (int k = 0; k < used; k++) {
@@ -480,7 +545,7 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
             for (int c = 0; c < nchunks && ok; c++) {
                 const bool last = c == nchunks - 1;
                 for (int i = 0; i < un.tiles && ok; i++) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(bar(BAR_D_FULL + rd.slot), rd.phase, abortp));
+                    ok = __all_sync(0xffffffffu, bar_wait(bar(BAR_D_FULL + rd.slot), rd.phase, abortp));
                     if (!ok) break;
                     tc_fence_after();
                     const float f = s_f[rf.slot * 128 + r];
@@ -497,8 +562,15 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
                     if (lane == 0) mbar_arrive(bar(BAR_D_EMPTY + rd.slot));
                     rd.next();
                     if (live <= 0) continue;
+                    if (c > 0) {
+                        uint64_t ff;
+                        asm("mov.b64 %0, {%1, %1};\n" : "=l"(ff) : "f"(f));
 #pragma unroll
-                    for (int k = 0; k < 32; k++) d[k] = __float_as_uint(fmaf(__uint_as_float(d[k]), f, c > 0 ? __uint_as_float(s[k]) : 0.f));
+                        for (int k = 0; k < 32; k += 2) fma_f32x2(d[k], d[k + 1], ff, s[k], s[k + 1]);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 32; k++) d[k] = __float_as_uint(__uint_as_float(d[k]) * f);
+                    }
                     if (!last || (MODE == kGateUp && !(i & 1))) {
                         tc_st32(tsum, d);
                         tc_wait_st();
