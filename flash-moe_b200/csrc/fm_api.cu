@@ -1105,7 +1105,7 @@ extern "C" fm_status fm_proj_forward(FmCtx *ctx, int count, const FmProjWeights 
         if (!gemm) {
             st = launched(ctx, launch_q4_stream(kProj, p, ctx->sm_count, ctx->stream), "proj_forward");
         } else {
-            st = launched(ctx, launch_q4_split(p.x, n, p.in_dim, nullptr, xs, tscale, ctx->stream), "proj_forward split");
+            st = launched(ctx, launch_q4_split(p.x, n, p.in_dim, nullptr, nullptr, 1, xs, tscale, ctx->stream), "proj_forward split");
             if (st == FM_OK) st = launched(ctx, launch_q4_gemm(kProj, p, xs, n, tscale, ctx->d_err, ctx->sm_count, ctx->stream), "proj_forward");
         }
     }
@@ -1198,8 +1198,8 @@ extern "C" fm_status fm_moe_experts(FmCtx *ctx, const FmExpertWeights *w, int n,
         hbuf = cv.take<float>(pairs * I);
         ybuf = cv.take<float>(pairs * H);
         if (gemm) {
-            xs = cv.take<uint16_t>((size_t)n * 2 * q4_split_columns(w->hidden));
-            xscale = cv.take<float>((size_t)n);
+            xs = cv.take<uint16_t>(pairs * 2 * q4_split_columns(w->hidden));
+            xscale = cv.take<float>(pairs);
             hs = cv.take<uint16_t>(pairs * 2 * q4_split_columns(w->inter));
             hscale = cv.take<float>(pairs);
         }
@@ -1236,11 +1236,11 @@ extern "C" fm_status fm_moe_experts(FmCtx *ctx, const FmExpertWeights *w, int n,
             if (st) return st;
             st = launched(ctx, launch_q4_stream(kDown, dn, ctx->sm_count, ctx->stream), "moe down");
         } else {
-            st = launched(ctx, launch_q4_split(d_x, n, w->hidden, nullptr, xs, xscale, ctx->stream), "moe split");
+            st = launched(ctx, launch_q4_split(d_x, (int)pairs, w->hidden, plan.njobs + 1, plan.pair_of, top_k, xs, xscale, ctx->stream), "moe split");
             if (st) return st;
-            st = launched(ctx, launch_q4_gemm(kGateUp, gu, xs, n, xscale, ctx->d_err, ctx->sm_count, ctx->stream), "moe gate_up");
+            st = launched(ctx, launch_q4_gemm(kGateUp, gu, xs, (int)pairs, xscale, ctx->d_err, ctx->sm_count, ctx->stream), "moe gate_up");
             if (st) return st;
-            st = launched(ctx, launch_q4_split(hbuf, (int)pairs, w->inter, plan.njobs + 1, hs, hscale, ctx->stream), "moe split");
+            st = launched(ctx, launch_q4_split(hbuf, (int)pairs, w->inter, plan.njobs + 1, nullptr, 1, hs, hscale, ctx->stream), "moe split");
             if (st) return st;
             st = launched(ctx, launch_q4_gemm(kDown, dn, hs, (int)pairs, hscale, ctx->d_err, ctx->sm_count, ctx->stream), "moe down");
         }

@@ -319,12 +319,13 @@ struct Q4Params {
 };
 // Few tokens per matrix: the weights stream past the activations once per job of up to 2 * ntl tokens (q4_stream.cu).
 int launch_q4_stream(Q4Mode mode, const Q4Params &p, int sm_count, cudaStream_t st);
-// Many tokens per matrix: tcgen05 (q4_gemm.cu).  xs, tscale: what launch_q4_split left of the activations -- of p.x for
-// kProj and kGateUp (by token), of the h rows for kDown (sorted, like pair_of); with experts h comes out sorted and y by pair
-// number.  plan.jobs hold up to 64 pairs.  err: the context's error word.
-constexpr int kGemmTokens = 64;
+// Many tokens per matrix: tcgen05 (q4_gemm.cu).  xs, tscale: what launch_q4_split left of the activations, one row per token
+// (kProj) or per pair in pair_of's order; h comes out in that order, y by pair number.  plan.jobs hold up to kGemmTokens
+// pairs.  err: the context's error word.
+constexpr int kGemmTokens = 96;
 int q4_split_columns(int in_dim);  // fp16 numbers per term and row
-int launch_q4_split(const float *x, int rows, int in_dim, const int *count, void *xs, float *tscale, cudaStream_t st);
+// rows of x (count: how many of them exist, on the device, or null; source: row i is row source[i] / per of x, or null)
+int launch_q4_split(const float *x, int rows, int in_dim, const int *count, const int *source, int per, void *xs, float *tscale, cudaStream_t st);
 int launch_q4_gemm(Q4Mode mode, const Q4Params &p, const void *xs, int xs_rows, const float *tscale, int *err, int sm_count, cudaStream_t st);
 // Which pairs go to which expert, in runs of `tile` (moe_plan.cu)
 int launch_moe_plan(const int *ids, int pairs, int first_expert, int num_experts, int tile, const MoePlan &plan, cudaStream_t st);

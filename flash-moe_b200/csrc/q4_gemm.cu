@@ -20,8 +20,7 @@
 //                the MMA wants it, and half of the shared-memory traffic of an A tile there.
 //   warps 8-15   epilogue: running sums in TMEM, added up per step; the last step of a tile writes the results, 128
 //                consecutive features per token and store
-//   warp 16      TMA producer: weight tiles [128 rows][128 bytes], token tiles hi | lo (kGateUp: gathered by token, 4 rows per
-//                instruction)
+//   warp 16      TMA producer of token tiles, hi | lo;  warp 18  of weight tiles [128 rows][128 bytes]
 //   warp 17      issues the MMAs (M128, N = the unit's tokens rounded up to 16, K16)
 // TMEM columns: T * 64 running sums, 2 * 64 of steps in flight, the rest operand A in slots of 32.
 // With two terms the tensor work is twice the product's; what bounds a long prompt is that, a short one the weights' stream.
@@ -41,17 +40,18 @@ namespace fm {
 
 namespace {
 
-constexpr int kTok = 64;                    // tokens per unit
+constexpr int kTok = kGemmTokens;           // tokens per unit (96)
 constexpr int kChunk = 4;                   // groups per step
 constexpr int kBSlot = 2 * kTok * 128;      // bytes of a token tile: one group, hi then lo
-constexpr int kBSlots = 8;
+constexpr int kBSlots = 6;
 constexpr int kWSlot = 128 * 128;           // bytes of a weight tile: 128 rows, 4 groups
-constexpr int kWSlots = 5;
-constexpr int kGemmThreads = 18 * 32;
+constexpr int kWSlots = 4;
+constexpr int kGemmThreads = 19 * 32;
 constexpr int kDBufs = 2;
 // Steps whose row factors are kept: the widening warps are at most the operand slots (8, one to a step at the least), the
 // steps in flight and their own step ahead of the epilogue.
 constexpr int kFSteps = 16;
+constexpr int kHalf = kTok / 2;            // columns of an epilogue warp
 constexpr uint32_t kColStep = 0, kColSum = kDBufs * kTok;  // TMEM columns; operand A behind the sums
 
 template <int T>
@@ -84,14 +84,14 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map
                  "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
                  : "memory");
 }
-// four rows of a 2-D tensor, one 128-byte piece of each
-__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap *map, int x, int4 rows, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];\n" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(rows.x), "r"(rows.y), "r"(rows.z), "r"(rows.w), "r"(bar)
-        : "memory");
+// 32 lanes x 16 consecutive 32-bit columns
+__device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr)
+                 : "memory");
 }
-
 // True in one lane of the warp, the same one for every call.
 __device__ __forceinline__ bool elect_one() {
     uint32_t one;
@@ -120,7 +120,7 @@ struct Unit {
     int start, cnt, ncols; // tokens (kProj) or positions in pair_of; columns of the MMA
 };
 
-template <Q4Mode MODE, int T>
+template <Q4Mode MODE, int T, bool WARP = true>
 __device__ __forceinline__ Unit unit_at(const GemmParams &g, int u) {
     Unit r;
     const int job = u / g.units_per_job;
@@ -132,7 +132,8 @@ __device__ __forceinline__ Unit unit_at(const GemmParams &g, int u) {
         r.cnt = min(kTok, g.p.n - r.start);
     } else {
         const int4 j = g.p.plan.jobs[job];
-        r.expert = uniform(j.x); r.start = uniform(j.y); r.cnt = uniform(j.z);
+        if constexpr (WARP) { r.expert = uniform(j.x); r.start = uniform(j.y); r.cnt = uniform(j.z); }
+        else { r.expert = j.x; r.start = j.y; r.cnt = j.z; }
     }
     constexpr int kRows = MODE == kGateUp ? T * 64 : T * 128;
     r.row0 = mu * kRows;
@@ -265,6 +266,15 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
     const int njobs = MODE == kProj ? (g.p.n + kTok - 1) / kTok : uniform(*g.p.plan.njobs);
     const int nunits = njobs * g.units_per_job;
     const size_t s_pitch = (size_t)G * 2;
+    // after a wait that ran out: the copies in flight land before the CTA goes (a ring's last `count` loads)
+    auto drain = [&](int first, int n, int slot, uint32_t phase, int count) {
+        const long long t0 = clock64();
+        for (int i = 0; i < count; i++) {
+            if (slot == 0) { slot = n; phase ^= 1; }
+            slot--;
+            while (!mbar_try(bar(first + slot), phase) && clock64() - t0 < 200000000LL) {}
+        }
+    };
     // one thread's row of a tile: its scales and biases (rows beyond the matrix read the last one; their results are dropped)
     auto row_ptr = [&](const Unit &u, int tile, int r, bool biases) {
         const Q4View &m = g.p.mat[tile_mat<MODE>(u, tile)];
@@ -274,77 +284,54 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
     };
 
     if (warp == 16) {
-        // ================= TMA producer =================
-        Ring<kWSlots> rw;
+        // ================= TMA producer: tokens =================
         Ring<kBSlots> rb;
-        int wcount = 0, bcount = 0;
+        int count = 0;
         bool ok = true;
         for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x) {
             const Unit un = unit_at<MODE, T>(g, u);
-            int4 tok = make_int4(0, 0, 0, 0);
-            if constexpr (MODE == kGateUp) {  // lane l < 16: tokens of columns 4 l .. 4 l + 3 (columns without one repeat the first)
-                auto token = [&](int c) { return g.p.plan.pair_of[un.start + (c < un.cnt ? c : 0)] / g.p.top_k; };
-                if (lane < 16) tok = make_int4(token(4 * lane), token(4 * lane + 1), token(4 * lane + 2), token(4 * lane + 3));
-            }
-            for (int c = 0; c < nchunks && ok; c++) {
-                const int ng = c < nreal ? min(kChunk, G - c * kChunk) : 1;
-                auto load_b = [&](int grp) {  // grp: 64 columns of x
-                    if (lane == 0) ok = bcount < kBSlots || bar_wait(bar(BAR_B_EMPTY + rb.slot), rb.phase ^ 1, abortp);
-                    ok = __shfl_sync(0xffffffffu, ok, 0);
-                    if (!ok) return;
-                    const uint32_t full = bar(BAR_B_FULL + rb.slot), dst = sB + (uint32_t)rb.slot * kBSlot;
-                    if (lane == 0) mbar_expect_tx(full, (uint32_t)un.ncols * 256u);
-                    __syncwarp();
-                    if constexpr (MODE == kGateUp) {
-                        if (lane * 4 < un.ncols) {
-                            tma_gather4(dst + (uint32_t)lane * 512u, &maps.x, grp * 64, tok, full);
-                            tma_gather4(dst + kTok * 128u + (uint32_t)lane * 512u, &maps.x, g.kp + grp * 64, tok, full);
-                        }
-                    } else {
-                        if (lane * 16 < un.ncols) {
-                            tma_load_2d(dst + (uint32_t)lane * 2048u, &maps.x, grp * 64, un.start + lane * 16, full);
-                            tma_load_2d(dst + kTok * 128u + (uint32_t)lane * 2048u, &maps.x, g.kp + grp * 64, un.start + lane * 16, full);
-                        }
-                    }
-                    rb.next(); bcount = min(bcount + 1, kBSlots);
-                };
-                auto load_w = [&](const CUtensorMap *map, int x, int tile) {  // 128 bytes of each of the tile's rows
-                    if (lane == 0) ok = wcount < kWSlots || bar_wait(bar(BAR_W_EMPTY + rw.slot), rw.phase ^ 1, abortp);
-                    ok = __shfl_sync(0xffffffffu, ok, 0);
-                    if (!ok) return;
-                    if (lane == 0) {
-                        mbar_expect_tx(bar(BAR_W_FULL + rw.slot), kWSlot);
-                        tma_load_3d(sW + (uint32_t)rw.slot * kWSlot, map, x, tile_row<MODE>(un, tile), un.expert, bar(BAR_W_FULL + rw.slot));
-                    }
-                    rw.next(); wcount = min(wcount + 1, kWSlots);
-                };
-                auto load_tile = [&](int tile) {
-                    const int m = tile_mat<MODE>(un, tile);
-                    if (c < nreal) load_w(&maps.w[m], c * 32, tile);
-                    else if (g.wide) {
-                        load_w(&maps.s[m], (c - nreal) * 64, tile);
-                        if (ok) load_w(&maps.b[m], (c - nreal) * 64, tile);
-                    }
-                };
-                // in the order they are wanted: the first tile, the chunk's tokens, the other tiles
-                load_tile(0);
-                for (int j = 0; j < ng && ok; j++) load_b(c < nreal ? c * kChunk + j : G + c - nreal);
-                for (int i = 1; i < un.tiles && ok; i++) load_tile(i);
-            }
-        }
-        // the copies in flight land before the CTA goes (they have, unless a wait ran out)
-        if (lane == 0 && *abortp) {
-            const long long t0 = clock64();
-            auto drain = [&](int first, int n, auto r, int count) {
-                for (int i = 0; i < count; i++) {
-                    if (r.slot == 0) { r.slot = n; r.phase ^= 1; }
-                    r.slot--;
-                    while (!mbar_try(bar(first + r.slot), r.phase) && clock64() - t0 < 200000000LL) {}
+            for (int grp = 0; grp < G + g.pseudo && ok; grp++) {  // 64 columns of x at a time
+                ok = __all_sync(0xffffffffu, count < kBSlots || bar_wait(bar(BAR_B_EMPTY + rb.slot), rb.phase ^ 1, abortp));
+                if (!ok) break;
+                const uint32_t full = bar(BAR_B_FULL + rb.slot), dst = sB + (uint32_t)rb.slot * kBSlot;
+                if (lane == 0) mbar_expect_tx(full, (uint32_t)un.ncols * 256u);
+                __syncwarp();
+                if (lane * 16 < un.ncols) {
+                    tma_load_2d(dst + (uint32_t)lane * 2048u, &maps.x, grp * 64, un.start + lane * 16, full);
+                    tma_load_2d(dst + kTok * 128u + (uint32_t)lane * 2048u, &maps.x, g.kp + grp * 64, un.start + lane * 16, full);
                 }
-            };
-            drain(BAR_W_FULL, kWSlots, rw, wcount);
-            drain(BAR_B_FULL, kBSlots, rb, bcount);
+                rb.next(); count = min(count + 1, kBSlots);
+            }
         }
+        if (lane == 0 && *abortp) drain(BAR_B_FULL, kBSlots, rb.slot, rb.phase, count);
+    } else if (warp == 18) {
+        // ================= TMA producer: weights =================
+        if (lane == 0) {
+            Ring<kWSlots> rw;
+            int count = 0;
+            bool ok = true;
+            for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x) {
+                const Unit un = unit_at<MODE, T, false>(g, u);
+                for (int c = 0; c < nchunks && ok; c++)
+                    for (int i = 0; i < un.tiles && ok; i++) {
+                        auto load = [&](const CUtensorMap *map, int x) {  // 128 bytes of each of the tile's rows
+                            ok = count < kWSlots || bar_wait(bar(BAR_W_EMPTY + rw.slot), rw.phase ^ 1, abortp);
+                            if (!ok) return;
+                            mbar_expect_tx(bar(BAR_W_FULL + rw.slot), kWSlot);
+                            tma_load_3d(sW + (uint32_t)rw.slot * kWSlot, map, x, tile_row<MODE>(un, i), un.expert, bar(BAR_W_FULL + rw.slot));
+                            rw.next(); count = min(count + 1, kWSlots);
+                        };
+                        const int m = tile_mat<MODE>(un, i);
+                        if (c < nreal) load(&maps.w[m], c * 32);
+                        else if (g.wide) {
+                            load(&maps.s[m], (c - nreal) * 64);
+                            if (ok) load(&maps.b[m], (c - nreal) * 64);
+                        }
+                    }
+            }
+            if (*abortp) drain(BAR_W_FULL, kWSlots, rw.slot, rw.phase, count);
+        }
+        __syncwarp();
     } else if (warp == 17) {
         // ================= MMA issuer =================
         // The whole warp walks the steps and one elected lane issues a slot's MMAs in one go: everything they read is then
@@ -377,10 +364,19 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
                         const uint64_t hi = smem_desc(b, 0, 1024), lo = smem_desc(b + kTok * 128, 0, 1024);
                         const bool done_b = i == tiles - 1 && (real || j == na - 1);
                         if (elect_one()) {
+                            // the bias block holds one column per group, and only steps of 16 columns that have some
+                            if (real) {
 #pragma unroll
-                            for (int k = 0; k < 4; k++) tc_mma_f16_ta(d, a + k * 8, lo + k * 2, idesc, j > 0 || k > 0);
+                                for (int k = 0; k < 4; k++) tc_mma_f16_ta(d, a + k * 8, lo + k * 2, idesc, j > 0 || k > 0);
 #pragma unroll
-                            for (int k = 0; k < 4; k++) tc_mma_f16_ta(d, a + k * 8, hi + k * 2, idesc, 1);
+                                for (int k = 0; k < 4; k++) tc_mma_f16_ta(d, a + k * 8, hi + k * 2, idesc, 1);
+                            } else {
+                                const int nk = (min(64, G - (c - nreal) * 64) + 15) / 16;
+                                for (int k = 0; k < nk; k++) {
+                                    tc_mma_f16_ta(d, a + k * 8, lo + k * 2, idesc, j > 0 || k > 0);
+                                    tc_mma_f16_ta(d, a + k * 8, hi + k * 2, idesc, 1);
+                                }
+                            }
                             tc_commit(bar(BAR_A_EMPTY + ra.slot));
                             if (done_b) tc_commit(bar(BAR_B_EMPTY + rt.slot));
                             if (j == na - 1) tc_commit(bar(BAR_D_FULL + rd.slot));
@@ -450,6 +446,11 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
                     if (!ok) break;
 #pragma unroll
                     for (int q = 0; q < 8; q++) {
+                        if (q * 8 >= gn) {
+#pragma unroll
+                            for (int k = 0; k < 8; k++) v[8 * q + k] = 0.f;
+                            continue;
+                        }
                         const uint4 s4 = ld_shared16(srow + (uint32_t)((q ^ (r & 7)) << 4)), b4 = ld_shared16(brow + (uint32_t)((q ^ (r & 7)) << 4));
                         const uint32_t sw[4] = {s4.x, s4.y, s4.z, s4.w}, bw[4] = {b4.x, b4.y, b4.z, b4.w};
 #pragma unroll
@@ -524,75 +525,83 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
         }
     } else {
         // ================= epilogue =================
-        const int r = (warp & 3) * 32 + lane, half = (warp - 8) >> 2;
+        const int r = (warp & 3) * 32 + lane, half = (warp - 8) >> 2;  // columns half * 48 .. + 47
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;
         Ring<kDBufs> rd;
         Ring<kFSteps> rf;
         bool ok = true;
         for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x) {
             const Unit un = unit_at<MODE, T>(g, u);
-            // column `half * 32 + lane`: the row of the output it goes to, and what takes its token's power of two off again
-            const int col = half * 32 + lane;
-            const bool there = col < un.cnt;
-            long long out_row = 0;
-            float ts = 0.f;
-            if (there) {
-                if constexpr (MODE == kProj) { out_row = un.start + col; ts = __ldg(g.tscale + un.start + col); }
-                if constexpr (MODE == kGateUp) { out_row = un.start + col; ts = __ldg(g.tscale + g.p.plan.pair_of[un.start + col] / g.p.top_k); }
-                if constexpr (MODE == kDown) { out_row = g.p.plan.pair_of[un.start + col]; ts = __ldg(g.tscale + un.start + col); }
+            // columns half * 48 + 32 q + lane: the row of the output it goes to, and what takes its token's power of two off again
+            int out_row[2] = {0, 0};
+            float ts[2] = {0.f, 0.f};
+#pragma unroll
+            for (int q = 0; q < 2; q++) {
+                const int col = half * kHalf + q * 32 + lane;
+                if (col >= un.cnt || q * 32 + lane >= kHalf) continue;
+                out_row[q] = MODE == kDown ? g.p.plan.pair_of[un.start + col] : un.start + col;
+                ts[q] = __ldg(g.tscale + un.start + col);
             }
-            const int live = min(32, un.cnt - half * 32);  // columns of this warp
+            const int live = un.cnt - half * kHalf;  // columns of this warp that are tokens
             for (int c = 0; c < nchunks && ok; c++) {
                 const bool last = c == nchunks - 1;
                 for (int i = 0; i < un.tiles && ok; i++) {
                     ok = __all_sync(0xffffffffu, bar_wait(bar(BAR_D_FULL + rd.slot), rd.phase, abortp));
                     if (!ok) break;
                     tc_fence_after();
-                    const float f = s_f[rf.slot * 128 + r];
-                    rf.next();
-                    uint32_t d[32], s[32];
-                    const uint32_t tsum = tmem + lanes + kColSum + (uint32_t)i * kTok + (uint32_t)half * 32;
+                    uint32_t d[3][16];
+                    const uint32_t tstep = tmem + lanes + kColStep + (uint32_t)(rd.slot * kTok + half * kHalf);
+                    const uint32_t tsum = tmem + lanes + kColSum + (uint32_t)(i * kTok + half * kHalf);
                     if (live > 0) {
-                        tc_ld32(tmem + lanes + kColStep + (uint32_t)rd.slot * kTok + (uint32_t)half * 32, d);
-                        if (c > 0) tc_ld32(tsum, s);
+                        tc_ld16(tstep, d[0]);
+                        if (live > 16) tc_ld16(tstep + 16, d[1]);
+                        if (live > 32) tc_ld16(tstep + 32, d[2]);
                         tc_wait_ld();
                     }
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bar(BAR_D_EMPTY + rd.slot));
+                    const float f = s_f[rf.slot * 128 + r];
+                    rf.next();
                     rd.next();
-                    if (live <= 0) continue;
-                    if (c > 0) {
-                        uint64_t ff;
-                        asm("mov.b64 %0, {%1, %1};\n" : "=l"(ff) : "f"(f));
-#pragma unroll
-                        for (int k = 0; k < 32; k += 2) fma_f32x2(d[k], d[k + 1], ff, s[k], s[k + 1]);
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < 32; k++) d[k] = __float_as_uint(__uint_as_float(d[k]) * f);
-                    }
-                    if (!last || (MODE == kGateUp && !(i & 1))) {
-                        tc_st32(tsum, d);
-                        tc_wait_st();
-                        continue;
-                    }
-                    if constexpr (MODE == kGateUp) {  // the gate's sums wait one tile to the left
-                        tc_ld32(tsum - kTok, s);
-                        tc_wait_ld();
-                    }
+                    uint64_t ff;
+                    asm("mov.b64 %0, {%1, %1};\n" : "=l"(ff) : "f"(f));
                     const int row = tile_row<MODE>(un, i) + r;
-                    float *out = g.p.out[MODE == kProj ? un.mat : 0];
+                    float *out = g.p.out[MODE == kProj ? un.mat : 0] + row;
 #pragma unroll
-                    for (int k = 0; k < 32; k++) {
-                        const long long o = __shfl_sync(0xffffffffu, out_row, k);
-                        const float t = __shfl_sync(0xffffffffu, ts, k);
-                        float v = __uint_as_float(d[k]) * t;
-                        if constexpr (MODE == kGateUp) {
-                            const float a = __uint_as_float(s[k]) * t;
-                            v = a / (1.f + expf(-a)) * v;
+                    for (int q = 0; q < 3; q++) {  // 16 columns at a time
+                        if (live <= q * 16) break;
+                        uint32_t (&v)[16] = d[q], s[16];
+                        if (c > 0) {
+                            tc_ld16(tsum + q * 16, s);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int k = 0; k < 16; k += 2) fma_f32x2(v[k], v[k + 1], ff, s[k], s[k + 1]);
+                        } else {
+#pragma unroll
+                            for (int k = 0; k < 16; k++) v[k] = __float_as_uint(__uint_as_float(v[k]) * f);
                         }
-                        if (k < live && row < un.rows) out[o * un.rows + row] = v;
+                        if (!last || (MODE == kGateUp && !(i & 1))) {
+                            tc_st16(tsum + q * 16, v);
+                            continue;
+                        }
+                        if constexpr (MODE == kGateUp) {  // the gate's sums wait one tile to the left
+                            tc_ld16(tsum + q * 16 - kTok, s);
+                            tc_wait_ld();
+                        }
+#pragma unroll
+                        for (int k = 0; k < 16; k++) {
+                            const int o = __shfl_sync(0xffffffffu, out_row[q >> 1], (q & 1) * 16 + k);
+                            const float t = __shfl_sync(0xffffffffu, ts[q >> 1], (q & 1) * 16 + k);
+                            float y = __uint_as_float(v[k]) * t;
+                            if constexpr (MODE == kGateUp) {
+                                const float a = __uint_as_float(s[k]) * t;
+                                y = a / (1.f + expf(-a)) * y;
+                            }
+                            if (q * 16 + k < live && row < un.rows) out[(size_t)o * un.rows] = y;
+                        }
                     }
+                    tc_wait_st();
                 }
             }
         }
@@ -608,16 +617,17 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
 
 // Rows of fp32 activations -> two fp16 terms each, brought into range by a power of two per row, in the order the widened
 // words have along K (0 4 1 5 2 6 3 7 of every eight); behind them the sums of every 64 inputs, likewise in two terms.
-// One CTA per row.
+// One CTA per row of the result; `source` (may be null): row i is row source[i] / per of x.
 __global__ void __launch_bounds__(256)
-q4_split_kernel(const float *__restrict__ x, int K, int kp, const int *count, __half *__restrict__ xs, float *__restrict__ tscale) {
+q4_split_kernel(const float *__restrict__ x, int K, int kp, const int *count, const int *source, int per, __half *__restrict__ xs,
+                float *__restrict__ tscale) {
     __shared__ float s_red[8], s_sum[8];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     const size_t row = blockIdx.x;
     if (count != nullptr && (int)row >= *count) return;
-    const float4 *src = reinterpret_cast<const float4 *>(x + row * K);
+    const float4 *src = reinterpret_cast<const float4 *>(x + (source != nullptr ? (size_t)(source[row] / per) : row) * K);
     float am = 0.f, sum = 0.f;
     for (int i = tid; i < K / 4; i += 256) {
         const float4 v = __ldg(src + i);
@@ -702,9 +712,9 @@ int launch_gemm(const GemmMaps &maps, GemmParams &g, long long jobs, int sm_coun
 
 int q4_split_columns(int in_dim) { return in_dim + (in_dim / 64 + 63) / 64 * 64; }
 
-int launch_q4_split(const float *x, int rows, int in_dim, const int *count, void *xs, float *tscale, cudaStream_t st) {
-    return launch_dependent(q4_split_kernel, dim3(rows), dim3(256), 0, st, x, in_dim, q4_split_columns(in_dim), count, reinterpret_cast<__half *>(xs), tscale) ==
-                   cudaSuccess ? 1 : -1;
+int launch_q4_split(const float *x, int rows, int in_dim, const int *count, const int *source, int per, void *xs, float *tscale, cudaStream_t st) {
+    return launch_dependent(q4_split_kernel, dim3(rows), dim3(256), 0, st, x, in_dim, q4_split_columns(in_dim), count, source, per,
+                            reinterpret_cast<__half *>(xs), tscale) == cudaSuccess ? 1 : -1;
 }
 
 int launch_q4_gemm(Q4Mode mode, const Q4Params &p, const void *xs, int xs_rows, const float *tscale, int *err, int sm_count, cudaStream_t st) {
@@ -722,11 +732,11 @@ int launch_q4_gemm(Q4Mode mode, const Q4Params &p, const void *xs, int xs_rows, 
                        !map_rows(&maps.b[i], m.biases, m.s_stride, m.rows, g.G * 2, matrices, false)))
             return -1;
     }
-    if (!make_map_2d(&maps.x, xs, (uint64_t)xs_rows, (uint64_t)2 * g.kp, mode == kGateUp ? 1 : 16, false)) return -1;
+    if (!make_map_2d(&maps.x, xs, (uint64_t)xs_rows, (uint64_t)2 * g.kp, 16, false)) return -1;
     const long long jobs = mode == kProj ? (p.n + kTok - 1) / kTok : (long long)p.n * p.top_k;
-    if (mode == kProj) return launch_gemm<kProj, 4>(maps, g, jobs, sm_count, st);
-    if (mode == kGateUp) return launch_gemm<kGateUp, 4>(maps, g, jobs, sm_count, st);
-    return launch_gemm<kDown, 4>(maps, g, jobs, sm_count, st);
+    if (mode == kProj) return launch_gemm<kProj, 2>(maps, g, jobs, sm_count, st);
+    if (mode == kGateUp) return launch_gemm<kGateUp, 2>(maps, g, jobs, sm_count, st);
+    return launch_gemm<kDown, 2>(maps, g, jobs, sm_count, st);
 }
 
 }  // namespace fm
