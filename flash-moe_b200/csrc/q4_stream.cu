@@ -31,7 +31,6 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kDepth = 4;        // weight groups a warp has in flight
 constexpr int kTiles = 2;        // 16-row tiles per unit
 constexpr int kTokBytes = 256;   // a token's group as bytes: 64 inputs x 4
 constexpr int kFactorBytes = 32; // per group and pair of tokens: (factor, input sum) for each of the four lanes of a quad
@@ -42,12 +41,6 @@ __device__ __forceinline__ void mma_u8s8(int (&d)[4], uint32_t a0, uint32_t a1, 
         : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-
-// Row sources of a unit: where its two tiles start.
-struct Rows {
-    const unsigned char *w[kTiles], *s[kTiles], *b[kTiles];  // first row of the tile
-    int rows[kTiles];                                        // rows of the tile that exist (0..16)
-};
 
 // Eight inputs (those of one weight word) of a token -> fixed point bytes in the order of the B fragments.
 // The eight threads of a group of 64 inputs sit in consecutive lanes.
@@ -100,105 +93,141 @@ __device__ __forceinline__ void widen8(const float *x, bool valid, unsigned char
     if (wi < 2) factor[wi] = make_float2(wi == 0 ? down * 65536.f : down, sum);
 }
 
-template <Q4Mode MODE, int NTL>
+// S groups of a row pair as a lane holds them: 8 bytes of words per group and row, the scales of rows g and g + 8, and the
+// bias of row g (even lanes) or g + 8 (odd lanes).
+template <int S>
+struct Held {
+    uint2 w[kTiles][2][S];
+    uint32_t sc[kTiles][2][(S + 1) / 2], bi[kTiles][(S + 1) / 2];
+};
+template <int S>
+__device__ __forceinline__ void load_bf16s(uint32_t (&d)[(S + 1) / 2], const unsigned char *p) {
+    if constexpr (S == 4) {
+        const uint2 v = __ldg(reinterpret_cast<const uint2 *>(p));
+        d[0] = v.x; d[1] = v.y;
+    } else {
+        d[0] = __ldg(reinterpret_cast<const uint16_t *>(p));
+    }
+}
+__device__ __forceinline__ float bf16_at(uint32_t pair, int j) { return __uint_as_float(j & 1 ? pair & 0xffff0000u : pair << 16); }
+// The same value in every lane, and known to the compiler as such (values of at least 0).
+__device__ __forceinline__ int uniform(int v) { return __reduce_max_sync(0xffffffffu, v); }
+
+// Warps: WK of them side by side along a row's steps (S groups each), 8 / WK along the rows.
+template <Q4Mode MODE, int NTL, int S>
 __global__ void __launch_bounds__(kThreads, NTL == 4 ? 1 : 2)
-q4_stream_kernel(Q4Params p, int chunk_groups, int units_per_job, int fixed_jobs) {
+q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units_per_job, int fixed_jobs, int wk_log2) {
     extern __shared__ __align__(16) unsigned char smem[];
     constexpr int kTok = 2 * NTL;
     unsigned char *s_b = smem;                                                                      // [NTL][2 tokens][chunk][256]
     float2 *s_f = reinterpret_cast<float2 *>(smem + (size_t)kTok * chunk_groups * kTokBytes);       // [NTL][chunk][4]
     float *s_red = reinterpret_cast<float *>(reinterpret_cast<unsigned char *>(s_f) + (size_t)NTL * chunk_groups * kFactorBytes);  // [2][warp][tok][32 rows]
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int WK = 1 << wk_log2, wk = warp & (WK - 1), wr = warp >> wk_log2, rows_unit = (MODE == kGateUp ? 16 : 32) * (kWarps >> wk_log2);
     const int G = p.in_dim / 64;
-    const size_t w_pitch = (size_t)G * 32, s_pitch = (size_t)G * 2;
+    const uint32_t w_pitch = (uint32_t)G * 32, s_pitch = (uint32_t)G * 2;
     const int nchunks = (G + chunk_groups - 1) / chunk_groups;
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
-    const int njobs = p.plan.njobs != nullptr ? *p.plan.njobs : fixed_jobs;
+    const int njobs = p.plan.njobs != nullptr ? uniform(*p.plan.njobs) : fixed_jobs;
     const long long units = (long long)njobs * units_per_job;
     const long long u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1) / gridDim.x;
 
-    auto job_of = [&](int job, int &expert, int &start, int &cnt) {
-        if constexpr (MODE == kProj) {
-            expert = 0; start = job * kTok; cnt = min(kTok, p.n - start);
-        } else if (p.plan.njobs != nullptr) {
-            const int4 j = p.plan.jobs[job];
-            expert = j.x; start = j.y; cnt = j.z;
-        } else {
-            expert = local_expert(p.ids[job], p.first_expert, p.num_experts); start = job; cnt = expert >= 0 ? 1 : 0;
-        }
+    struct Unit {
+        int job, expert, start, cnt, mat, row0;
     };
     auto pair_at = [&](int start, int i) { return MODE == kProj ? start + i : p.plan.njobs != nullptr ? p.plan.pair_of[start + i] : start; };
-    // the unit's matrix (kProj) and first row in it
-    auto where = [&](int rb, int &mat, int &row0) {
-        mat = 0;
-        if constexpr (MODE == kGateUp) {
-            row0 = rb * 16;
-        } else {
-            if constexpr (MODE == kProj)
-                while (rb >= (p.mat[mat].rows + 31) / 32) rb -= (p.mat[mat++].rows + 31) / 32;
-            row0 = rb * 32;
+    auto unit_at = [&](long long u) {
+        Unit r;
+        r.job = (int)(u / units_per_job);
+        int rb = (int)(u - (long long)r.job * units_per_job);
+        r.mat = 0;
+        if constexpr (MODE == kProj) {
+            r.expert = 0; r.start = r.job * kTok; r.cnt = min(kTok, p.n - r.start);
+            while (rb >= (p.mat[r.mat].rows + rows_unit - 1) / rows_unit) rb -= (p.mat[r.mat++].rows + rows_unit - 1) / rows_unit;
+        } else if (p.plan.njobs != nullptr) {
+            const int4 j = p.plan.jobs[r.job];
+            r.expert = uniform(j.x); r.start = uniform(j.y); r.cnt = uniform(j.z);
+        } else {  // -1: a slot without an expert here
+            r.expert = uniform(local_expert(p.ids[r.job], p.first_expert, p.num_experts) + 1) - 1;
+            r.start = r.job; r.cnt = r.expert >= 0 ? 1 : 0;
         }
-    };
-    auto rows_of = [&](int expert, int mat, int row0) {
-        Rows r;
-#pragma unroll
-        for (int i = 0; i < kTiles; i++) {
-            const Q4View &m = p.mat[MODE == kGateUp ? i : mat];
-            const int first = MODE == kGateUp ? row0 : row0 + 16 * i;
-            r.rows[i] = max(0, min(16, m.rows - first));
-            const size_t at = r.rows[i] > 0 ? first : 0;
-            r.w[i] = m.w + (size_t)expert * m.w_stride + at * w_pitch;
-            r.s[i] = m.scales + (size_t)expert * m.s_stride + at * s_pitch;
-            r.b[i] = m.biases + (size_t)expert * m.s_stride + at * s_pitch;
-        }
+        r.row0 = rb * rows_unit;
         return r;
     };
 
-    uint2 wq[kDepth][kTiles][2];
-    uint32_t sc[kDepth][kTiles];  // scales of rows g | g + 8
-    uint16_t bi[kDepth][kTiles];  // bias of row g (even lanes) or g + 8 (odd lanes)
-    auto fetch = [&](const Rows &r, int grp, int slot) {
+    Held<S> h;
+    // where the lane's rows start: offsets of rows g and g + 8 of each tile (rows without a place read the last one there is)
+    const unsigned char *bw[kTiles], *bs[kTiles], *bb[kTiles];
+    uint32_t ow[kTiles][2], os[kTiles][2], ob[kTiles];
+    auto aim = [&](const Unit &un) {
 #pragma unroll
         for (int i = 0; i < kTiles; i++) {
-            const int l0 = min(g, max(r.rows[i] - 1, 0)), l1 = min(g + 8, max(r.rows[i] - 1, 0));  // rows without a place read the last one
-            wq[slot][i][0] = __ldg(reinterpret_cast<const uint2 *>(r.w[i] + l0 * w_pitch + (size_t)grp * 32) + t);
-            wq[slot][i][1] = __ldg(reinterpret_cast<const uint2 *>(r.w[i] + l1 * w_pitch + (size_t)grp * 32) + t);
-            sc[slot][i] = (uint32_t)__ldg(reinterpret_cast<const uint16_t *>(r.s[i] + l0 * s_pitch) + grp) |
-                          ((uint32_t)__ldg(reinterpret_cast<const uint16_t *>(r.s[i] + l1 * s_pitch) + grp) << 16);
-            bi[slot][i] = __ldg(reinterpret_cast<const uint16_t *>(r.b[i] + (t & 1 ? l1 : l0) * s_pitch) + grp);
+            const Q4View &m = p.mat[MODE == kGateUp ? i : un.mat];
+            const int want = un.row0 + (MODE == kGateUp ? 16 * wr : 32 * wr + 16 * i), first = min(want, m.rows - 1), last = m.rows - 1 - first;
+            bw[i] = m.w + (size_t)un.expert * m.w_stride + (size_t)first * w_pitch;
+            bs[i] = m.scales + (size_t)un.expert * m.s_stride + (size_t)first * s_pitch;
+            bb[i] = m.biases + (size_t)un.expert * m.s_stride + (size_t)first * s_pitch;
+            const uint32_t l0 = min(g, last), l1 = min(g + 8, last);
+            ow[i][0] = l0 * w_pitch + t * 8; ow[i][1] = l1 * w_pitch + t * 8;
+            os[i][0] = l0 * s_pitch; os[i][1] = l1 * s_pitch;
+            ob[i] = t & 1 ? os[i][1] : os[i][0];
+        }
+    };
+    auto fetch_words = [&](int step, int j) {  // group j of the step (of S groups)
+#pragma unroll
+        for (int i = 0; i < kTiles; i++)
+#pragma unroll
+            for (int q = 0; q < 2; q++) h.w[i][q][j] = __ldg(reinterpret_cast<const uint2 *>(bw[i] + (ow[i][q] + (uint32_t)(step * S + j) * 32u)));
+    };
+    auto fetch_scales = [&](int step) {
+#pragma unroll
+        for (int i = 0; i < kTiles; i++) {
+            load_bf16s<S>(h.sc[i][0], bs[i] + (os[i][0] + (uint32_t)step * (S * 2)));
+            load_bf16s<S>(h.sc[i][1], bs[i] + (os[i][1] + (uint32_t)step * (S * 2)));
+            load_bf16s<S>(h.bi[i], bb[i] + (ob[i] + (uint32_t)step * (S * 2)));
         }
     };
 
     int held_start = -1, held_job = -1;  // whose activations shared memory holds
     int half = 0;                        // of s_red: units alternate
-    for (long long u = u0; u < u1; u++) {
-        const int job = (int)(u / units_per_job), rb = (int)(u - (long long)job * units_per_job);
-        int expert, start, cnt, mat, row0;
-        job_of(job, expert, start, cnt);
-        if (cnt == 0) continue;  // an expert of another rank, or a slot without one
-        where(rb, mat, row0);
-        const Rows r = rows_of(expert, mat, row0);
-        const int ntl = (cnt + 1) / 2;
-        float acc[kTiles][2][NTL] = {}, accb[kTiles][NTL] = {};
-        for (int c = 0; c < nchunks; c++) {
-            const int cg0 = c * chunk_groups, cgn = min(chunk_groups, G - cg0);
-            const int ga = cg0 + cgn * warp / kWarps, gb = cg0 + cgn * (warp + 1) / kWarps;  // this warp's groups
+    auto next_unit = [&](long long &u, Unit &un) {  // the next one that has tokens
+        while (++u < u1) {
+            un = unit_at(u);
+            if (un.cnt > 0) return;
+        }
+    };
+    long long u = u0 - 1;
+    Unit un = {};
+    next_unit(u, un);
+    if (u < u1) {
+        aim(un);
+        if (wk < min(chunk_groups, G) / S) {
 #pragma unroll
-            for (int s = 0; s < kDepth; s++)
-                if (ga + s < gb) fetch(r, ga + s, s);
+            for (int j = 0; j < S; j++) fetch_words(wk, j);
+            fetch_scales(wk);
+        }
+    }
+    const unsigned char *lane_b = s_b + (size_t)(g >> 2) * chunk_groups * kTokBytes + ((g & 3) * 4 + t) * 16;
+    while (u < u1) {
+        const int ntl = (un.cnt + 1) / 2;
+        float acc[kTiles][2][NTL] = {}, accb[kTiles][NTL] = {};
+        Unit nx = un;
+        long long v = u;
+        for (int c = 0; c < nchunks; c++) {
+            const int cg0 = c * chunk_groups, cgn = min(chunk_groups, G - cg0), step0 = cg0 / S, steps = cgn / S;
             // activations of the job: of one token the source is the token, so consecutive single-token jobs share them
-            int source = start;
-            if (MODE == kGateUp && cnt == 1) source = pair_at(start, 0) / p.top_k;
-            const int kind = MODE == kGateUp && cnt == 1 ? -2 : job;
+            int source = un.start;
+            if (MODE == kGateUp && un.cnt == 1) source = pair_at(un.start, 0) / p.top_k;
+            const int kind = MODE == kGateUp && un.cnt == 1 ? -2 : un.job;
             if (nchunks > 1 || kind != held_job || source != held_start) {
                 __syncthreads();  // everyone is done with the previous activations
-                const int words = cgn * 8, total = cnt * words;
+                const int words = cgn * 8, total = un.cnt * words;
                 for (int i0 = 0; i0 < total; i0 += kThreads) {
                     const int i = i0 + tid;
                     const bool valid = i < total;
                     const int tok = valid ? i / words : 0, w8 = valid ? i - tok * words : 0;
-                    int row = pair_at(start, tok);
+                    int row = pair_at(un.start, tok);
                     if (MODE == kGateUp) row /= p.top_k;
                     unsigned char *tb = s_b + ((size_t)tok * chunk_groups + (w8 >> 3)) * kTokBytes;
                     float2 *f = s_f + ((size_t)(tok >> 1) * chunk_groups + (w8 >> 3)) * 4 + (tok & 1) * 2;
@@ -207,46 +236,72 @@ q4_stream_kernel(Q4Params p, int chunk_groups, int units_per_job, int fixed_jobs
                 held_start = source; held_job = kind;
                 __syncthreads();
             }
-            for (int grp0 = ga; grp0 < gb; grp0 += kDepth) {
+            for (int st = wk; st < steps; st += WK) {
+                // what comes into the registers as this step leaves them: the warp's next step, of this chunk, of the next one, or of
+                // the next unit
+                int more = st + WK < steps ? step0 + st + WK : -1;
+                if (more < 0) {
+                    if (c + 1 < nchunks) {
+                        if (wk < (min(chunk_groups, G - cg0 - chunk_groups)) / S) more = step0 + steps + wk;
+                    } else {
+                        next_unit(v, nx);
+                        if (v < u1) {
+                            aim(nx);
+                            if (wk < min(chunk_groups, G) / S) more = wk;
+                        }
+                    }
+                }
+                uint32_t sc[kTiles][2][(S + 1) / 2], bi[kTiles][(S + 1) / 2];
 #pragma unroll
-                for (int s = 0; s < kDepth; s++) {
-                    const int grp = grp0 + s;
-                    if (grp >= gb) break;
+                for (int i = 0; i < kTiles; i++)
+#pragma unroll
+                    for (int q = 0; q < (S + 1) / 2; q++) { sc[i][0][q] = h.sc[i][0][q]; sc[i][1][q] = h.sc[i][1][q]; bi[i][q] = h.bi[i][q]; }
+                if (more >= 0) fetch_scales(more);
+                const unsigned char *fb = lane_b + (size_t)st * S * kTokBytes;
+                const float2 *ff = s_f + (size_t)st * S * 4 + t;
+#pragma unroll
+                for (int j = 0; j < S; j++) {
                     uint32_t a[kTiles][2][4];  // nibbles as bytes: [tile][word of the lane's two][fragment register]
-                    float s0[kTiles], s1[kTiles], sb[kTiles];
 #pragma unroll
                     for (int i = 0; i < kTiles; i++) {
-                        const uint2 w0 = wq[s][i][0], w1 = wq[s][i][1];
+                        const uint2 w0 = h.w[i][0][j], w1 = h.w[i][1][j];
                         a[i][0][0] = w0.x & 0x0F0F0F0Fu; a[i][0][1] = w1.x & 0x0F0F0F0Fu;
                         a[i][0][2] = (w0.x >> 4) & 0x0F0F0F0Fu; a[i][0][3] = (w1.x >> 4) & 0x0F0F0F0Fu;
                         a[i][1][0] = w0.y & 0x0F0F0F0Fu; a[i][1][1] = w1.y & 0x0F0F0F0Fu;
                         a[i][1][2] = (w0.y >> 4) & 0x0F0F0F0Fu; a[i][1][3] = (w1.y >> 4) & 0x0F0F0F0Fu;
-                        s0[i] = __uint_as_float(sc[s][i] << 16);
-                        s1[i] = __uint_as_float(sc[s][i] & 0xffff0000u);
-                        sb[i] = __uint_as_float((uint32_t)bi[s][i] << 16);
                     }
-                    if (grp + kDepth < gb) fetch(r, grp + kDepth, s);
+                    if (more >= 0) fetch_words(more, j);
 #pragma unroll
                     for (int nt = 0; nt < NTL; nt++) {
                         if (nt >= ntl) break;
-                        const uint4 bf = *reinterpret_cast<const uint4 *>(s_b + ((size_t)(nt * 2 + (g >> 2)) * chunk_groups + (grp - cg0)) * kTokBytes +
-                                                                          ((g & 3) * 4 + t) * 16);
-                        const float2 f = s_f[((size_t)nt * chunk_groups + (grp - cg0)) * 4 + t];
+                        const uint4 bf = *reinterpret_cast<const uint4 *>(fb + (size_t)nt * 2 * chunk_groups * kTokBytes + j * kTokBytes);
+                        const float2 f = ff[(size_t)nt * chunk_groups * 4 + j * 4];
 #pragma unroll
                         for (int i = 0; i < kTiles; i++) {
                             int d[4] = {0, 0, 0, 0};
                             mma_u8s8(d, a[i][0][0], a[i][0][1], a[i][0][2], a[i][0][3], bf.x, bf.y);
                             mma_u8s8(d, a[i][1][0], a[i][1][1], a[i][1][2], a[i][1][3], bf.z, bf.w);
                             // |d| <= 64 * 15 * 128, so two digits still fit an int; lane t holds the digit pair t & 1 of token t / 2
-                            acc[i][0][nt] = fmaf(s0[i] * f.x, (float)(d[0] * 256 + d[1]), acc[i][0][nt]);
-                            acc[i][1][nt] = fmaf(s1[i] * f.x, (float)(d[2] * 256 + d[3]), acc[i][1][nt]);
-                            accb[i][nt] = fmaf(sb[i], f.y, accb[i][nt]);
+                            acc[i][0][nt] = fmaf(bf16_at(sc[i][0][j / 2], j) * f.x, (float)(d[0] * 256 + d[1]), acc[i][0][nt]);
+                            acc[i][1][nt] = fmaf(bf16_at(sc[i][1][j / 2], j) * f.x, (float)(d[2] * 256 + d[3]), acc[i][1][nt]);
+                            accb[i][nt] = fmaf(bf16_at(bi[i][j / 2], j), f.y, accb[i][nt]);
                         }
                     }
                 }
             }
         }
-        // ---- the digit pairs of a row meet, then the eight warps ----
+        if (v == u) {  // a warp without a step in the last chunk has not looked ahead yet
+            next_unit(v, nx);
+            if (v < u1) {
+                aim(nx);
+                if (wk < min(chunk_groups, G) / S) {
+#pragma unroll
+                    for (int j = 0; j < S; j++) fetch_words(wk, j);
+                    fetch_scales(wk);
+                }
+            }
+        }
+        // ---- the digit pairs of a row meet, then the warps along the row ----
         float *red = s_red + (size_t)half * kWarps * kTok * 32;
         half ^= 1;
 #pragma unroll
@@ -259,19 +314,20 @@ q4_stream_kernel(Q4Params p, int chunk_groups, int units_per_job, int fixed_jobs
                 red[((size_t)warp * kTok + nt * 2 + (t >> 1)) * 32 + i * 16 + g + (t & 1) * 8] = t & 1 ? v1 : v0;
             }
         __syncthreads();  // (the other half of s_red is free again once everyone is here)
-        for (int e = tid; e < cnt * 32; e += kThreads) {
-            const int tok = e >> 5, row = e & 31;
-            float v = 0.f;
-#pragma unroll
-            for (int w = 0; w < kWarps; w++) v += red[((size_t)w * kTok + tok) * 32 + row];
-            const size_t pr = (size_t)pair_at(start, tok);
+        for (int e = warp; e < un.cnt * (kWarps >> wk_log2); e += kWarps) {  // 32 rows of one token per warp
+            const int wq = e / un.cnt, tok = e - wq * un.cnt;
+            float y = 0.f;
+            for (int w = 0; w < WK; w++) y += red[((size_t)(wq * WK + w) * kTok + tok) * 32 + lane];
+            const size_t pr = (size_t)pair_at(un.start, tok);
+            const int row = un.row0 + (MODE == kGateUp ? wq * 16 : wq * 32) + lane;
             if constexpr (MODE == kGateUp) {
-                const float up = __shfl_down_sync(0xffffffffu, v, 16);
-                if (row < 16 && row0 + row < p.mat[0].rows) p.out[0][pr * p.mat[0].rows + row0 + row] = v / (1.f + expf(-v)) * up;
+                const float up = __shfl_down_sync(0xffffffffu, y, 16);
+                if (lane < 16 && row < p.mat[0].rows) p.out[0][pr * p.mat[0].rows + row] = y / (1.f + expf(-y)) * up;
             } else {
-                if (row0 + row < p.mat[mat].rows) p.out[mat][pr * p.mat[mat].rows + row0 + row] = v;
+                if (row < p.mat[un.mat].rows) p.out[un.mat][pr * p.mat[un.mat].rows + row] = y;
             }
         }
+        un = nx; u = v;
     }
 }
 
@@ -281,24 +337,35 @@ size_t smem_bytes(int ntl, int chunk) {
     return (size_t)2 * ntl * chunk * kTokBytes + (size_t)ntl * chunk * kFactorBytes + (size_t)2 * kWarps * 2 * ntl * 32 * 4;
 }
 
-template <Q4Mode MODE, int NTL>
+template <Q4Mode MODE, int NTL, int S>
 int launch_one(const Q4Params &p, int jobs, int sm_count, cudaStream_t st) {
     const int G = p.in_dim / 64;
     int chunk = G;
-    while (smem_bytes(NTL, chunk) > kMaxSmem) chunk = (chunk + 1) / 2;
+    while (smem_bytes(NTL, chunk) > kMaxSmem) chunk = ((chunk + 1) / 2 + 3) / 4 * 4;
     const size_t smem = smem_bytes(NTL, chunk);
     static unsigned long long configured = 0;
     if (first_use_on_device(&configured) &&
-        cudaFuncSetAttribute(q4_stream_kernel<MODE, NTL>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem) != cudaSuccess)
+        cudaFuncSetAttribute(q4_stream_kernel<MODE, NTL, S>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem) != cudaSuccess)
         return -1;
+    // as many warps along a row as it has steps; the others take more rows
+    int wk_log2 = 3;
+    while (wk_log2 > 0 && (1 << wk_log2) > chunk / S) wk_log2--;
+    const int rows_unit = (MODE == kGateUp ? 16 : 32) * (kWarps >> wk_log2);
     int per_job = 0;
-    if (MODE == kGateUp) per_job = (p.mat[0].rows + 15) / 16;
-    else
-        for (int i = 0; i < p.nmat; i++) per_job += (p.mat[i].rows + 31) / 32;
+    for (int i = 0; i < (MODE == kGateUp ? 1 : p.nmat); i++) per_job += (p.mat[i].rows + rows_unit - 1) / rows_unit;
     const int per_sm = std::max(1, std::min(NTL == 4 ? 1 : 2, (int)((220 * 1024) / (smem + 1024))));
     const long long units = (long long)jobs * per_job;
     const int grid = (int)std::min<long long>(units, (long long)sm_count * per_sm);
-    return launch_dependent(q4_stream_kernel<MODE, NTL>, dim3(grid), dim3(kThreads), smem, st, p, chunk, per_job, jobs) == cudaSuccess ? 1 : -1;
+    return launch_dependent(q4_stream_kernel<MODE, NTL, S>, dim3(grid), dim3(kThreads), smem, st, p, chunk, per_job, jobs, wk_log2) == cudaSuccess ? 1 : -1;
+}
+
+// Four groups per step where a row has a multiple of four and its scales can be read four at a time; else one by one.
+template <Q4Mode MODE, int NTL>
+int launch_steps(const Q4Params &p, int jobs, int sm_count, cudaStream_t st) {
+    bool four = p.in_dim % 256 == 0;
+    for (int i = 0; i < p.nmat; i++)
+        four = four && (((uintptr_t)p.mat[i].scales | (uintptr_t)p.mat[i].biases | (uintptr_t)p.mat[i].s_stride) & 7) == 0;
+    return four ? launch_one<MODE, NTL, 4>(p, jobs, sm_count, st) : launch_one<MODE, NTL, 1>(p, jobs, sm_count, st);
 }
 
 }  // namespace
@@ -306,13 +373,13 @@ int launch_one(const Q4Params &p, int jobs, int sm_count, cudaStream_t st) {
 int launch_q4_stream(Q4Mode mode, const Q4Params &p, int sm_count, cudaStream_t st) {
     if (mode == kProj) {
         // tokens per pass over the weights: as many as there are, up to 8; more take more passes, which find the weights in L2
-        if (p.n <= 2) return launch_one<kProj, 1>(p, 1, sm_count, st);
-        if (p.n <= 4) return launch_one<kProj, 2>(p, 1, sm_count, st);
-        return launch_one<kProj, 4>(p, (p.n + 7) / 8, sm_count, st);
+        if (p.n <= 2) return launch_steps<kProj, 1>(p, 1, sm_count, st);
+        if (p.n <= 4) return launch_steps<kProj, 2>(p, 1, sm_count, st);
+        return launch_steps<kProj, 4>(p, (p.n + 7) / 8, sm_count, st);
     }
     const int pairs = p.n * p.top_k;  // an upper bound of the jobs; with a plan the device knows how many there are
-    if (p.plan.njobs == nullptr) return mode == kGateUp ? launch_one<kGateUp, 1>(p, pairs, sm_count, st) : launch_one<kDown, 1>(p, pairs, sm_count, st);
-    return mode == kGateUp ? launch_one<kGateUp, 2>(p, pairs, sm_count, st) : launch_one<kDown, 2>(p, pairs, sm_count, st);
+    if (p.plan.njobs == nullptr) return mode == kGateUp ? launch_steps<kGateUp, 1>(p, pairs, sm_count, st) : launch_steps<kDown, 1>(p, pairs, sm_count, st);
+    return mode == kGateUp ? launch_steps<kGateUp, 2>(p, pairs, sm_count, st) : launch_steps<kDown, 2>(p, pairs, sm_count, st);
 }
 
 }  // namespace fm
