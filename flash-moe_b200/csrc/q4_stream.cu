@@ -137,14 +137,11 @@ q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units
         int job, expert, start, cnt, mat, row0;
     };
     auto pair_at = [&](int start, int i) { return MODE == kProj ? start + i : p.plan.njobs != nullptr ? p.plan.pair_of[start + i] : start; };
-    auto unit_at = [&](long long u) {
-        Unit r;
-        r.job = (int)(u / units_per_job);
-        int rb = (int)(u - (long long)r.job * units_per_job);
-        r.mat = 0;
+    auto enter_job = [&](Unit &r) {
         if constexpr (MODE == kProj) {
             r.expert = 0; r.start = r.job * kTok; r.cnt = min(kTok, p.n - r.start);
-            while (rb >= (p.mat[r.mat].rows + rows_unit - 1) / rows_unit) rb -= (p.mat[r.mat++].rows + rows_unit - 1) / rows_unit;
+        } else if (r.job >= njobs) {
+            r.cnt = 0;
         } else if (p.plan.njobs != nullptr) {
             const int4 j = p.plan.jobs[r.job];
             r.expert = uniform(j.x); r.start = uniform(j.y); r.cnt = uniform(j.z);
@@ -152,8 +149,6 @@ q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units
             r.expert = uniform(local_expert(p.ids[r.job], p.first_expert, p.num_experts) + 1) - 1;
             r.start = r.job; r.cnt = r.expert >= 0 ? 1 : 0;
         }
-        r.row0 = rb * rows_unit;
-        return r;
     };
 
     Held<S> h;
@@ -174,11 +169,18 @@ q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units
             ob[i] = t & 1 ? os[i][1] : os[i][0];
         }
     };
-    auto fetch_words = [&](int step, int j) {  // group j of the step (of S groups)
+    const unsigned char *pw[kTiles][2];  // the step being fetched
+    auto point = [&](int step) {
 #pragma unroll
         for (int i = 0; i < kTiles; i++)
 #pragma unroll
-            for (int q = 0; q < 2; q++) h.w[i][q][j] = __ldg(reinterpret_cast<const uint2 *>(bw[i] + (ow[i][q] + (uint32_t)(step * S + j) * 32u)));
+            for (int q = 0; q < 2; q++) pw[i][q] = bw[i] + (ow[i][q] + (uint32_t)step * (S * 32u));
+    };
+    auto fetch_words = [&](int j) {  // group j of the step (of S groups)
+#pragma unroll
+        for (int i = 0; i < kTiles; i++)
+#pragma unroll
+            for (int q = 0; q < 2; q++) h.w[i][q][j] = __ldg(reinterpret_cast<const uint2 *>(pw[i][q] + j * 32));
     };
     auto fetch_scales = [&](int step) {
 #pragma unroll
@@ -192,21 +194,41 @@ q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units
     int held_start = -1, held_job = -1;  // whose activations shared memory holds
     int half = 0;                        // of s_red: units alternate
     auto next_unit = [&](long long &u, Unit &un) {  // the next one that has tokens
-        while (++u < u1) {
-            un = unit_at(u);
-            if (un.cnt > 0) return;
-        }
+        do {
+            if (++u >= u1) return;
+            un.row0 += rows_unit;
+            if (un.row0 >= p.mat[un.mat].rows) {
+                un.row0 = 0;
+                if (MODE == kProj && un.mat + 1 < p.nmat) {
+                    un.mat++;
+                } else {
+                    un.mat = 0; un.job++;
+                    enter_job(un);
+                }
+            }
+        } while (un.cnt == 0);
     };
-    long long u = u0 - 1;
+    long long u = u0;
     Unit un = {};
-    next_unit(u, un);
+    un.job = (int)(u0 / units_per_job);
+    {
+        int rb = (int)(u0 - (long long)un.job * units_per_job);
+        if constexpr (MODE == kProj)
+            while (rb >= (p.mat[un.mat].rows + rows_unit - 1) / rows_unit) rb -= (p.mat[un.mat++].rows + rows_unit - 1) / rows_unit;
+        un.row0 = rb * rows_unit;
+        enter_job(un);
+        if (u < u1 && un.cnt == 0) next_unit(u, un);
+    }
+    auto fetch_first = [&]() {
+        point(wk);
+#pragma unroll
+        for (int j = 0; j < S; j++) fetch_words(j);
+        fetch_scales(wk);
+    };
+    const bool has_first = wk < min(chunk_groups, G) / S;  // this warp has a step in a unit's first chunk
     if (u < u1) {
         aim(un);
-        if (wk < min(chunk_groups, G) / S) {
-#pragma unroll
-            for (int j = 0; j < S; j++) fetch_words(wk, j);
-            fetch_scales(wk);
-        }
+        if (has_first) fetch_first();
     }
     const unsigned char *lane_b = s_b + (size_t)(g >> 2) * chunk_groups * kTokBytes + ((g & 3) * 4 + t) * 16;
     while (u < u1) {
@@ -223,11 +245,11 @@ q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units
             if (nchunks > 1 || kind != held_job || source != held_start) {
                 __syncthreads();  // everyone is done with the previous activations
                 const int words = cgn * 8, total = un.cnt * words;
-                for (int i0 = 0; i0 < total; i0 += kThreads) {
-                    const int i = i0 + tid;
-                    const bool valid = i < total;
-                    const int tok = valid ? i / words : 0, w8 = valid ? i - tok * words : 0;
-                    int row = pair_at(un.start, tok);
+                int tok = 0, w8 = tid;
+                for (int i0 = 0; i0 < total; i0 += kThreads, w8 += kThreads) {
+                    while (w8 >= words && tok < un.cnt) { w8 -= words; tok++; }
+                    const bool valid = tok < un.cnt;
+                    int row = pair_at(un.start, valid ? tok : 0);
                     if (MODE == kGateUp) row /= p.top_k;
                     unsigned char *tb = s_b + ((size_t)tok * chunk_groups + (w8 >> 3)) * kTokBytes;
                     float2 *f = s_f + ((size_t)(tok >> 1) * chunk_groups + (w8 >> 3)) * 4 + (tok & 1) * 2;
@@ -247,7 +269,7 @@ q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units
                         next_unit(v, nx);
                         if (v < u1) {
                             aim(nx);
-                            if (wk < min(chunk_groups, G) / S) more = wk;
+                            if (has_first) more = wk;
                         }
                     }
                 }
@@ -256,7 +278,7 @@ q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units
                 for (int i = 0; i < kTiles; i++)
 #pragma unroll
                     for (int q = 0; q < (S + 1) / 2; q++) { sc[i][0][q] = h.sc[i][0][q]; sc[i][1][q] = h.sc[i][1][q]; bi[i][q] = h.bi[i][q]; }
-                if (more >= 0) fetch_scales(more);
+                if (more >= 0) { fetch_scales(more); point(more); }
                 const unsigned char *fb = lane_b + (size_t)st * S * kTokBytes;
                 const float2 *ff = s_f + (size_t)st * S * 4 + t;
 #pragma unroll
@@ -270,7 +292,7 @@ q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units
                         a[i][1][0] = w0.y & 0x0F0F0F0Fu; a[i][1][1] = w1.y & 0x0F0F0F0Fu;
                         a[i][1][2] = (w0.y >> 4) & 0x0F0F0F0Fu; a[i][1][3] = (w1.y >> 4) & 0x0F0F0F0Fu;
                     }
-                    if (more >= 0) fetch_words(more, j);
+                    if (more >= 0) fetch_words(j);
 #pragma unroll
                     for (int nt = 0; nt < NTL; nt++) {
                         if (nt >= ntl) break;
@@ -294,11 +316,7 @@ q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units
             next_unit(v, nx);
             if (v < u1) {
                 aim(nx);
-                if (wk < min(chunk_groups, G) / S) {
-#pragma unroll
-                    for (int j = 0; j < S; j++) fetch_words(wk, j);
-                    fetch_scales(wk);
-                }
+                if (has_first) fetch_first();
             }
         }
         // ---- the digit pairs of a row meet, then the warps along the row ----
