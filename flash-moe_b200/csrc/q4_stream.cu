@@ -42,6 +42,14 @@ __device__ __forceinline__ void mma_u8s8(int (&d)[4], uint32_t a0, uint32_t a1, 
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// the same with nothing to add to
+__device__ __forceinline__ void mma_u8s8_first(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
+}
+
 // Eight inputs (those of one weight word) of a token -> fixed point bytes in the order of the B fragments.
 // The eight threads of a group of 64 inputs sit in consecutive lanes.
 __device__ __forceinline__ void widen8(const float *x, bool valid, unsigned char *tok_group, float2 *factor, int wi) {
@@ -155,7 +163,19 @@ q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units
     // where the lane's rows start: offsets of rows g and g + 8 of each tile (rows without a place read the last one there is)
     const unsigned char *bw[kTiles], *bs[kTiles], *bb[kTiles];
     uint32_t ow[kTiles][2], os[kTiles][2], ob[kTiles];
+    // where the rows of a unit start; the next unit of the same matrix, all of its rows in place, only moves the starts on
+    bool whole = false;
+    int at_job = -1, at_mat = -1;
     auto aim = [&](const Unit &un) {
+        const bool fits = un.row0 + rows_unit <= p.mat[un.mat].rows;
+        if (whole && fits && un.job == at_job && un.mat == at_mat) {
+#pragma unroll
+            for (int i = 0; i < kTiles; i++) {
+                bw[i] += (size_t)rows_unit * w_pitch; bs[i] += (uint32_t)rows_unit * s_pitch; bb[i] += (uint32_t)rows_unit * s_pitch;
+            }
+            return;
+        }
+        whole = fits; at_job = un.job; at_mat = un.mat;
 #pragma unroll
         for (int i = 0; i < kTiles; i++) {
             const Q4View &m = p.mat[MODE == kGateUp ? i : un.mat];
@@ -300,8 +320,8 @@ q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units
                         const float2 f = ff[(size_t)nt * chunk_groups * 4 + j * 4];
 #pragma unroll
                         for (int i = 0; i < kTiles; i++) {
-                            int d[4] = {0, 0, 0, 0};
-                            mma_u8s8(d, a[i][0][0], a[i][0][1], a[i][0][2], a[i][0][3], bf.x, bf.y);
+                            int d[4];
+                            mma_u8s8_first(d, a[i][0][0], a[i][0][1], a[i][0][2], a[i][0][3], bf.x, bf.y);
                             mma_u8s8(d, a[i][1][0], a[i][1][1], a[i][1][2], a[i][1][3], bf.z, bf.w);
                             // |d| <= 64 * 15 * 128, so two digits still fit an int; lane t holds the digit pair t & 1 of token t / 2
                             acc[i][0][nt] = fmaf(bf16_at(sc[i][0][j / 2], j) * f.x, (float)(d[0] * 256 + d[1]), acc[i][0][nt]);
@@ -365,15 +385,20 @@ int launch_one(const Q4Params &p, int jobs, int sm_count, cudaStream_t st) {
     if (first_use_on_device(&configured) &&
         cudaFuncSetAttribute(q4_stream_kernel<MODE, NTL, S>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem) != cudaSuccess)
         return -1;
-    // as many warps along a row as it has steps; the others take more rows
-    int wk_log2 = 3;
-    while (wk_log2 > 0 && (1 << wk_log2) > chunk / S) wk_log2--;
-    const int rows_unit = (MODE == kGateUp ? 16 : 32) * (kWarps >> wk_log2);
-    int per_job = 0;
-    for (int i = 0; i < (MODE == kGateUp ? 1 : p.nmat); i++) per_job += (p.mat[i].rows + rows_unit - 1) / rows_unit;
-    const int per_sm = std::max(1, std::min(NTL == 4 ? 1 : 2, (int)((220 * 1024) / (smem + 1024))));
-    const long long units = (long long)jobs * per_job;
-    const int grid = (int)std::min<long long>(units, (long long)sm_count * per_sm);
+    const int grid_max = sm_count * std::max(1, std::min(NTL == 4 ? 1 : 2, (int)((220 * 1024) / (smem + 1024))));
+    // Warps along a row (at most as many as it has steps), the others side by side on more rows.  A unit costs its steps and an
+    // end worth about 1 1/3 of a step (the warps meet, the next unit's addresses); a CTA takes whole units: the cheapest split.
+    int wk_log2 = 0, per_job = 0;
+    double best = 0.0;
+    for (int k = 0; k <= 3 && (k == 0 || (1 << k) <= chunk / S); k++) {
+        const int rows = (MODE == kGateUp ? 16 : 32) * (kWarps >> k);
+        int n = 0;
+        for (int i = 0; i < (MODE == kGateUp ? 1 : p.nmat); i++) n += (p.mat[i].rows + rows - 1) / rows;
+        const long long waves = ((long long)jobs * n + grid_max - 1) / grid_max;
+        const double cost = (double)waves * ((double)((G / S + (1 << k) - 1) >> k) * S + 1.33 * 4);
+        if (k == 0 || cost < best) { best = cost; wk_log2 = k; per_job = n; }
+    }
+    const int grid = (int)std::min<long long>((long long)jobs * per_job, grid_max);
     return launch_dependent(q4_stream_kernel<MODE, NTL, S>, dim3(grid), dim3(kThreads), smem, st, p, chunk, per_job, jobs, wk_log2) == cudaSuccess ? 1 : -1;
 }
 
