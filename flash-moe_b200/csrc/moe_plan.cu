@@ -1,6 +1,8 @@
 // Around the experts' products: which pairs (token, slot) go to which expert, and the weighted sum behind them.
 #include <math.h>
 
+#include <algorithm>
+
 #include "fm_device.cuh"
 #include "fm_internal.h"
 
@@ -62,15 +64,18 @@ moe_plan_kernel(const int *__restrict__ ids, int pairs, int first_expert, int nu
     }
 }
 
-// One CTA per token.  The slots are summed in their order, so the result does not depend on the launch.
-__global__ void __launch_bounds__(256)
+// One CTA per token, four columns per thread (more where a row is longer than 4096).  The slots are summed in their order,
+// so the result does not depend on the launch; eight of their loads are in flight at a time.
+constexpr int kCombineThreads = 1024;
+constexpr int kCombineBatch = 8;
+
+__global__ void __launch_bounds__(kCombineThreads)
 moe_combine_kernel(const float *__restrict__ y, const int *__restrict__ ids, const float *__restrict__ weights, int top_k, int first_expert,
                    int num_experts, int hidden, const float *residual, const uint16_t *__restrict__ norm_w, float eps, float *h_out, float *h_norm) {
-    __shared__ float s_w[32];
+    __shared__ float s_w[32], s_sq[32];
     __shared__ int s_slot[32];
     __shared__ int s_n;
-    __shared__ float s_sq[8];
-    const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nwarps = blockDim.x >> 5, step = blockDim.x * 4;
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     if (warp == 0) {  // the slots that have an expert here
@@ -87,17 +92,23 @@ moe_combine_kernel(const float *__restrict__ y, const int *__restrict__ ids, con
     const int ns = s_n;
     const float *yt = y + (size_t)t * top_k * hidden;
     float sq = 0.f;
-    for (int i = tid * 4; i < hidden; i += 1024) {
-        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int s = 0; s < ns; s++) {
-            const float4 v = *reinterpret_cast<const float4 *>(yt + (size_t)s_slot[s] * hidden + i);
-            const float w = s_w[s];
-            a.x = fmaf(w, v.x, a.x); a.y = fmaf(w, v.y, a.y); a.z = fmaf(w, v.z, a.z); a.w = fmaf(w, v.w, a.w);
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = tid * 4; i < hidden; i += step) {
+        const float4 r = residual != nullptr ? *reinterpret_cast<const float4 *>(residual + (size_t)t * hidden + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+        a = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int s0 = 0; s0 < ns; s0 += kCombineBatch) {
+            float4 v[kCombineBatch];
+#pragma unroll
+            for (int s = 0; s < kCombineBatch; s++)
+                if (s0 + s < ns) v[s] = __ldg(reinterpret_cast<const float4 *>(yt + (size_t)s_slot[s0 + s] * hidden + i));
+#pragma unroll
+            for (int s = 0; s < kCombineBatch; s++)
+                if (s0 + s < ns) {
+                    const float w = s_w[s0 + s];
+                    a.x = fmaf(w, v[s].x, a.x); a.y = fmaf(w, v[s].y, a.y); a.z = fmaf(w, v[s].z, a.z); a.w = fmaf(w, v[s].w, a.w);
+                }
         }
-        if (residual != nullptr) {
-            const float4 r = *reinterpret_cast<const float4 *>(residual + (size_t)t * hidden + i);
-            a.x += r.x; a.y += r.y; a.z += r.z; a.w += r.w;
-        }
+        a.x += r.x; a.y += r.y; a.z += r.z; a.w += r.w;
         *reinterpret_cast<float4 *>(h_out + (size_t)t * hidden + i) = a;
         sq += (a.x * a.x + a.y * a.y) + (a.z * a.z + a.w * a.w);
     }
@@ -106,11 +117,10 @@ moe_combine_kernel(const float *__restrict__ y, const int *__restrict__ ids, con
     if (lane == 0) s_sq[warp] = sq;
     __syncthreads();
     float tot = 0.f;
-#pragma unroll
-    for (int w = 0; w < 8; w++) tot += s_sq[w];
+    for (int w = 0; w < nwarps; w++) tot += s_sq[w];
     const float inv = 1.0f / sqrtf(tot / hidden + eps);
-    for (int i = tid * 4; i < hidden; i += 1024) {
-        const float4 h = *reinterpret_cast<const float4 *>(h_out + (size_t)t * hidden + i);
+    for (int i = tid * 4; i < hidden; i += step) {
+        const float4 h = hidden <= step ? a : *reinterpret_cast<const float4 *>(h_out + (size_t)t * hidden + i);  // its own columns
         uint2 wb = make_uint2(0x3f803f80u, 0x3f803f80u);
         if (norm_w != nullptr) wb = __ldg(reinterpret_cast<const uint2 *>(norm_w + i));
         *reinterpret_cast<float4 *>(h_norm + (size_t)t * hidden + i) =
@@ -127,7 +137,7 @@ int launch_moe_plan(const int *ids, int pairs, int first_expert, int num_experts
 
 int launch_moe_combine(const float *y, const int *ids, const float *weights, int n, int top_k, int first_expert, int num_experts, int hidden,
                        const float *residual, const uint16_t *norm_w, float eps, float *h_out, float *h_norm, cudaStream_t st) {
-    return launch_dependent(moe_combine_kernel, dim3(n), dim3(256), 0, st, y, ids, weights, top_k, first_expert, num_experts, hidden, residual, norm_w, eps,
+    return launch_dependent(moe_combine_kernel, dim3(n), dim3(std::min(kCombineThreads, (hidden / 4 + 31) / 32 * 32)), 0, st, y, ids, weights, top_k, first_expert, num_experts, hidden, residual, norm_w, eps,
                             h_out, h_norm) == cudaSuccess ? 1 : -1;
 }
 
