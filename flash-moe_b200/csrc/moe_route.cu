@@ -8,14 +8,15 @@
 //     ids = the top_k largest c, ties to the lowest index;   w = s, divided by the selected ones' sum, times a factor
 //
 // One warp per token, expert j * 32 + lane in register j: the row is read once, coalesced, and nothing leaves the
-// registers.  Selection works on order-preserving 32-bit keys, one redux for the value and one for the lowest index that
-// holds it; a slot's result stays in the lane of its number.  What bounds it is that chain (two redux and a pass over
-// the lane's keys per slot), not the bytes.
+// registers.  Selection works on order-preserving 32-bit keys whose low bits make room for the expert's index, one redux
+// per slot for value and holder together.  What bounds it is that chain (a redux and a pass over the lane's keys per slot),
+// not the bytes.
 //
-// Borders.  Which expert is the k-th best is a whole number, so a rounding must not decide it.  Softmax without a bias
-// is ordered by the logits themselves (exact).  Otherwise the 32-bit choices carry an error of a few units in the last
-// place; where two neighbours in the order, or two groups at the border, are nearer than a bound on that error, the warp
-// takes the row again in 64 bits (rare: about one row in a thousand of random logits).
+// Borders.  Which expert is the k-th best is a whole number, so a rounding must not decide it.  The chain therefore takes
+// every expert that the lost bits, or the error of a 32-bit choice, leave possible -- one or two more than asked for -- and
+// these few, one per lane, are put in their exact order: softmax without a bias by the logits themselves, sigmoid by
+// choices in 64 bits.  Where that does not settle it (softmax with a bias, whose denominator would be needed in 64 bits;
+// two groups at the border; more than 32 candidates) the warp takes the whole row again in 64 bits.
 #include <math.h>
 
 #include "fm_device.cuh"
@@ -129,13 +130,14 @@ __device__ __noinline__ int select_in_double(const RouteParams &p, const float *
 
 template <int VPL>
 __global__ void __launch_bounds__(32 * kRtWarps)
-moe_route_kernel(RouteParams p) {
+moe_route_kernel(const __grid_constant__ RouteParams p) {
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     const int lane = threadIdx.x & 31, t = blockIdx.x * kRtWarps + (threadIdx.x >> 5);
     if (t >= p.n) return;
     const float *row = p.logits + (size_t)t * (p.experts + p.shared);
     const bool softmax = p.score == FM_SCORE_SOFTMAX;
+    const bool by_logit = softmax && p.bias == nullptr;  // order of the logits = order of the scores, without rounding
 
     // logits; -inf where the expert cannot be chosen (its logit or bias is NaN or -inf)
     float x[VPL];
@@ -144,60 +146,54 @@ moe_route_kernel(RouteParams p) {
     for (int j = 0; j < VPL; j++) {
         const int e = j * 32 + lane;
         x[j] = e < p.experts ? __ldg(row + e) : -INFINITY;
+    }
+#pragma unroll
+    for (int j = 0; j < VPL; j++) {
+        const int e = j * 32 + lane;
         if (!(x[j] > -INFINITY)) x[j] = -INFINITY;
         if (p.bias != nullptr && e < p.experts && !(__ldg(p.bias + e) > -INFINITY)) x[j] = -INFINITY;
         m = fmaxf(m, x[j]);
     }
-    m = warp_max(m);
-    // scores' denominator (softmax); +inf logits share the weight equally
-    float sum = 0.f, inv = 0.f;
-    const bool by_logit = softmax && p.bias == nullptr;  // order of the logits = order of the scores, without rounding
-    uint32_t key[VPL];
-    float top_score = 0.f;
-#pragma unroll
-    for (int j = 0; j < VPL; j++) {
-        float s = 0.f;
-        if (x[j] > -INFINITY) s = softmax ? (x[j] == m ? 1.f : expf(x[j] - m)) : 1.f / (1.f + expf(-x[j]));
-        sum += s;
-        key[j] = by_logit ? (x[j] > -INFINITY ? key_of(x[j]) : 0u) : __float_as_uint(s);  // scores for now: the choice follows below
-        top_score = fmaxf(top_score, s);
-    }
+    float inv = 0.f, top_score = 1.f;
+    uint32_t key[VPL];  // order-preserving; 0: not available
     if (softmax) {
-        sum = warp_sum(sum);
-        inv = sum > 0.f ? 1.f / sum : 0.f;
+        // the denominator; +inf logits share the weight equally
+        m = warp_max(m);
+        float sum = 0.f;
+        const bool scores = !by_logit || p.groups > 1 || !p.renormalize;  // (renormalised weights need no denominator)
+        if (scores) {
+#pragma unroll
+            for (int j = 0; j < VPL; j++) sum += x[j] > -INFINITY ? (x[j] == m ? 1.f : expf(x[j] - m)) : 0.f;
+            sum = warp_sum(sum);
+            inv = sum > 0.f ? 1.f / sum : 0.f;
+        }
+        top_score = inv;
     }
-    if (!by_logit) {
-        top_score = warp_max(top_score) * (softmax ? inv : 1.f);
+    // error bound of an approximate choice: the score's (softmax: the exponent's rounding grows with its size; sigmoid: the two
+    // special functions, 2^-22 each) and the sum's
+    const float tol_score = (softmax ? 8e-6f : 1e-6f) * top_score;
+    if (by_logit) {
+#pragma unroll
+        for (int j = 0; j < VPL; j++) key[j] = x[j] > -INFINITY ? key_of(x[j]) : 0u;
+    } else {
 #pragma unroll
         for (int j = 0; j < VPL; j++) {
-            const float s = __uint_as_float(key[j]) * (softmax ? inv : 1.f);
-            key[j] = x[j] > -INFINITY ? key_of(p.bias != nullptr ? s + __ldg(p.bias + j * 32 + lane) : s) : 0u;
+            const float s = softmax ? (x[j] == m ? 1.f : expf(x[j] - m)) * inv : fast_sigmoid(x[j]);
+            key[j] = x[j] > -INFINITY ? key_of(p.bias != nullptr ? s + __ldg(p.bias + min(j * 32 + lane, p.experts - 1)) : s) : 0u;
         }
     }
-    // error bound of a choice: the score's (softmax: the exponent's rounding grows with its size) and the sum's
-    const float tol_score = (softmax ? 8e-6f : 1e-6f) * top_score;
     bool unsure = false;
 
     if (p.groups > 1) {
         const int size = p.experts / p.groups;
-        float mine = -INFINITY;
-        for (int g = 0; g < p.groups; g++) {
-            uint32_t m1 = 0, m2 = 0;
-#pragma unroll
-            for (int j = 0; j < VPL; j++) {
-                if (j * 32 + 31 < g * size || j * 32 >= (g + 1) * size) continue;  // uniform: no expert of the group in register j
-                const int e = j * 32 + lane;
-                const uint32_t k = e >= g * size && e < (g + 1) * size ? key[j] : 0u;
-                m2 = max(m2, min(m1, k));
-                m1 = max(m1, k);
-            }
+        float mine = -INFINITY;  // lane g: the total of group g
+        auto total_of = [&](int g, uint32_t m1, uint32_t m2) {  // each lane's best two of the group
             const uint32_t a = __reduce_max_sync(kFull, m1);
             float total = -INFINITY;
             if (a != 0u) {
-                // by_logit: the group's best scores are those of its best logits
+                // by_logit: the group's best scores are those of its best logits; of one best, compare the logits themselves
                 const float va = value_of(a);
-                total = by_logit ? (va == m ? 1.f : expf(va - m)) * inv : va;
-                if (by_logit && p.group_best == 1) total = va;  // one best: compare the logits themselves
+                total = by_logit && p.group_best == 2 ? (va == m ? 1.f : expf(va - m)) * inv : va;
                 if (p.group_best == 2) {
                     const uint32_t at = __ballot_sync(kFull, m1 == a);
                     const uint32_t b = __popc(at) > 1 ? a : __reduce_max_sync(kFull, m1 == a ? m2 : m1);
@@ -208,6 +204,33 @@ moe_route_kernel(RouteParams p) {
                 }
             }
             if (lane == g) mine = total;
+        };
+        if (size % 32 == 0) {  // whole registers per group
+            const int regs = size / 32;
+            uint32_t m1 = 0, m2 = 0;
+            int left = regs, g = 0;
+#pragma unroll
+            for (int j = 0; j < VPL; j++) {
+                m2 = max(m2, min(m1, key[j]));
+                m1 = max(m1, key[j]);
+                if (--left == 0 && g < p.groups) {
+                    total_of(g++, m1, m2);
+                    m1 = m2 = 0; left = regs;
+                }
+            }
+        } else {
+            for (int g = 0; g < p.groups; g++) {
+                uint32_t m1 = 0, m2 = 0;
+#pragma unroll
+                for (int j = 0; j < VPL; j++) {
+                    if (j * 32 + 31 < g * size || j * 32 >= (g + 1) * size) continue;  // uniform: no expert of the group in register j
+                    const int e = j * 32 + lane;
+                    const uint32_t k = e >= g * size && e < (g + 1) * size ? key[j] : 0u;
+                    m2 = max(m2, min(m1, k));
+                    m1 = max(m1, k);
+                }
+                total_of(g, m1, m2);
+            }
         }
         float gap, border;
         const uint32_t keep = best_groups<float>(mine, p.groups, p.top_groups, lane, &gap, &border);
@@ -220,54 +243,86 @@ moe_route_kernel(RouteParams p) {
         }
     }
 
-    int id = -1;
-    uint32_t prev = 0;
-    const int rounds = p.top_k + (by_logit ? 0 : 1);  // one more than asked for: the border needs its other side
-    for (int s = 0; s < rounds; s++) {
-        uint32_t best = 0;
+    // Candidates: lane s gets the s-th largest key, its low bits replaced by the index (one redux finds value and holder).  The
+    // top_k of them, and as many more as the lost bits and the choice's error leave possible.
+    constexpr uint32_t kIndex = 32 * VPL - 1;
 #pragma unroll
-        for (int j = 0; j < VPL; j++) best = max(best, key[j]);
-        best = __reduce_max_sync(kFull, best);
-        if (best == 0u) break;
-        int at = 0x7fffffff;
+    for (int j = 0; j < VPL; j++)
+        if (key[j] != 0u) key[j] = (key[j] & ~kIndex) | (kIndex - (uint32_t)(j * 32 + lane));
+    uint32_t mine = 0, last = 0;
+    int nc = 0;
+    if (!unsure) {
+        while (true) {
+            uint32_t best = 0;
 #pragma unroll
-        for (int j = VPL - 1; j >= 0; j--)
-            if (key[j] == best) at = j * 32 + lane;
-        at = __reduce_min_sync(kFull, at);
+            for (int j = 0; j < VPL; j++) best = max(best, key[j]);
+            best = __reduce_max_sync(kFull, best);
+            if (best == 0u) break;
+            if (nc >= p.top_k && value_of(best | kIndex) + 2.f * tol_score * (by_logit ? 0.f : 1.f) + (by_logit ? 0.f : 2.4e-7f * fabsf(value_of(best))) < value_of(last & ~kIndex)) break;
+            if (nc == 32) { unsure = true; break; }
+            if (lane == nc) mine = best;
+            nc++;
+            if (nc == p.top_k) last = best;
 #pragma unroll
-        for (int j = 0; j < VPL; j++)
-            if (j * 32 + lane == at) key[j] = 0u;
-        if (s < p.top_k && lane == s) id = at;
-        if (!by_logit) {
-            const float v = value_of(best);
-            if (s > 0 && !(value_of(prev) - v > 2.f * tol_score + 2.4e-7f * fabsf(v))) unsure = true;
-            prev = best;
+            for (int j = 0; j < VPL; j++) key[j] = key[j] == best ? 0u : key[j];
         }
     }
-    if (unsure) id = select_in_double<VPL>(p, row, lane);
+    // Their exact order: logits as they are, choices in 64 bits (softmax with a bias: in 32, where that decides).
+    int id = lane < nc ? (int)(kIndex - (mine & kIndex)) : -1, rank = 0;
+    const float v0 = id >= 0 ? __ldg(row + id) : -INFINITY;
+    if (by_logit) {
+        for (int j = 0; j < nc; j++) {
+            const float o = __shfl_sync(kFull, v0, j);
+            const int oe = __shfl_sync(kFull, id, j);
+            rank += (o > v0 || (o == v0 && oe < id)) ? 1 : 0;
+        }
+    } else if (!softmax) {
+        double c = -INFINITY;
+        if (id >= 0) c = 1.0 / (1.0 + exp(-(double)v0)) + (p.bias != nullptr ? (double)__ldg(p.bias + id) : 0.0);
+        for (int j = 0; j < nc; j++) {
+            const double o = __shfl_sync(kFull, c, j);
+            const int oe = __shfl_sync(kFull, id, j);
+            rank += (o > c || (o == c && oe < id)) ? 1 : 0;
+        }
+    } else {
+        const float c = id >= 0 ? (v0 == m ? 1.f : expf(v0 - m)) * inv + __ldg(p.bias + id) : -INFINITY;
+        bool near = false;
+        for (int j = 0; j < nc; j++) {
+            const float o = __shfl_sync(kFull, c, j);
+            const int oe = __shfl_sync(kFull, id, j);
+            rank += (o > c || (o == c && oe < id)) ? 1 : 0;
+            near |= oe != id && !(fabsf(o - c) > 2.f * tol_score + 2.4e-7f * fabsf(c));
+        }
+        unsure |= __any_sync(kFull, near && id >= 0);
+    }
+    if (unsure) {
+        id = select_in_double<VPL>(p, row, lane);
+        rank = lane;
+    }
+    const bool chosen = id >= 0 && rank < p.top_k;
+    const int found = __popc(__ballot_sync(kFull, chosen)), slots = p.top_k + p.shared;
 
-    const int slots = p.top_k + p.shared;
-    const float v = id >= 0 ? __ldg(row + id) : -INFINITY;
+    const float v = chosen ? __ldg(row + id) : -INFINITY;
     float w = 0.f;
     if (!p.renormalize) {
-        if (id >= 0) w = softmax ? (v == m ? 1.f : expf(v - m)) * inv : 1.f / (1.f + expf(-v));
+        if (chosen) w = softmax ? (v == m ? 1.f : expf(v - m)) * inv : 1.f / (1.f + expf(-v));
     } else {
         // a common factor drops out: the scores relative to the largest selected one, so that small ones do not underflow
         const float vm = warp_max(v);
-        if (id >= 0) {
+        if (chosen) {
             const float rel = v == vm ? 1.f : expf(v - vm);
             w = softmax ? rel : vm > 0.f ? 1.f / (1.f + expf(-v)) : rel / (1.f + expf(v));
         }
         const float tot = warp_sum(w);
         w = tot > 0.f ? w / tot : 0.f;
     }
-    if (lane < p.top_k) {
-        p.ids[(size_t)t * slots + lane] = id;
-        p.weights[(size_t)t * slots + lane] = w * p.scale;
-    }
+    int *ids = p.ids + (size_t)t * slots;
+    float *weights = p.weights + (size_t)t * slots;
+    if (chosen) { ids[rank] = id; weights[rank] = w * p.scale; }
+    if (lane >= found && lane < p.top_k) { ids[lane] = -1; weights[lane] = 0.f; }
     if (p.shared && lane == 0) {
-        p.ids[(size_t)t * slots + p.top_k] = p.experts;
-        p.weights[(size_t)t * slots + p.top_k] = 1.f / (1.f + expf(-__ldg(row + p.experts)));
+        ids[p.top_k] = p.experts;
+        weights[p.top_k] = 1.f / (1.f + expf(-__ldg(row + p.experts)));
     }
 }
 
