@@ -48,6 +48,7 @@ template <typename T>
 __device__ uint32_t best_groups(T total, int groups, int top, int lane, T *gap, T *border) {
     int rank = 0;
     T last = -INFINITY, next = -INFINITY;
+#pragma unroll 4
     for (int g = 0; g < groups; g++) {
         const T o = __shfl_sync(kFull, total, g);
         rank += (o > total || (o == total && g < lane)) ? 1 : 0;
@@ -236,11 +237,10 @@ moe_route_kernel(const __grid_constant__ RouteParams p) {
         const uint32_t keep = best_groups<float>(mine, p.groups, p.top_groups, lane, &gap, &border);
         if (!(by_logit && p.group_best == 1))
             unsure = !(gap > (by_logit ? 1.6e-5f * border : 4.f * tol_score + 4.8e-7f * fabsf(border)));
+        const uint32_t per = ((1u << 20) + size - 1) / size;  // e / size = e * per >> 20 for e < 1024
 #pragma unroll
-        for (int j = 0; j < VPL; j++) {
-            const int e = j * 32 + lane;
-            if (e < p.experts && !((keep >> (e / size)) & 1)) key[j] = 0u;
-        }
+        for (int j = 0; j < VPL; j++)
+            if (!((keep >> ((uint32_t)(j * 32 + lane) * per >> 20)) & 1)) key[j] = 0u;
     }
 
     // Candidates: lane s gets the s-th largest key, its low bits replaced by the index (one redux finds value and holder).  The
