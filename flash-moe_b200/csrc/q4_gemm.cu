@@ -22,7 +22,7 @@
 //                consecutive features per token and store
 //   warp 16      TMA producer of token tiles, hi | lo;  warp 18  of weight tiles [128 rows][128 bytes]
 //   warp 17      issues the MMAs (M128, N = the unit's tokens rounded up to 16, K16)
-// TMEM columns: T * 64 running sums, 2 * 64 of steps in flight, the rest operand A in slots of 32.
+// TMEM columns: T * 64 running sums, 2 * 64 of steps in flight, the rest operand A in slots of 64 (two groups).
 // With two terms the tensor work is twice the product's; what bounds a long prompt is that, a short one the weights' stream.
 // Every wait is bounded; on expiry the CTA records an error code and winds down.
 #include <cuda.h>
@@ -42,13 +42,14 @@ namespace {
 
 constexpr int kTok = kGemmTokens;           // tokens per unit (96)
 constexpr int kChunk = 4;                   // groups per step
-constexpr int kBSlot = 2 * kTok * 128;      // bytes of a token tile: one group, hi then lo
-constexpr int kBSlots = 6;
+constexpr int kBTile = kTok * 128;          // bytes of a token tile: one group, one term
+constexpr int kBSlot = 4 * kBTile;          // two groups, hi then lo each
+constexpr int kBSlots = 3;
 constexpr int kWSlot = 128 * 128;           // bytes of a weight tile: 128 rows, 4 groups
 constexpr int kWSlots = 4;
 constexpr int kGemmThreads = 19 * 32;
 constexpr int kDBufs = 2;
-// Steps whose row factors are kept: the widening warps are at most the operand slots (8, one to a step at the least), the
+// Steps whose row factors are kept: the widening warps are at most the operand slots (one to a step at the least), the
 // steps in flight and their own step ahead of the epilogue.
 constexpr int kFSteps = 16;
 constexpr int kHalf = kTok / 2;            // columns of an epilogue warp
@@ -57,7 +58,7 @@ constexpr uint32_t kColStep = 0, kColSum = kDBufs * kTok;  // TMEM columns; oper
 template <int T>
 struct Layout {
     static constexpr uint32_t colA = kColSum + T * kTok;
-    static constexpr int aslots = (512 - (int)colA) / 32;
+    static constexpr int aslots = (512 - (int)colA) / 64;  // of two groups
 };
 
 enum Bar { BAR_W_FULL = 0, BAR_W_EMPTY = BAR_W_FULL + kWSlots, BAR_B_FULL = BAR_W_EMPTY + kWSlots, BAR_B_EMPTY = BAR_B_FULL + kBSlots,
@@ -247,7 +248,7 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
         for (int i = 0; i < kBSlots; i++) { mbar_init(bar(BAR_B_FULL + i), 1); mbar_init(bar(BAR_B_EMPTY + i), 1); }
         for (int i = 0; i < kDBufs; i++) { mbar_init(bar(BAR_D_FULL + i), 1); mbar_init(bar(BAR_D_EMPTY + i), 8); }
         mbar_init(bar(BAR_END), 1);
-        for (int i = 0; i < 8; i++) { mbar_init(bar(BAR_A_FULL + i), 4); mbar_init(bar(BAR_A_EMPTY + i), 1); }
+        for (int i = 0; i < 8; i++) { mbar_init(bar(BAR_A_FULL + i), 8); mbar_init(bar(BAR_A_EMPTY + i), 1); }
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     if (warp == 17) {
@@ -290,17 +291,22 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
         bool ok = true;
         for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x) {
             const Unit un = unit_at<MODE, T>(g, u);
-            for (int grp = 0; grp < G + g.pseudo && ok; grp++) {  // 64 columns of x at a time
-                ok = __all_sync(0xffffffffu, count < kBSlots || bar_wait(bar(BAR_B_EMPTY + rb.slot), rb.phase ^ 1, abortp));
-                if (!ok) break;
-                const uint32_t full = bar(BAR_B_FULL + rb.slot), dst = sB + (uint32_t)rb.slot * kBSlot;
-                if (lane == 0) mbar_expect_tx(full, (uint32_t)un.ncols * 256u);
-                __syncwarp();
-                if (lane * 16 < un.ncols) {
-                    tma_load_2d(dst + (uint32_t)lane * 2048u, &maps.x, grp * 64, un.start + lane * 16, full);
-                    tma_load_2d(dst + kTok * 128u + (uint32_t)lane * 2048u, &maps.x, g.kp + grp * 64, un.start + lane * 16, full);
+            for (int c = 0; c < nchunks && ok; c++) {
+                const int first = c < nreal ? c * kChunk : G + c - nreal, ng = c < nreal ? min(kChunk, G - first) : 1;  // 64 columns of x each
+                for (int j = 0; j < ng && ok; j += 2) {
+                    ok = __all_sync(0xffffffffu, count < kBSlots || bar_wait(bar(BAR_B_EMPTY + rb.slot), rb.phase ^ 1, abortp));
+                    if (!ok) break;
+                    const uint32_t full = bar(BAR_B_FULL + rb.slot), dst = sB + (uint32_t)rb.slot * kBSlot + (uint32_t)lane * 2048u;
+                    const int n = min(2, ng - j);
+                    if (lane == 0) mbar_expect_tx(full, (uint32_t)(un.ncols * 256 * n));
+                    __syncwarp();
+                    if (lane * 16 < un.ncols)
+                        for (int q = 0; q < n; q++) {
+                            tma_load_2d(dst + (uint32_t)(2 * q) * kBTile, &maps.x, (first + j + q) * 64, un.start + lane * 16, full);
+                            tma_load_2d(dst + (uint32_t)(2 * q + 1) * kBTile, &maps.x, g.kp + (first + j + q) * 64, un.start + lane * 16, full);
+                        }
+                    rb.next(); count = min(count + 1, kBSlots);
                 }
-                rb.next(); count = min(count + 1, kBSlots);
             }
         }
         if (lane == 0 && *abortp) drain(BAR_B_FULL, kBSlots, rb.slot, rb.phase, count);
@@ -349,46 +355,54 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
             const uint32_t idesc = idesc_dense(128, un.ncols, false, 0);
             for (int c = 0; c < nchunks && ok; c++) {
                 const bool real = c < nreal;
-                const int na = real ? min(kChunk, G - c * kChunk) : 2, nb = real ? na : 1;
+                const int na = real ? min(kChunk, G - c * kChunk) : 2, npairs = (na + 1) / 2;
+                const int nk = real ? 4 : (min(64, G - (c - nreal) * 64) + 15) / 16;  // the bias block: one column per group
                 for (int i = 0; i < tiles && ok; i++) {
                     ok = dcount < kDBufs || __all_sync(0xffffffffu, bar_wait(bar(BAR_D_EMPTY + rd.slot), rd.phase ^ 1, abortp));
                     if (!ok) break;
                     const uint32_t d = tm + kColStep + (uint32_t)rd.slot * kTok;
                     Ring<kBSlots> rt = rb;
-                    for (int j = 0; j < na && ok; j++) {
+                    for (int q = 0; q < npairs && ok; q++) {
                         ok = __all_sync(0xffffffffu, bar_wait(bar(BAR_B_FULL + rt.slot), rt.phase, abortp) &&
                                                          bar_wait(bar(BAR_A_FULL + ra.slot), ra.phase, abortp));
                         if (!ok) break;
                         tc_fence_after();
-                        const uint32_t a = tm + L::colA + (uint32_t)ra.slot * 32, b = sB + (uint32_t)rt.slot * kBSlot;
-                        const uint64_t hi = smem_desc(b, 0, 1024), lo = smem_desc(b + kTok * 128, 0, 1024);
-                        const bool done_b = i == tiles - 1 && (real || j == na - 1);
+                        const uint32_t a = tm + L::colA + (uint32_t)ra.slot * 64;
+                        const uint64_t b0 = smem_desc(sB + (uint32_t)rt.slot * kBSlot, 0, 1024);
+                        constexpr uint64_t kTile = kBTile >> 4;  // in the descriptor's units of 16 bytes
+                        const bool two = 2 * q + 1 < na;
                         if (elect_one()) {
-                            // the bias block holds one column per group, and only steps of 16 columns that have some
                             if (real) {
 #pragma unroll
-                                for (int k = 0; k < 4; k++) tc_mma_f16_ta(d, a + k * 8, lo + k * 2, idesc, j > 0 || k > 0);
+                                for (int k = 0; k < 4; k++) tc_mma_f16_ta(d, a + k * 8, b0 + kTile + k * 2, idesc, q > 0 || k > 0);  // lo
 #pragma unroll
-                                for (int k = 0; k < 4; k++) tc_mma_f16_ta(d, a + k * 8, hi + k * 2, idesc, 1);
+                                for (int k = 0; k < 4; k++) tc_mma_f16_ta(d, a + k * 8, b0 + k * 2, idesc, 1);  // hi
+                                if (two) {
+#pragma unroll
+                                    for (int k = 0; k < 4; k++) tc_mma_f16_ta(d, a + 32 + k * 8, b0 + 3 * kTile + k * 2, idesc, 1);
+#pragma unroll
+                                    for (int k = 0; k < 4; k++) tc_mma_f16_ta(d, a + 32 + k * 8, b0 + 2 * kTile + k * 2, idesc, 1);
+                                }
                             } else {
-                                const int nk = (min(64, G - (c - nreal) * 64) + 15) / 16;
                                 for (int k = 0; k < nk; k++) {
-                                    tc_mma_f16_ta(d, a + k * 8, lo + k * 2, idesc, j > 0 || k > 0);
-                                    tc_mma_f16_ta(d, a + k * 8, hi + k * 2, idesc, 1);
+                                    tc_mma_f16_ta(d, a + k * 8, b0 + kTile + k * 2, idesc, k > 0);
+                                    tc_mma_f16_ta(d, a + k * 8, b0 + k * 2, idesc, 1);
+                                    tc_mma_f16_ta(d, a + 32 + k * 8, b0 + kTile + k * 2, idesc, 1);
+                                    tc_mma_f16_ta(d, a + 32 + k * 8, b0 + k * 2, idesc, 1);
                                 }
                             }
                             tc_commit(bar(BAR_A_EMPTY + ra.slot));
-                            if (done_b) tc_commit(bar(BAR_B_EMPTY + rt.slot));
-                            if (j == na - 1) tc_commit(bar(BAR_D_FULL + rd.slot));
+                            if (i == tiles - 1) tc_commit(bar(BAR_B_EMPTY + rt.slot));
+                            if (q == npairs - 1) tc_commit(bar(BAR_D_FULL + rd.slot));
                         }
                         __syncwarp();
                         ra.next();
-                        if (real) rt.next();
+                        rt.next();
                     }
                     if (!ok) break;
                     rd.next(); dcount = min(dcount + 1, kDBufs);
                 }
-                for (int j = 0; j < nb; j++) rb.next();
+                for (int q = 0; q < npairs; q++) rb.next();
             }
         }
         if (!ok && elect_one()) {  // a wait ran out: let what was issued finish before tensor memory is given back
@@ -404,7 +418,7 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
         Ring<kWSlots> rw;
         Ring<kA> ra;
         Ring<kFSteps> rf;
-        int ahead = 0, turn = 0;  // operand slots used so far (up to all); they alternate between the two groups of four warps
+        int ahead = 0;  // operand slots used so far (up to all); the two groups of four warps take a group of 64 inputs each
         bool ok = true;
         // the steps in order; the scales of a step are fetched while the one before it is worked on
         Unit un;
@@ -433,7 +447,7 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
                 e = chunk_exponent(sc);
                 ok = __all_sync(0xffffffffu, bar_wait(bar(BAR_W_FULL + rw.slot), rw.phase, abortp));
             } else {
-                // b + 8 s of the row's groups; slot `turn` is the first term, the other the second
+                // b + 8 s of the row's groups; warps 0-3 take the first term, the others the second
                 float v[64];
                 const int g0 = (c - nreal) * 64, gn = min(64, G - g0);
                 if (g.wide) {  // both tiles came like weight tiles, 64 bf16 to a row
@@ -475,28 +489,31 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
                     const float a0 = v[2 * q] * up, a1 = v[2 * q + 1] * up;
                     const __half2 h = __floats2half2_rn(a0, a1);
                     const float2 hf = __half22float2(h);
-                    pw[q] = h2_bits(turn == wg ? h : __floats2half2_rn(a0 - hf.x, a1 - hf.y));
+                    pw[q] = h2_bits(wg == 0 ? h : __floats2half2_rn(a0 - hf.x, a1 - hf.y));
                 }
             }
             if (!ok) break;
             // for the epilogue: what the step's sums have to be multiplied with (seen through A_FULL, the MMAs and D_FULL)
-            if (turn == wg) s_f[rf.slot * 128 + r] = real ? pow2(127 + e - 141 + 24) : pow2(127 + e - 135);
-            // one group's operand into the next slot of TMEM
-            auto put = [&](const uint32_t (&a)[32]) {
+            if (wg == 0) s_f[rf.slot * 128 + r] = real ? pow2(127 + e - 141 + 24) : pow2(127 + e - 135);
+            // one group's operand into its half of the next slot of TMEM
+            auto put = [&](const uint32_t (&a)[32], bool any) {
                 ok = __all_sync(0xffffffffu, ahead < kA || bar_wait(bar(BAR_A_EMPTY + ra.slot), ra.phase ^ 1, abortp));
                 if (!ok) return;
-                tc_fence_after();
-                tc_st32(tmem + lanes + L::colA + (uint32_t)ra.slot * 32, a);
-                tc_wait_st();
-                tc_fence_before();
+                if (any) {
+                    tc_fence_after();
+                    tc_st32(tmem + lanes + L::colA + (uint32_t)(ra.slot * 64 + wg * 32), a);
+                    tc_wait_st();
+                    tc_fence_before();
+                }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(BAR_A_FULL + ra.slot));
+                ra.next();
+                ahead = min(ahead + 1, kA);
             };
             if (real) {
                 const float up = pow2(127 + 141 - e);  // the largest scale comes to [2^14, 2^15)
                 const uint32_t wrow = sW + (uint32_t)rw.slot * kWSlot + (uint32_t)r * 128u;
-                for (int j = 0; j < na && ok; j++, ra.next(), turn ^= 1, ahead = min(ahead + 1, kA)) {
-                    if (turn != wg) continue;
+                for (int j = wg; j < na + wg && ok; j += 2) {  // (of an odd number the second half of the last slot stays empty)
                     const float mf = __uint_as_float(((j & 2 ? sc.y : sc.x) >> ((j & 1) * 16)) << 16) * up;
                     const uint32_t m = dup_h2(mf), m16 = dup_h2(mf * 0.0625f), mc = dup_h2(mf * -0x1p-21f);
                     uint32_t a[32];
@@ -508,11 +525,10 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
                         widen_word(w4.z, m, m16, mc, a + h * 16 + 8);
                         widen_word(w4.w, m, m16, mc, a + h * 16 + 12);
                     }
-                    put(a);
+                    put(a, j < na);
                 }
             } else {
-                for (int j = 0; j < 2 && ok; j++, ra.next(), turn ^= 1, ahead = min(ahead + 1, kA))
-                    if (turn == wg) put(pw);
+                put(pw, true);
             }
             const int used = real ? 1 : g.wide ? 2 : 0;  // weight slots of the step
             for (int k = 0; k < used; k++) {
