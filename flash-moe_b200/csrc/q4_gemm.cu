@@ -21,7 +21,7 @@
 //   warps 8-15   epilogue: running sums in TMEM, added up per step; the last step of a tile writes the results, 128
 //                consecutive features per token and store
 //   warp 16      TMA producer of token tiles, hi | lo;  warp 18  of weight tiles [128 rows][128 bytes]
-//   warp 17      issues the MMAs (M128, N = the unit's tokens rounded up to 16, K16)
+//   warps 17, 19 issue the MMAs of a tile each (M128, N = the unit's tokens rounded up to 16, K16)
 // TMEM columns: T * 64 running sums, 2 * 64 of steps in flight, the rest operand A in slots of 64 (two groups).
 // With two terms the tensor work is twice the product's; what bounds a long prompt is that, a short one the weights' stream.
 // Every wait is bounded; on expiry the CTA records an error code and winds down.
@@ -47,8 +47,8 @@ constexpr int kBSlot = 4 * kBTile;          // two groups, hi then lo each
 constexpr int kBSlots = 3;
 constexpr int kWSlot = 128 * 128;           // bytes of a weight tile: 128 rows, 4 groups
 constexpr int kWSlots = 4;
-constexpr int kGemmThreads = 19 * 32;
-constexpr int kDBufs = 2;
+constexpr int kGemmThreads = 20 * 32;
+constexpr int kDBufs = 2;                   // one per tile of a unit
 // Steps whose row factors are kept: the widening warps are at most the operand slots (one to a step at the least), the
 // steps in flight and their own step ahead of the epilogue.
 constexpr int kFSteps = 16;
@@ -57,13 +57,14 @@ constexpr uint32_t kColStep = 0, kColSum = kDBufs * kTok;  // TMEM columns; oper
 
 template <int T>
 struct Layout {
+    static_assert(T == kDBufs, "a step buffer and an issuing warp per tile");
     static constexpr uint32_t colA = kColSum + T * kTok;
     static constexpr int aslots = (512 - (int)colA) / 64;  // of two groups
 };
 
 enum Bar { BAR_W_FULL = 0, BAR_W_EMPTY = BAR_W_FULL + kWSlots, BAR_B_FULL = BAR_W_EMPTY + kWSlots, BAR_B_EMPTY = BAR_B_FULL + kBSlots,
            BAR_D_FULL = BAR_B_EMPTY + kBSlots, BAR_D_EMPTY = BAR_D_FULL + kDBufs, BAR_A_FULL = BAR_D_EMPTY + kDBufs,
-           BAR_A_EMPTY = BAR_A_FULL + 8, BAR_END = BAR_A_EMPTY + 8, BAR_COUNT };
+           BAR_A_EMPTY = BAR_A_FULL + 8, BAR_END = BAR_A_EMPTY + 8, BAR_COUNT = BAR_END + 2 };
 constexpr int kGemmSmem = kBSlots * kBSlot + kWSlots * kWSlot + kFSteps * 128 * 4 + BAR_COUNT * 8 + 1024;
 
 struct GemmMaps {
@@ -245,9 +246,9 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
     if (tid == 0) {
         s_abort = 0;
         for (int i = 0; i < kWSlots; i++) { mbar_init(bar(BAR_W_FULL + i), 1); mbar_init(bar(BAR_W_EMPTY + i), 8); }
-        for (int i = 0; i < kBSlots; i++) { mbar_init(bar(BAR_B_FULL + i), 1); mbar_init(bar(BAR_B_EMPTY + i), 1); }
+        for (int i = 0; i < kBSlots; i++) { mbar_init(bar(BAR_B_FULL + i), 1); mbar_init(bar(BAR_B_EMPTY + i), 2); }
         for (int i = 0; i < kDBufs; i++) { mbar_init(bar(BAR_D_FULL + i), 1); mbar_init(bar(BAR_D_EMPTY + i), 8); }
-        mbar_init(bar(BAR_END), 1);
+        mbar_init(bar(BAR_END), 1); mbar_init(bar(BAR_END + 1), 1);
         for (int i = 0; i < 8; i++) { mbar_init(bar(BAR_A_FULL + i), 8); mbar_init(bar(BAR_A_EMPTY + i), 1); }
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
@@ -338,38 +339,39 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
             if (*abortp) drain(BAR_W_FULL, kWSlots, rw.slot, rw.phase, count);
         }
         __syncwarp();
-    } else if (warp == 17) {
-        // ================= MMA issuer =================
-        // The whole warp walks the steps and one elected lane issues a slot's MMAs in one go: everything they read is then
-        // uniform across the warp (the reductions below say so to the compiler), and an MMA costs what the tensor core takes,
-        // 41 cycles at N = 64.  Issued by `lane == 0` in divergent code each took 120 to 190.
-        const uint32_t tm = uniform(tmem);
+    } else if (warp == 17 || warp == 19) {
+        // ================= MMA issuers =================
+        // A warp per tile: while one waits and counts, the other's MMAs keep the tensor core busy (its queue holds two or three).
+        // A whole warp walks the steps and one elected lane issues a slot's MMAs in one go: everything they read is then uniform
+        // across the warp (the reductions say so to the compiler), and an MMA costs what the tensor core takes, 57 cycles at
+        // N = 96.  Issued by `lane == 0` in divergent code each took 120 to 190.
+        const int tile = warp == 17 ? 0 : 1;
+        const uint32_t d = uniform(tmem) + kColStep + (uint32_t)(tile * kTok), a0 = uniform(tmem) + L::colA;
+        const uint64_t desc0 = smem_desc(sB, 0, 1024);
+        constexpr uint64_t kTile = kBTile >> 4;  // in the descriptor's units of 16 bytes
         Ring<kBSlots> rb;
-        Ring<kA> ra;
-        Ring<kDBufs> rd;
-        int dcount = 0;
+        // operand slots filled before this chunk (both tiles), of this tile (a pair of barriers of its own announces them, so that a
+        // warp never waits on a phase it is two behind), steps of this tile
+        uint32_t pairs = 0, mine = 0, steps = 0;
         bool ok = true;
         for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x) {
             const Unit un = unit_at<MODE, T>(g, u);
-            const int tiles = un.tiles;
             const uint32_t idesc = idesc_dense(128, un.ncols, false, 0);
             for (int c = 0; c < nchunks && ok; c++) {
                 const bool real = c < nreal;
                 const int na = real ? min(kChunk, G - c * kChunk) : 2, npairs = (na + 1) / 2;
                 const int nk = real ? 4 : (min(64, G - (c - nreal) * 64) + 15) / 16;  // the bias block: one column per group
-                for (int i = 0; i < tiles && ok; i++) {
-                    ok = dcount < kDBufs || __all_sync(0xffffffffu, bar_wait(bar(BAR_D_EMPTY + rd.slot), rd.phase ^ 1, abortp));
-                    if (!ok) break;
-                    const uint32_t d = tm + kColStep + (uint32_t)rd.slot * kTok;
-                    Ring<kBSlots> rt = rb;
-                    for (int q = 0; q < npairs && ok; q++) {
-                        ok = __all_sync(0xffffffffu, bar_wait(bar(BAR_B_FULL + rt.slot), rt.phase, abortp) &&
-                                                         bar_wait(bar(BAR_A_FULL + ra.slot), ra.phase, abortp));
+                if (tile < un.tiles) {
+                    uint32_t n = pairs + (uint32_t)(tile * npairs);
+                    ok = steps == 0 || __all_sync(0xffffffffu, bar_wait(bar(BAR_D_EMPTY + tile), (steps - 1) & 1, abortp));
+                    for (int q = 0; q < npairs && ok; q++, n++, mine++) {
+                        const uint32_t slot = n % kA;
+                        ok = __all_sync(0xffffffffu, bar_wait(bar(BAR_B_FULL + rb.slot), rb.phase, abortp) &&
+                                                         bar_wait(bar(BAR_A_FULL + 2 * tile + (int)(mine & 1)), mine >> 1 & 1, abortp));
                         if (!ok) break;
                         tc_fence_after();
-                        const uint32_t a = tm + L::colA + (uint32_t)ra.slot * 64;
-                        const uint64_t b0 = smem_desc(sB + (uint32_t)rt.slot * kBSlot, 0, 1024);
-                        constexpr uint64_t kTile = kBTile >> 4;  // in the descriptor's units of 16 bytes
+                        const uint32_t a = a0 + slot * 64;
+                        const uint64_t b0 = desc0 + (uint64_t)(rb.slot * (kBSlot >> 4));
                         const bool two = 2 * q + 1 < na;
                         if (elect_one()) {
                             if (real) {
@@ -391,159 +393,185 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
                                     tc_mma_f16_ta(d, a + 32 + k * 8, b0 + k * 2, idesc, 1);
                                 }
                             }
-                            tc_commit(bar(BAR_A_EMPTY + ra.slot));
-                            if (i == tiles - 1) tc_commit(bar(BAR_B_EMPTY + rt.slot));
-                            if (q == npairs - 1) tc_commit(bar(BAR_D_FULL + rd.slot));
+                            tc_commit(bar(BAR_A_EMPTY + slot));
+                            tc_commit(bar(BAR_B_EMPTY + rb.slot));  // (the other warp's arrival and this one's free the token tile)
+                            if (q == npairs - 1) tc_commit(bar(BAR_D_FULL + tile));
                         }
                         __syncwarp();
-                        ra.next();
-                        rt.next();
+                        rb.next();
                     }
-                    if (!ok) break;
-                    rd.next(); dcount = min(dcount + 1, kDBufs);
+                    steps++;
+                } else {
+                    for (int q = 0; q < npairs && ok; q++) {  // no such tile in this unit: it only lets the token tiles go
+                        ok = __all_sync(0xffffffffu, bar_wait(bar(BAR_B_FULL + rb.slot), rb.phase, abortp));
+                        if (ok && lane == 0) mbar_arrive(bar(BAR_B_EMPTY + rb.slot));
+                        rb.next();
+                    }
                 }
-                for (int q = 0; q < npairs; q++) rb.next();
+                pairs += (uint32_t)(un.tiles * npairs);
             }
         }
         if (!ok && elect_one()) {  // a wait ran out: let what was issued finish before tensor memory is given back
-            tc_commit(bar(BAR_END));
+            tc_commit(bar(BAR_END + tile));
             const long long t0 = clock64();
-            while (!mbar_try(bar(BAR_END), 0) && clock64() - t0 < 200000000LL) {}
+            while (!mbar_try(bar(BAR_END + tile), 0) && clock64() - t0 < 200000000LL) {}
         }
         __syncwarp();
     } else if (warp < 8) {
         // ================= widen: weight tiles -> operand A =================
         const int wg = warp >> 2, r = (warp & 3) * 32 + lane;
-        const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // TMEM lane of the warp's first row, in bits 16+
+        const uint32_t put_at = tmem + ((uint32_t)(warp & 3) << 21) + L::colA + (uint32_t)(wg * 32);  // TMEM lane of the warp's first row in bits 16+
+        // the row's words in a weight tile: this warp group's two groups of a chunk, 16-byte pieces swizzled by the row
+        uint32_t piece[2][2];
+#pragma unroll
+        for (int q = 0; q < 2; q++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) piece[q][h] = (uint32_t)r * 128u + (uint32_t)(((4 * q + 2 * wg + h) ^ (r & 7)) << 4);
         Ring<kWSlots> rw;
         Ring<kA> ra;
         Ring<kFSteps> rf;
         int ahead = 0;  // operand slots used so far (up to all); the two groups of four warps take a group of 64 inputs each
         bool ok = true;
-        // the steps in order; the scales of a step are fetched while the one before it is worked on
+        // one group's operand into its half of the next slot of TMEM
+        uint32_t turn = 0;  // bit i: which of tile i's two barriers announces its next slot
+        auto put = [&](const uint32_t (&a)[32], int i) {
+            ok = __all_sync(0xffffffffu, ahead < kA || bar_wait(bar(BAR_A_EMPTY + ra.slot), ra.phase ^ 1, abortp));
+            if (!ok) return;
+            tc_fence_after();
+            tc_st32(put_at + (uint32_t)(ra.slot * 64), a);
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(BAR_A_FULL + 2 * i + (int)(turn >> i & 1)));
+            turn ^= 1u << i;
+            ra.next();
+            ahead = min(ahead + 1, kA);
+        };
+        // scales of the next chunk, a tile's row each: fetched a chunk ahead, those of a unit's first one before the bias block
+        const unsigned char *sp[T];
+        uint2 sc[T];
+        auto aim = [&](const Unit &un) {
+#pragma unroll
+            for (int i = 0; i < T; i++) {
+                sp[i] = row_ptr(un, i < un.tiles ? i : 0, r, false);
+                sc[i] = chunk_scales(sp[i], 0, G, g.wide);
+            }
+        };
         Unit un;
-        int u = blockIdx.x, c = 0, i = 0;
-        uint2 sc = make_uint2(0, 0);
+        int u = blockIdx.x;
         if (u < nunits) {
             un = unit_at<MODE, T>(g, u);
-            sc = chunk_scales(row_ptr(un, 0, r, false), 0, G, g.wide);
+            aim(un);
         }
         while (u < nunits && ok) {
-            Unit un2 = un;
-            int u2 = u, c2 = c, i2 = i + 1;
-            if (i2 == un.tiles) { i2 = 0; c2++; }
-            if (c2 == nchunks) {
-                c2 = 0; u2 = u + gridDim.x;
-                if (u2 < nunits) un2 = unit_at<MODE, T>(g, u2);
-            }
-            uint2 sc2 = make_uint2(0, 0);
-            if (u2 < nunits && c2 < nreal) sc2 = chunk_scales(row_ptr(un2, i2, r, false), c2, G, g.wide);
-
-            const bool real = c < nreal;
-            const int na = real ? min(kChunk, G - c * kChunk) : 2;
-            int e = 0;
-            uint32_t pw[32];  // bias block: this thread's term of its row, as fp16 pairs
-            if (real) {
-                e = chunk_exponent(sc);
-                ok = __all_sync(0xffffffffu, bar_wait(bar(BAR_W_FULL + rw.slot), rw.phase, abortp));
-            } else {
-                // b + 8 s of the row's groups; warps 0-3 take the first term, the others the second
-                float v[64];
-                const int g0 = (c - nreal) * 64, gn = min(64, G - g0);
-                if (g.wide) {  // both tiles came like weight tiles, 64 bf16 to a row
-                    Ring<kWSlots> rs = rw;
-                    ok = __all_sync(0xffffffffu, bar_wait(bar(BAR_W_FULL + rs.slot), rs.phase, abortp));
-                    const uint32_t srow = sW + (uint32_t)rs.slot * kWSlot + (uint32_t)r * 128u;
-                    rs.next();
-                    ok = ok && __all_sync(0xffffffffu, bar_wait(bar(BAR_W_FULL + rs.slot), rs.phase, abortp));
-                    const uint32_t brow = sW + (uint32_t)rs.slot * kWSlot + (uint32_t)r * 128u;
+            for (int c = 0; c < nreal && ok; c++) {
+                const int na = min(kChunk, G - c * kChunk);
+#pragma unroll
+                for (int i = 0; i < T; i++) {
+                    if (i >= un.tiles || !ok) break;
+                    const uint2 s = sc[i];
+                    if (c + 1 < nreal) sc[i] = chunk_scales(sp[i], c + 1, G, g.wide);
+                    const int e = chunk_exponent(s);
+                    const float up = pow2(127 + 141 - e);  // the largest scale comes to [2^14, 2^15)
+                    // for the epilogue: what the step's sums have to be multiplied with (seen through A_FULL, the MMAs and D_FULL)
+                    if (wg == 0) s_f[rf.slot * 128 + r] = pow2(127 + e - 141 + 24);
+                    ok = __all_sync(0xffffffffu, bar_wait(bar(BAR_W_FULL + rw.slot), rw.phase, abortp));
                     if (!ok) break;
+                    const uint32_t tile = sW + (uint32_t)rw.slot * kWSlot;
+                    uint4 w4[2][2];
 #pragma unroll
-                    for (int q = 0; q < 8; q++) {
-                        if (q * 8 >= gn) {
+                    for (int q = 0; q < 2; q++)
 #pragma unroll
-                            for (int k = 0; k < 8; k++) v[8 * q + k] = 0.f;
-                            continue;
+                        for (int h = 0; h < 2; h++) w4[q][h] = ld_shared16(tile + piece[q][h]);
+#pragma unroll
+                    for (int q = 0; q < 2; q++) {
+                        if (2 * q >= na || !ok) break;  // (of an odd number of groups the last slot's second half is zeros)
+                        const uint32_t bits = q ? s.y : s.x;
+                        const float mf = __uint_as_float(wg ? bits & 0xffff0000u : bits << 16) * up;
+                        const uint32_t m = dup_h2(mf), m16 = dup_h2(mf * 0.0625f), mc = dup_h2(mf * -0x1p-21f);
+                        uint32_t a[32];
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            widen_word(w4[q][h].x, m, m16, mc, a + h * 16);
+                            widen_word(w4[q][h].y, m, m16, mc, a + h * 16 + 4);
+                            widen_word(w4[q][h].z, m, m16, mc, a + h * 16 + 8);
+                            widen_word(w4[q][h].w, m, m16, mc, a + h * 16 + 12);
                         }
-                        const uint4 s4 = ld_shared16(srow + (uint32_t)((q ^ (r & 7)) << 4)), b4 = ld_shared16(brow + (uint32_t)((q ^ (r & 7)) << 4));
-                        const uint32_t sw[4] = {s4.x, s4.y, s4.z, s4.w}, bw[4] = {b4.x, b4.y, b4.z, b4.w};
+                        put(a, i);
+                    }
+                    if (lane == 0) mbar_arrive(bar(BAR_W_EMPTY + rw.slot));  // (the last put brought the warp together)
+                    rw.next();
+                    rf.next();
+                }
+            }
+            const Unit cur = un;
+            u += gridDim.x;
+            if (u < nunits) {
+                un = unit_at<MODE, T>(g, u);
+                aim(un);
+            }
+            for (int c = 0; c < g.pseudo && ok; c++) {
+                const int gn = min(64, G - c * 64);
+                for (int i = 0; i < cur.tiles && ok; i++) {
+                    // b + 8 s of the row's groups; warps 0-3 take the first fp16 term, the others the second
+                    float v[64];
+                    uint32_t pw[32];
+                    if (g.wide) {  // both tiles came like weight tiles, 64 bf16 to a row
+                        Ring<kWSlots> rs = rw;
+                        ok = __all_sync(0xffffffffu, bar_wait(bar(BAR_W_FULL + rs.slot), rs.phase, abortp));
+                        const uint32_t srow = sW + (uint32_t)rs.slot * kWSlot + (uint32_t)r * 128u;
+                        rs.next();
+                        ok = ok && __all_sync(0xffffffffu, bar_wait(bar(BAR_W_FULL + rs.slot), rs.phase, abortp));
+                        const uint32_t brow = sW + (uint32_t)rs.slot * kWSlot + (uint32_t)r * 128u;
+                        if (!ok) break;
 #pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            v[8 * q + 2 * k] = fmaf(8.f, __uint_as_float(sw[k] << 16), __uint_as_float(bw[k] << 16));
-                            v[8 * q + 2 * k + 1] = fmaf(8.f, __uint_as_float(sw[k] & 0xffff0000u), __uint_as_float(bw[k] & 0xffff0000u));
+                        for (int q = 0; q < 8; q++) {
+                            if (q * 8 >= gn) {
+#pragma unroll
+                                for (int k = 0; k < 8; k++) v[8 * q + k] = 0.f;
+                                continue;
+                            }
+                            const uint4 s4 = ld_shared16(srow + (uint32_t)((q ^ (r & 7)) << 4)), b4 = ld_shared16(brow + (uint32_t)((q ^ (r & 7)) << 4));
+                            const uint32_t sw[4] = {s4.x, s4.y, s4.z, s4.w}, bw[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                v[8 * q + 2 * k] = fmaf(8.f, __uint_as_float(sw[k] << 16), __uint_as_float(bw[k] << 16));
+                                v[8 * q + 2 * k + 1] = fmaf(8.f, __uint_as_float(sw[k] & 0xffff0000u), __uint_as_float(bw[k] & 0xffff0000u));
+                            }
                         }
+                    } else {
+                        const uint16_t *ps = reinterpret_cast<const uint16_t *>(row_ptr(cur, i, r, false)) + c * 64;
+                        const uint16_t *pb = reinterpret_cast<const uint16_t *>(row_ptr(cur, i, r, true)) + c * 64;
+#pragma unroll
+                        for (int q = 0; q < 64; q++) v[q] = q < gn ? fmaf(8.f, bf16_bits_to_float(__ldg(ps + q)), bf16_bits_to_float(__ldg(pb + q))) : 0.f;
                     }
-                } else {
-                    const uint16_t *ps = reinterpret_cast<const uint16_t *>(row_ptr(un, i, r, false)) + g0;
-                    const uint16_t *pb = reinterpret_cast<const uint16_t *>(row_ptr(un, i, r, true)) + g0;
+                    float m = 0.f;
 #pragma unroll
-                    for (int q = 0; q < 64; q++) v[q] = q < gn ? fmaf(8.f, bf16_bits_to_float(__ldg(ps + q)), bf16_bits_to_float(__ldg(pb + q))) : 0.f;
-                }
-                float m = 0.f;
+                    for (int q = 0; q < 64; q++) m = fmaxf(m, fabsf(v[q]));
+                    const int e = max((int)(__float_as_uint(m) >> 23), 16);
+                    const float up = pow2(127 + 135 - e);
 #pragma unroll
-                for (int q = 0; q < 64; q++) m = fmaxf(m, fabsf(v[q]));
-                e = max((int)(__float_as_uint(m) >> 23), 16);
-                const float up = pow2(127 + 135 - e);
-#pragma unroll
-                for (int q = 0; q < 32; q++) {
-                    const float a0 = v[2 * q] * up, a1 = v[2 * q + 1] * up;
-                    const __half2 h = __floats2half2_rn(a0, a1);
-                    const float2 hf = __half22float2(h);
-                    pw[q] = h2_bits(wg == 0 ? h : __floats2half2_rn(a0 - hf.x, a1 - hf.y));
-                }
-            }
-            if (!ok) break;
-            // for the epilogue: what the step's sums have to be multiplied with (seen through A_FULL, the MMAs and D_FULL)
-            if (wg == 0) s_f[rf.slot * 128 + r] = real ? pow2(127 + e - 141 + 24) : pow2(127 + e - 135);
-            // one group's operand into its half of the next slot of TMEM
-            auto put = [&](const uint32_t (&a)[32], bool any) {
-                ok = __all_sync(0xffffffffu, ahead < kA || bar_wait(bar(BAR_A_EMPTY + ra.slot), ra.phase ^ 1, abortp));
-                if (!ok) return;
-                if (any) {
-                    tc_fence_after();
-                    tc_st32(tmem + lanes + L::colA + (uint32_t)(ra.slot * 64 + wg * 32), a);
-                    tc_wait_st();
-                    tc_fence_before();
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar(BAR_A_FULL + ra.slot));
-                ra.next();
-                ahead = min(ahead + 1, kA);
-            };
-            if (real) {
-                const float up = pow2(127 + 141 - e);  // the largest scale comes to [2^14, 2^15)
-                const uint32_t wrow = sW + (uint32_t)rw.slot * kWSlot + (uint32_t)r * 128u;
-                for (int j = wg; j < na + wg && ok; j += 2) {  // (of an odd number the second half of the last slot stays empty)
-                    const float mf = __uint_as_float(((j & 2 ? sc.y : sc.x) >> ((j & 1) * 16)) << 16) * up;
-                    const uint32_t m = dup_h2(mf), m16 = dup_h2(mf * 0.0625f), mc = dup_h2(mf * -0x1p-21f);
-                    uint32_t a[32];
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const uint4 w4 = ld_shared16(wrow + (uint32_t)(((2 * j + h) ^ (r & 7)) << 4));
-                        widen_word(w4.x, m, m16, mc, a + h * 16);
-                        widen_word(w4.y, m, m16, mc, a + h * 16 + 4);
-                        widen_word(w4.z, m, m16, mc, a + h * 16 + 8);
-                        widen_word(w4.w, m, m16, mc, a + h * 16 + 12);
+                    for (int q = 0; q < 32; q++) {
+                        const float a0 = v[2 * q] * up, a1 = v[2 * q + 1] * up;
+                        const __half2 h = __floats2half2_rn(a0, a1);
+                        const float2 hf = __half22float2(h);
+                        pw[q] = h2_bits(wg == 0 ? h : __floats2half2_rn(a0 - hf.x, a1 - hf.y));
                     }
-                    put(a, j < na);
+                    if (wg == 0) s_f[rf.slot * 128 + r] = pow2(127 + e - 135);
+                    put(pw, i);
+                    for (int k = 0; k < (g.wide ? 2 : 0); k++) {
+                        if (lane == 0) mbar_arrive(bar(BAR_W_EMPTY + rw.slot));
+                        rw.next();
+                    }
+                    rf.next();
                 }
-            } else {
-                put(pw, true);
             }
-            const int used = real ? 1 : g.wide ? 2 : 0;  // weight slots of the step
-            for (int k = 0; k < used; k++) {
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar(BAR_W_EMPTY + rw.slot));
-                rw.next();
-            }
-            rf.next();
-            un = un2; u = u2; c = c2; i = i2; sc = sc2;
         }
     } else {
         // ================= epilogue =================
         const int r = (warp & 3) * 32 + lane, half = (warp - 8) >> 2;  // columns half * 48 .. + 47
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;
-        Ring<kDBufs> rd;
+        uint32_t seen = 0;  // bit i: parity of tile i's next step
         Ring<kFSteps> rf;
         bool ok = true;
         for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x) {
@@ -562,11 +590,11 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
             for (int c = 0; c < nchunks && ok; c++) {
                 const bool last = c == nchunks - 1;
                 for (int i = 0; i < un.tiles && ok; i++) {
-                    ok = __all_sync(0xffffffffu, bar_wait(bar(BAR_D_FULL + rd.slot), rd.phase, abortp));
+                    ok = __all_sync(0xffffffffu, bar_wait(bar(BAR_D_FULL + i), seen >> i & 1, abortp));
                     if (!ok) break;
                     tc_fence_after();
                     uint32_t d[3][16];
-                    const uint32_t tstep = tmem + lanes + kColStep + (uint32_t)(rd.slot * kTok + half * kHalf);
+                    const uint32_t tstep = tmem + lanes + kColStep + (uint32_t)(i * kTok + half * kHalf);
                     const uint32_t tsum = tmem + lanes + kColSum + (uint32_t)(i * kTok + half * kHalf);
                     if (live > 0) {
                         tc_ld16(tstep, d[0]);
@@ -576,10 +604,10 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
                     }
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(bar(BAR_D_EMPTY + rd.slot));
+                    if (lane == 0) mbar_arrive(bar(BAR_D_EMPTY + i));
                     const float f = s_f[rf.slot * 128 + r];
                     rf.next();
-                    rd.next();
+                    seen ^= 1u << i;
                     uint64_t ff;
                     asm("mov.b64 %0, {%1, %1};\n" : "=l"(ff) : "f"(f));
                     const int row = tile_row<MODE>(un, i) + r;
