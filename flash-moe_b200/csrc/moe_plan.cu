@@ -45,10 +45,18 @@ moe_plan_kernel(const int *__restrict__ ids, int pairs, int first_expert, int nu
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     s_count[tid] = 0;
     __syncthreads();
-    for (int p = tid; p < pairs; p += kPlanThreads) {
-        const int e = local_expert(__ldg(ids + p), first_expert, num_experts);
-        if (e >= 0) atomicAdd(s_count + e, 1);
-    }
+    // eight ids per thread in flight
+    auto each = [&](auto &&use) {
+        for (int p0 = tid; p0 < pairs; p0 += 8 * kPlanThreads) {
+            int e[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) e[i] = p0 + i * kPlanThreads < pairs ? local_expert(__ldg(ids + p0 + i * kPlanThreads), first_expert, num_experts) : -1;
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (e[i] >= 0) use(e[i], p0 + i * kPlanThreads);
+        }
+    };
+    each([&](int e, int) { atomicAdd(s_count + e, 1); });
     __syncthreads();
     const int count = s_count[tid], tiles = (count + tile - 1) / tile;
     int end = count, tend = tiles;
@@ -58,10 +66,7 @@ moe_plan_kernel(const int *__restrict__ ids, int pairs, int first_expert, int nu
     for (int i = 0; i < tiles; i++) plan.jobs[tstart + i] = make_int4(tid, start + i * tile, min(tile, count - i * tile), 0);
     if (tid == kPlanThreads - 1) { plan.njobs[0] = tend; plan.njobs[1] = end; }
     __syncthreads();
-    for (int p = tid; p < pairs; p += kPlanThreads) {
-        const int e = local_expert(__ldg(ids + p), first_expert, num_experts);
-        if (e >= 0) plan.pair_of[atomicAdd(s_count + e, 1)] = p;
-    }
+    each([&](int e, int p) { plan.pair_of[atomicAdd(s_count + e, 1)] = p; });
 }
 
 // One CTA per token, four columns per thread (more where a row is longer than 4096).  The slots are summed in their order,

@@ -52,15 +52,8 @@ __device__ __forceinline__ void mma_u8s8_first(int (&d)[4], uint32_t a0, uint32_
 
 // Eight inputs (those of one weight word) of a token -> fixed point bytes in the order of the B fragments.
 // The eight threads of a group of 64 inputs sit in consecutive lanes.
-__device__ __forceinline__ void widen8(const float *x, bool valid, unsigned char *tok_group, float2 *factor, int wi) {
-    float v[8];
-    if (valid) {
-        const float4 a = __ldg(reinterpret_cast<const float4 *>(x)), b = __ldg(reinterpret_cast<const float4 *>(x) + 1);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = 0.f;
-    }
+__device__ __forceinline__ void widen8(const float4 &a, const float4 &b, bool valid, unsigned char *tok_group, float2 *factor, int wi) {
+    const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
     float am = 0.f, sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; i++) am = fmaxf(am, fabsf(v[i]));
@@ -101,32 +94,40 @@ __device__ __forceinline__ void widen8(const float *x, bool valid, unsigned char
     if (wi < 2) factor[wi] = make_float2(wi == 0 ? down * 65536.f : down, sum);
 }
 
-// S groups of a row pair as a lane holds them: 8 bytes of words per group and row, the scales of rows g and g + 8, and the
-// bias of row g (even lanes) or g + 8 (odd lanes).
-template <int S>
+constexpr int S = 4;             // groups per step
+// A step of a row pair as a lane holds it: 8 bytes of words per group and row, the scales of rows g and g + 8, and the bias of
+// row g (even lanes) or g + 8 (odd lanes).
 struct Held {
     uint2 w[kTiles][2][S];
-    uint32_t sc[kTiles][2][(S + 1) / 2], bi[kTiles][(S + 1) / 2];
+    uint2 sc[kTiles][2], bi[kTiles];
 };
-template <int S>
-__device__ __forceinline__ void load_bf16s(uint32_t (&d)[(S + 1) / 2], const unsigned char *p) {
-    if constexpr (S == 4) {
-        const uint2 v = __ldg(reinterpret_cast<const uint2 *>(p));
-        d[0] = v.x; d[1] = v.y;
+// The bf16 numbers of a step's groups: in one read where a row of them is a multiple of 8 bytes, 8-byte aligned; else one by
+// one, those behind the row's end repeating its last (their activations count nothing).
+template <bool WIDE>
+__device__ __forceinline__ uint2 load_bf16s(const unsigned char *row, int step, int G) {
+    if constexpr (WIDE) {
+        return __ldg(reinterpret_cast<const uint2 *>(row) + step);
     } else {
-        d[0] = __ldg(reinterpret_cast<const uint16_t *>(p));
+        const uint16_t *p = reinterpret_cast<const uint16_t *>(row);
+        const int j = step * S, last = G - 1;
+        return make_uint2((uint32_t)__ldg(p + j) | (uint32_t)__ldg(p + min(j + 1, last)) << 16,
+                          (uint32_t)__ldg(p + min(j + 2, last)) | (uint32_t)__ldg(p + min(j + 3, last)) << 16);
     }
 }
-__device__ __forceinline__ float bf16_at(uint32_t pair, int j) { return __uint_as_float(j & 1 ? pair & 0xffff0000u : pair << 16); }
+__device__ __forceinline__ float bf16_at(uint2 four, int j) {
+    const uint32_t pair = j & 2 ? four.y : four.x;
+    return __uint_as_float(j & 1 ? pair & 0xffff0000u : pair << 16);
+}
 // The same value in every lane, and known to the compiler as such (values of at least 0).
 __device__ __forceinline__ int uniform(int v) { return __reduce_max_sync(0xffffffffu, v); }
 
-// Warps: WK of them side by side along a row's steps (S groups each), 8 / WK along the rows.
-template <Q4Mode MODE, int NTL, int S>
+// Warps: WK of them side by side along a row's steps, 8 / WK along the rows.
+template <Q4Mode MODE, int NTL, bool WIDE>
 __global__ void __launch_bounds__(kThreads, NTL == 4 ? 1 : 2)
 q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units_per_job, int fixed_jobs, int wk_log2) {
     extern __shared__ __align__(16) unsigned char smem[];
     constexpr int kTok = 2 * NTL;
+    constexpr int kAhead = NTL == 4 ? 4 : 1;  // words of activations a thread has under way: as many as fit beside the weights' registers
     unsigned char *s_b = smem;                                                                      // [NTL][2 tokens][chunk][256]
     float2 *s_f = reinterpret_cast<float2 *>(smem + (size_t)kTok * chunk_groups * kTokBytes);       // [NTL][chunk][4]
     float *s_red = reinterpret_cast<float *>(reinterpret_cast<unsigned char *>(s_f) + (size_t)NTL * chunk_groups * kFactorBytes);  // [2][warp][tok][32 rows]
@@ -135,7 +136,9 @@ q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units
     const int G = p.in_dim / 64;
     const uint32_t w_pitch = (uint32_t)G * 32, s_pitch = (uint32_t)G * 2;
     const int nchunks = (G + chunk_groups - 1) / chunk_groups;
-    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    // The weights, the ids and the plan were there before the gate / up launch in front of a kDown one began (that one waited for
+    // them): only its activations have to be waited for, so the first weights are fetched under its tail.
+    if constexpr (MODE != kDown) asm volatile("griddepcontrol.wait;\n" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     const int njobs = p.plan.njobs != nullptr ? uniform(*p.plan.njobs) : fixed_jobs;
     const long long units = (long long)njobs * units_per_job;
@@ -159,7 +162,7 @@ q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units
         }
     };
 
-    Held<S> h;
+    Held h;
     // where the lane's rows start: offsets of rows g and g + 8 of each tile (rows without a place read the last one there is)
     const unsigned char *bw[kTiles], *bs[kTiles], *bb[kTiles];
     uint32_t ow[kTiles][2], os[kTiles][2], ob[kTiles];
@@ -190,24 +193,26 @@ q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units
         }
     };
     const unsigned char *pw[kTiles][2];  // the step being fetched
+    int left = S;                        // its groups that exist
     auto point = [&](int step) {
 #pragma unroll
         for (int i = 0; i < kTiles; i++)
 #pragma unroll
             for (int q = 0; q < 2; q++) pw[i][q] = bw[i] + (ow[i][q] + (uint32_t)step * (S * 32u));
+        if constexpr (!WIDE) left = G - step * S;
     };
-    auto fetch_words = [&](int j) {  // group j of the step (of S groups)
+    auto fetch_words = [&](int j) {  // group j of the step (behind the row's end: its last group again)
 #pragma unroll
         for (int i = 0; i < kTiles; i++)
 #pragma unroll
-            for (int q = 0; q < 2; q++) h.w[i][q][j] = __ldg(reinterpret_cast<const uint2 *>(pw[i][q] + j * 32));
+            for (int q = 0; q < 2; q++) h.w[i][q][j] = __ldg(reinterpret_cast<const uint2 *>(pw[i][q] + (WIDE ? j : min(j, left - 1)) * 32));
     };
     auto fetch_scales = [&](int step) {
 #pragma unroll
         for (int i = 0; i < kTiles; i++) {
-            load_bf16s<S>(h.sc[i][0], bs[i] + (os[i][0] + (uint32_t)step * (S * 2)));
-            load_bf16s<S>(h.sc[i][1], bs[i] + (os[i][1] + (uint32_t)step * (S * 2)));
-            load_bf16s<S>(h.bi[i], bb[i] + (ob[i] + (uint32_t)step * (S * 2)));
+            h.sc[i][0] = load_bf16s<WIDE>(bs[i] + os[i][0], step, G);
+            h.sc[i][1] = load_bf16s<WIDE>(bs[i] + os[i][1], step, G);
+            h.bi[i] = load_bf16s<WIDE>(bb[i] + ob[i], step, G);
         }
     };
 
@@ -245,11 +250,12 @@ q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units
         for (int j = 0; j < S; j++) fetch_words(j);
         fetch_scales(wk);
     };
-    const bool has_first = wk < min(chunk_groups, G) / S;  // this warp has a step in a unit's first chunk
+    const bool has_first = wk < (min(chunk_groups, G) + S - 1) / S;  // this warp has a step in a unit's first chunk
     if (u < u1) {
         aim(un);
         if (has_first) fetch_first();
     }
+    if constexpr (MODE == kDown) asm volatile("griddepcontrol.wait;\n" ::: "memory");
     const unsigned char *lane_b = s_b + (size_t)(g >> 2) * chunk_groups * kTokBytes + ((g & 3) * 4 + t) * 16;
     while (u < u1) {
         const int ntl = (un.cnt + 1) / 2;
@@ -257,7 +263,7 @@ q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units
         Unit nx = un;
         long long v = u;
         for (int c = 0; c < nchunks; c++) {
-            const int cg0 = c * chunk_groups, cgn = min(chunk_groups, G - cg0), step0 = cg0 / S, steps = cgn / S;
+            const int cg0 = c * chunk_groups, cgn = min(chunk_groups, G - cg0), step0 = cg0 / S, steps = (cgn + S - 1) / S;
             // activations of the job: of one token the source is the token, so consecutive single-token jobs share them
             int source = un.start;
             if (MODE == kGateUp && un.cnt == 1) source = pair_at(un.start, 0) / p.top_k;
@@ -266,14 +272,33 @@ q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units
                 __syncthreads();  // everyone is done with the previous activations
                 const int words = cgn * 8, total = un.cnt * words;
                 int tok = 0, w8 = tid;
-                for (int i0 = 0; i0 < total; i0 += kThreads, w8 += kThreads) {
-                    while (w8 >= words && tok < un.cnt) { w8 -= words; tok++; }
-                    const bool valid = tok < un.cnt;
-                    int row = pair_at(un.start, valid ? tok : 0);
-                    if (MODE == kGateUp) row /= p.top_k;
-                    unsigned char *tb = s_b + ((size_t)tok * chunk_groups + (w8 >> 3)) * kTokBytes;
-                    float2 *f = s_f + ((size_t)(tok >> 1) * chunk_groups + (w8 >> 3)) * 4 + (tok & 1) * 2;
-                    widen8(p.x + (size_t)row * p.in_dim + (size_t)cg0 * 64 + (size_t)w8 * 8, valid, tb, f, w8 & 7);
+                for (int i0 = 0; i0 < total; i0 += kAhead * kThreads) {  // the loads of a batch are under way before the first is used
+                    float4 xa[kAhead], xb[kAhead];
+                    int at[kAhead], who[kAhead];
+#pragma unroll
+                    for (int k = 0; k < kAhead; k++) {
+                        while (w8 >= words && tok < un.cnt) { w8 -= words; tok++; }
+                        at[k] = w8; who[k] = tok;
+                        if (tok < un.cnt) {
+                            int row = pair_at(un.start, tok);
+                            if (MODE == kGateUp) row /= p.top_k;
+                            const float4 *src = reinterpret_cast<const float4 *>(p.x + (size_t)row * p.in_dim + (size_t)cg0 * 64 + (size_t)w8 * 8);
+                            xa[k] = __ldg(src); xb[k] = __ldg(src + 1);
+                        } else {
+                            xa[k] = xb[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        }
+                        w8 += kThreads;
+                    }
+#pragma unroll
+                    for (int k = 0; k < kAhead; k++) {
+                        unsigned char *tb = s_b + ((size_t)who[k] * chunk_groups + (at[k] >> 3)) * kTokBytes;
+                        float2 *f = s_f + ((size_t)(who[k] >> 1) * chunk_groups + (at[k] >> 3)) * 4 + (who[k] & 1) * 2;
+                        widen8(xa[k], xb[k], who[k] < un.cnt, tb, f, at[k] & 7);
+                    }
+                }
+                for (int i = tid; i < NTL * 4 * (steps * S - cgn); i += kThreads) {  // the last step's groups behind the row's end
+                    const int nt = i / (4 * (steps * S - cgn)), q = i - nt * 4 * (steps * S - cgn);
+                    s_f[((size_t)nt * chunk_groups + cgn) * 4 + q] = make_float2(0.f, 0.f);
                 }
                 held_start = source; held_job = kind;
                 __syncthreads();
@@ -284,7 +309,7 @@ q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units
                 int more = st + WK < steps ? step0 + st + WK : -1;
                 if (more < 0) {
                     if (c + 1 < nchunks) {
-                        if (wk < (min(chunk_groups, G - cg0 - chunk_groups)) / S) more = step0 + steps + wk;
+                        if (wk < (min(chunk_groups, G - cg0 - chunk_groups) + S - 1) / S) more = step0 + steps + wk;
                     } else {
                         next_unit(v, nx);
                         if (v < u1) {
@@ -293,11 +318,9 @@ q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units
                         }
                     }
                 }
-                uint32_t sc[kTiles][2][(S + 1) / 2], bi[kTiles][(S + 1) / 2];
+                uint2 sc[kTiles][2], bi[kTiles];
 #pragma unroll
-                for (int i = 0; i < kTiles; i++)
-#pragma unroll
-                    for (int q = 0; q < (S + 1) / 2; q++) { sc[i][0][q] = h.sc[i][0][q]; sc[i][1][q] = h.sc[i][1][q]; bi[i][q] = h.bi[i][q]; }
+                for (int i = 0; i < kTiles; i++) { sc[i][0] = h.sc[i][0]; sc[i][1] = h.sc[i][1]; bi[i] = h.bi[i]; }
                 if (more >= 0) { fetch_scales(more); point(more); }
                 const unsigned char *fb = lane_b + (size_t)st * S * kTokBytes;
                 const float2 *ff = s_f + (size_t)st * S * 4 + t;
@@ -324,9 +347,9 @@ q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units
                             mma_u8s8_first(d, a[i][0][0], a[i][0][1], a[i][0][2], a[i][0][3], bf.x, bf.y);
                             mma_u8s8(d, a[i][1][0], a[i][1][1], a[i][1][2], a[i][1][3], bf.z, bf.w);
                             // |d| <= 64 * 15 * 128, so two digits still fit an int; lane t holds the digit pair t & 1 of token t / 2
-                            acc[i][0][nt] = fmaf(bf16_at(sc[i][0][j / 2], j) * f.x, (float)(d[0] * 256 + d[1]), acc[i][0][nt]);
-                            acc[i][1][nt] = fmaf(bf16_at(sc[i][1][j / 2], j) * f.x, (float)(d[2] * 256 + d[3]), acc[i][1][nt]);
-                            accb[i][nt] = fmaf(bf16_at(bi[i][j / 2], j), f.y, accb[i][nt]);
+                            acc[i][0][nt] = fmaf(bf16_at(sc[i][0], j) * f.x, (float)(d[0] * 256 + d[1]), acc[i][0][nt]);
+                            acc[i][1][nt] = fmaf(bf16_at(sc[i][1], j) * f.x, (float)(d[2] * 256 + d[3]), acc[i][1][nt]);
+                            accb[i][nt] = fmaf(bf16_at(bi[i], j), f.y, accb[i][nt]);
                         }
                     }
                 }
@@ -375,40 +398,39 @@ size_t smem_bytes(int ntl, int chunk) {
     return (size_t)2 * ntl * chunk * kTokBytes + (size_t)ntl * chunk * kFactorBytes + (size_t)2 * kWarps * 2 * ntl * 32 * 4;
 }
 
-template <Q4Mode MODE, int NTL, int S>
+template <Q4Mode MODE, int NTL, bool WIDE>
 int launch_one(const Q4Params &p, int jobs, int sm_count, cudaStream_t st) {
     const int G = p.in_dim / 64;
-    int chunk = G;
-    while (smem_bytes(NTL, chunk) > kMaxSmem) chunk = ((chunk + 1) / 2 + 3) / 4 * 4;
+    int chunk = (G + S - 1) / S * S;  // whole steps
+    while (smem_bytes(NTL, chunk) > kMaxSmem) chunk = (chunk / 2 + S - 1) / S * S;
     const size_t smem = smem_bytes(NTL, chunk);
     static unsigned long long configured = 0;
     if (first_use_on_device(&configured) &&
-        cudaFuncSetAttribute(q4_stream_kernel<MODE, NTL, S>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem) != cudaSuccess)
+        cudaFuncSetAttribute(q4_stream_kernel<MODE, NTL, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem) != cudaSuccess)
         return -1;
     const int grid_max = sm_count * std::max(1, std::min(NTL == 4 ? 1 : 2, (int)((220 * 1024) / (smem + 1024))));
-    // Warps along a row (at most as many as it has steps), the others side by side on more rows.  A unit costs its steps and an
+    // Warps along a row, the others side by side on more rows.  A unit costs its steps and an
     // end worth about 1 1/3 of a step (the warps meet, the next unit's addresses); a CTA takes whole units: the cheapest split.
     int wk_log2 = 0, per_job = 0;
     double best = 0.0;
-    for (int k = 0; k <= 3 && (k == 0 || (1 << k) <= chunk / S); k++) {
+    for (int k = 0; k <= 3; k++) {
         const int rows = (MODE == kGateUp ? 16 : 32) * (kWarps >> k);
         int n = 0;
         for (int i = 0; i < (MODE == kGateUp ? 1 : p.nmat); i++) n += (p.mat[i].rows + rows - 1) / rows;
         const long long waves = ((long long)jobs * n + grid_max - 1) / grid_max;
-        const double cost = (double)waves * ((double)((G / S + (1 << k) - 1) >> k) * S + 1.33 * 4);
+        const double cost = (double)waves * ((double)(((G + S - 1) / S + (1 << k) - 1) >> k) + 1.33);
         if (k == 0 || cost < best) { best = cost; wk_log2 = k; per_job = n; }
     }
     const int grid = (int)std::min<long long>((long long)jobs * per_job, grid_max);
-    return launch_dependent(q4_stream_kernel<MODE, NTL, S>, dim3(grid), dim3(kThreads), smem, st, p, chunk, per_job, jobs, wk_log2) == cudaSuccess ? 1 : -1;
+    return launch_dependent(q4_stream_kernel<MODE, NTL, WIDE>, dim3(grid), dim3(kThreads), smem, st, p, chunk, per_job, jobs, wk_log2) == cudaSuccess ? 1 : -1;
 }
 
-// Four groups per step where a row has a multiple of four and its scales can be read four at a time; else one by one.
 template <Q4Mode MODE, int NTL>
 int launch_steps(const Q4Params &p, int jobs, int sm_count, cudaStream_t st) {
-    bool four = p.in_dim % 256 == 0;
+    bool wide = p.in_dim % (64 * S) == 0;
     for (int i = 0; i < p.nmat; i++)
-        four = four && (((uintptr_t)p.mat[i].scales | (uintptr_t)p.mat[i].biases | (uintptr_t)p.mat[i].s_stride) & 7) == 0;
-    return four ? launch_one<MODE, NTL, 4>(p, jobs, sm_count, st) : launch_one<MODE, NTL, 1>(p, jobs, sm_count, st);
+        wide = wide && (((uintptr_t)p.mat[i].scales | (uintptr_t)p.mat[i].biases | (uintptr_t)p.mat[i].s_stride) & 7) == 0;
+    return wide ? launch_one<MODE, NTL, true>(p, jobs, sm_count, st) : launch_one<MODE, NTL, false>(p, jobs, sm_count, st);
 }
 
 }  // namespace
