@@ -63,15 +63,19 @@ moe_plan_kernel(const int *__restrict__ ids, int pairs, int first_expert, int nu
     block_scan2(end, tend, s_a, s_b);
     const int start = end - count, tstart = tend - tiles;
     s_count[tid] = start;  // from here on the next free position
-    for (int i = 0; i < tiles; i++) plan.jobs[tstart + i] = make_int4(tid, start + i * tile, min(tile, count - i * tile), 0);
+    // jobs of equal size (in the tensor cores' steps of 16 where they are that large), not full ones and a remainder
+    int size = tiles > 0 ? (count + tiles - 1) / tiles : 0;
+    if (tile > 16) size = (size + 15) / 16 * 16;
+    for (int i = 0; i < tiles; i++) plan.jobs[tstart + i] = make_int4(tid, start + i * size, min(size, count - i * size), 0);  // (size <= tile: none is empty)
     if (tid == kPlanThreads - 1) { plan.njobs[0] = tend; plan.njobs[1] = end; }
     __syncthreads();
     each([&](int e, int p) { plan.pair_of[atomicAdd(s_count + e, 1)] = p; });
 }
 
-// One CTA per token, four columns per thread (more where a row is longer than 4096).  The slots are summed in their order,
-// so the result does not depend on the launch; eight of their loads are in flight at a time.
-constexpr int kCombineThreads = 1024;
+// One CTA per token.  The slots are summed in their order, so the result does not depend on the launch; eight of their loads
+// are in flight at a time.  A few tokens get four columns per thread (the row at once: 7 us for 10 slots of 4096), many get
+// small CTAs, four to an SM, which cover each other's meeting points (4096 tokens: 180 -> 150 us, 4.9 TB/s).
+constexpr int kCombineThreads = 1024, kCombineThreadsMany = 256;
 constexpr int kCombineBatch = 8;
 
 __global__ void __launch_bounds__(kCombineThreads)
@@ -142,7 +146,7 @@ int launch_moe_plan(const int *ids, int pairs, int first_expert, int num_experts
 
 int launch_moe_combine(const float *y, const int *ids, const float *weights, int n, int top_k, int first_expert, int num_experts, int hidden,
                        const float *residual, const uint16_t *norm_w, float eps, float *h_out, float *h_norm, cudaStream_t st) {
-    return launch_dependent(moe_combine_kernel, dim3(n), dim3(std::min(kCombineThreads, (hidden / 4 + 31) / 32 * 32)), 0, st, y, ids, weights, top_k, first_expert, num_experts, hidden, residual, norm_w, eps,
+    return launch_dependent(moe_combine_kernel, dim3(n), dim3(std::min(n > 296 ? kCombineThreadsMany : kCombineThreads, (hidden / 4 + 31) / 32 * 32)), 0, st, y, ids, weights, top_k, first_expert, num_experts, hidden, residual, norm_w, eps,
                             h_out, h_norm) == cudaSuccess ? 1 : -1;
 }
 

@@ -422,11 +422,8 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
         const int wg = warp >> 2, r = (warp & 3) * 32 + lane;
         const uint32_t put_at = tmem + ((uint32_t)(warp & 3) << 21) + L::colA + (uint32_t)(wg * 32);  // TMEM lane of the warp's first row in bits 16+
         // the row's words in a weight tile: this warp group's two groups of a chunk, 16-byte pieces swizzled by the row
-        uint32_t piece[2][2];
-#pragma unroll
-        for (int q = 0; q < 2; q++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) piece[q][h] = (uint32_t)r * 128u + (uint32_t)(((4 * q + 2 * wg + h) ^ (r & 7)) << 4);
+        // (the second group four pieces on: bit 2 of the piece's number)
+        const uint32_t piece0 = (uint32_t)r * 128u + (uint32_t)(((2 * wg) ^ (r & 7)) << 4), piece1 = (uint32_t)r * 128u + (uint32_t)(((2 * wg + 1) ^ (r & 7)) << 4);
         Ring<kWSlots> rw;
         Ring<kA> ra;
         Ring<kFSteps> rf;
@@ -466,11 +463,13 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
         while (u < nunits && ok) {
             for (int c = 0; c < nreal && ok; c++) {
                 const int na = min(kChunk, G - c * kChunk);
-#pragma unroll
-                for (int i = 0; i < T; i++) {
-                    if (i >= un.tiles || !ok) break;
-                    const uint2 s = sc[i];
-                    if (c + 1 < nreal) sc[i] = chunk_scales(sp[i], c + 1, G, g.wide);
+#pragma unroll 1  // (one copy of the loop's body: the four roles' code has to fit the instruction cache)
+                for (int i = 0; i < un.tiles && ok; i++) {
+                    const uint2 s = i ? sc[1] : sc[0];
+                    if (c + 1 < nreal) {  // (in place: a copy of the result would wait for it)
+                        if (i) sc[1] = chunk_scales(sp[1], c + 1, G, g.wide);
+                        else sc[0] = chunk_scales(sp[0], c + 1, G, g.wide);
+                    }
                     const int e = chunk_exponent(s);
                     const float up = pow2(127 + 141 - e);  // the largest scale comes to [2^14, 2^15)
                     // for the epilogue: what the step's sums have to be multiplied with (seen through A_FULL, the MMAs and D_FULL)
@@ -478,25 +477,23 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
                     ok = __all_sync(0xffffffffu, bar_wait(bar(BAR_W_FULL + rw.slot), rw.phase, abortp));
                     if (!ok) break;
                     const uint32_t tile = sW + (uint32_t)rw.slot * kWSlot;
-                    uint4 w4[2][2];
+                    const uint4 ws[2][2] = {{ld_shared16(tile + piece0), ld_shared16(tile + piece1)}, {ld_shared16(tile + (piece0 ^ 64u)), ld_shared16(tile + (piece1 ^ 64u))}};
 #pragma unroll
-                    for (int q = 0; q < 2; q++)
-#pragma unroll
-                        for (int h = 0; h < 2; h++) w4[q][h] = ld_shared16(tile + piece[q][h]);
-#pragma unroll
-                    for (int q = 0; q < 2; q++) {
-                        if (2 * q >= na || !ok) break;  // (of an odd number of groups the last slot's second half is zeros)
+                    for (int q = 0; q < 2; q++) {  // (of an odd number of groups the last slot's second half is zeros)
+                        if (2 * q >= na || !ok) break;
+                        const uint4 w0 = ws[q][0], w1 = ws[q][1];
                         const uint32_t bits = q ? s.y : s.x;
                         const float mf = __uint_as_float(wg ? bits & 0xffff0000u : bits << 16) * up;
                         const uint32_t m = dup_h2(mf), m16 = dup_h2(mf * 0.0625f), mc = dup_h2(mf * -0x1p-21f);
                         uint32_t a[32];
-#pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            widen_word(w4[q][h].x, m, m16, mc, a + h * 16);
-                            widen_word(w4[q][h].y, m, m16, mc, a + h * 16 + 4);
-                            widen_word(w4[q][h].z, m, m16, mc, a + h * 16 + 8);
-                            widen_word(w4[q][h].w, m, m16, mc, a + h * 16 + 12);
-                        }
+                        widen_word(w0.x, m, m16, mc, a);
+                        widen_word(w0.y, m, m16, mc, a + 4);
+                        widen_word(w0.z, m, m16, mc, a + 8);
+                        widen_word(w0.w, m, m16, mc, a + 12);
+                        widen_word(w1.x, m, m16, mc, a + 16);
+                        widen_word(w1.y, m, m16, mc, a + 20);
+                        widen_word(w1.z, m, m16, mc, a + 24);
+                        widen_word(w1.w, m, m16, mc, a + 28);
                         put(a, i);
                     }
                     if (lane == 0) mbar_arrive(bar(BAR_W_EMPTY + rw.slot));  // (the last put brought the warp together)

@@ -409,8 +409,8 @@ int launch_one(const Q4Params &p, int jobs, int sm_count, cudaStream_t st) {
         cudaFuncSetAttribute(q4_stream_kernel<MODE, NTL, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem) != cudaSuccess)
         return -1;
     const int grid_max = sm_count * std::max(1, std::min(NTL == 4 ? 1 : 2, (int)((220 * 1024) / (smem + 1024))));
-    // Warps along a row, the others side by side on more rows.  A unit costs its steps and an
-    // end worth about 1 1/3 of a step (the warps meet, the next unit's addresses); a CTA takes whole units: the cheapest split.
+    // Warps along a row, the others side by side on more rows.  A unit costs its steps and an end worth about 1 1/3 of a step of
+    // two tokens (the warps meet, the next unit's addresses); a CTA takes whole units: the cheapest split.
     int wk_log2 = 0, per_job = 0;
     double best = 0.0;
     for (int k = 0; k <= 3; k++) {
@@ -418,7 +418,7 @@ int launch_one(const Q4Params &p, int jobs, int sm_count, cudaStream_t st) {
         int n = 0;
         for (int i = 0; i < (MODE == kGateUp ? 1 : p.nmat); i++) n += (p.mat[i].rows + rows - 1) / rows;
         const long long waves = ((long long)jobs * n + grid_max - 1) / grid_max;
-        const double cost = (double)waves * ((double)(((G + S - 1) / S + (1 << k) - 1) >> k) + 1.33);
+        const double cost = (double)waves * ((double)(((G + S - 1) / S + (1 << k) - 1) >> k) + 2.66 / (1 + NTL));
         if (k == 0 || cost < best) { best = cost; wk_log2 = k; per_job = n; }
     }
     const int grid = (int)std::min<long long>((long long)jobs * per_job, grid_max);
