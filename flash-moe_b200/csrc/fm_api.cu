@@ -1056,6 +1056,8 @@ constexpr int kProjStreamTokens = 16;
 constexpr int kExpertStreamPairs = 3;
 
 static bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+static bool aligned2(const void *a, const void *b) { return (((uintptr_t)a | (uintptr_t)b) & 1) == 0; }
+static bool aligned4(const void *p) { return ((uintptr_t)p & 3) == 0; }
 
 extern "C" fm_status fm_proj_forward(FmCtx *ctx, int count, const FmProjWeights *w, int n, const float *x, float *const *y) {
     if (!ctx) return FM_ERR_INVALID;
@@ -1067,7 +1069,8 @@ extern "C" fm_status fm_proj_forward(FmCtx *ctx, int count, const FmProjWeights 
             return fail(ctx, FM_ERR_UNSUPPORTED, "fm_proj_forward: matrix %d: format %d, group size %d, %d x %d (in a multiple of 64 up to 65536)", i,
                         w[i].format, w[i].group_size, w[i].out_dim, w[i].in_dim);
         if (w[i].in_dim != w[0].in_dim) return fail(ctx, FM_ERR_INVALID, "fm_proj_forward: matrix %d reads %d inputs, matrix 0 reads %d", i, w[i].in_dim, w[0].in_dim);
-        if (!aligned16(w[i].w)) return fail(ctx, FM_ERR_INVALID, "fm_proj_forward: the words of matrix %d are not 16-byte aligned", i);
+        if (!aligned16(w[i].w) || !aligned2(w[i].scales, w[i].biases) || !aligned4(y[i]))
+            return fail(ctx, FM_ERR_INVALID, "fm_proj_forward: matrix %d: words have to be 16-byte aligned, scales and biases 2-byte, y 4-byte", i);
     }
     if (n == 0) return FM_OK;
     FM_CUDA(ctx, cudaSetDevice(ctx->cfg.device));
@@ -1130,10 +1133,13 @@ extern "C" fm_status fm_moe_route(FmCtx *ctx, const FmRouteConfig *rc, int n, co
     if (rc->score != FM_SCORE_SOFTMAX && rc->score != FM_SCORE_SIGMOID) return fail(ctx, FM_ERR_INVALID, "fm_moe_route: score %d", rc->score);
     if (rc->num_experts < 1 || rc->num_experts > 1024 || rc->top_k < 1 || rc->top_k > 32 || rc->num_groups < 1 || rc->num_groups > 32)
         return fail(ctx, FM_ERR_UNSUPPORTED, "fm_moe_route: %d experts (1..1024), top_k %d (1..32), %d groups (1..32)", rc->num_experts, rc->top_k, rc->num_groups);
+    if (rc->top_k + (rc->shared_expert != 0) > 32) return fail(ctx, FM_ERR_UNSUPPORTED, "fm_moe_route: top_k %d and the shared expert (32 slots)", rc->top_k);
     if (rc->num_experts % rc->num_groups || rc->top_groups < 1 || rc->top_groups > rc->num_groups || rc->group_best < 1 || rc->group_best > 2 ||
         rc->top_k > rc->num_experts / rc->num_groups * rc->top_groups || (rc->shared_expert != 0 && rc->shared_expert != 1))
         return fail(ctx, FM_ERR_INVALID, "fm_moe_route: %d experts in %d groups, the best %d by %d experts each, top_k %d, shared_expert %d", rc->num_experts,
                     rc->num_groups, rc->top_groups, rc->group_best, rc->top_k, rc->shared_expert);
+    if (!(rc->scale == rc->scale)) return fail(ctx, FM_ERR_INVALID, "fm_moe_route: scale is NaN");
+    if (!aligned4(logits) || !aligned4(bias) || !aligned4(expert_ids) || !aligned4(weights)) return fail(ctx, FM_ERR_INVALID, "fm_moe_route: arrays have to be 4-byte aligned");
     if (n < 0 || n > ctx->cfg.max_batch_tokens) return fail(ctx, FM_ERR_INVALID, "fm_moe_route: n=%d exceeds max_batch_tokens=%d", n, ctx->cfg.max_batch_tokens);
     if (n == 0) return FM_OK;
     FM_CUDA(ctx, cudaSetDevice(ctx->cfg.device));
@@ -1170,7 +1176,9 @@ extern "C" fm_status fm_moe_experts(FmCtx *ctx, const FmExpertWeights *w, int n,
     if (w->first_expert < 0 || w->expert_stride < 0 || w->expert_stride % 16)
         return fail(ctx, FM_ERR_INVALID, "fm_moe_experts: first_expert %d, expert_stride %lld (0 or a multiple of 16)", w->first_expert, (long long)w->expert_stride);
     if (n < 0 || n > ctx->cfg.max_batch_tokens) return fail(ctx, FM_ERR_INVALID, "fm_moe_experts: n=%d exceeds max_batch_tokens=%d", n, ctx->cfg.max_batch_tokens);
-    if (!aligned16(w->gate_w) || !aligned16(w->up_w) || !aligned16(w->down_w)) return fail(ctx, FM_ERR_INVALID, "fm_moe_experts: weight words are not 16-byte aligned");
+    if (!aligned16(w->gate_w) || !aligned16(w->up_w) || !aligned16(w->down_w) || !aligned2(w->gate_scales, w->gate_biases) || !aligned2(w->up_scales, w->up_biases) ||
+        !aligned2(w->down_scales, w->down_biases) || !aligned4(expert_ids) || !aligned4(weights))
+        return fail(ctx, FM_ERR_INVALID, "fm_moe_experts: weight words have to be 16-byte aligned, scales and biases 2-byte, expert_ids and weights 4-byte");
     if ((long long)n * top_k > (1 << 24)) return fail(ctx, FM_ERR_UNSUPPORTED, "fm_moe_experts: %d tokens with %d slots each", n, top_k);
     if (n == 0) return FM_OK;
     FM_CUDA(ctx, cudaSetDevice(ctx->cfg.device));

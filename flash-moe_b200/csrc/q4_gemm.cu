@@ -13,17 +13,27 @@
 // few 2^-24 per addition; so TMEM accumulates over 256 inputs only, and the parts are added in fp32 by the epilogue
 // warps, which apply the row's power of two in the same fused multiply-add.
 //
-// Organisation (persistent, one CTA per SM).  A unit is T row tiles of 128 rows and up to 64 tokens; a step is one tile
-// over one chunk of 4 groups.  kGateUp: the tiles alternate between gate and up, so that SwiGLU needs no exchange.
-//   warps 0-7    widen: a thread owns a row; two 16-byte reads from the TMA-filled weight tile, 13 instructions per word of
-//                eight nibbles, 32 TMEM columns (one group) per store.  Operand A lives in TMEM: written row by row where
-//                the MMA wants it, and half of the shared-memory traffic of an A tile there.
+// Organisation (persistent, one CTA per SM).  A unit is two row tiles of 128 rows (kGateUp: the same rows of gate and up, so
+// that SwiGLU needs no exchange) and up to 96 tokens; a step is one tile over one chunk of 4 groups.
+//   warps 0-7    widen: a thread owns a row; two 16-byte reads from the TMA-filled weight tile per group, 9 instructions per word
+//                of eight nibbles, 32 TMEM columns per store.  Operand A lives in TMEM: written row by row where the MMA wants
+//                it, and an MMA of N = 96 takes 57 cycles from there, 87 from shared memory.
 //   warps 8-15   epilogue: running sums in TMEM, added up per step; the last step of a tile writes the results, 128
 //                consecutive features per token and store
-//   warp 16      TMA producer of token tiles, hi | lo;  warp 18  of weight tiles [128 rows][128 bytes]
-//   warps 17, 19 issue the MMAs of a tile each (M128, N = the unit's tokens rounded up to 16, K16)
-// TMEM columns: T * 64 running sums, 2 * 64 of steps in flight, the rest operand A in slots of 64 (two groups).
-// With two terms the tensor work is twice the product's; what bounds a long prompt is that, a short one the weights' stream.
+//   warps 16, 18 TMA producers of token tiles (two groups, hi | lo each) and of weight tiles [128 rows][128 bytes]
+//   warps 17, 19 issue the MMAs of a tile each (M128, N = the unit's tokens rounded up to 16, K16): while one waits, the other's
+//                keep the tensor core busy
+// TMEM columns: 2 * 96 of steps in flight, 2 * 96 running sums, 2 * 64 operand A (two slots of two groups).
+// Why 96: sums, steps and operands share 512 columns, token tiles 144 KB; at 64 tokens a weight is widened half as often again
+// and the MMA's start-up counts more, at 128 the steps could not be double-buffered.
+//
+// Measured (B200, 1.9 GHz; the tensor work is twice the product's, because of the two terms): 4096 tokens x 4096 x 8192 in
+// 520 us, 530 TFLOP/s of products (the tensor core is busy 73 % of the time in MMAs of 57 cycles, ideal 48); 300 tokens through
+// qkv + z + beta + alpha of 4096 in 130 us; 4096 tokens through 10 of 512 experts of 4096 x 1024: gate / up 1.8 ms, down 1.0 ms.
+// What bounds it: the issue slots.  Widening, the epilogue and the hand-overs between the roles take 2000 to 2300 instructions
+// per operand slot of 915 tensor cycles; below 64 tokens a unit takes about 950 cycles per slot whatever its tokens.
+// Tried and not kept: 16 widening warps (the same time), the two issuing warps as one (+10 %), operand slots of one group
+// (+12 %), gathering token rows with tile::gather4 instead of in the split (+30 % of the gate / up launch).
 // Every wait is bounded; on expiry the CTA records an error code and winds down.
 #include <cuda.h>
 #include <cuda_fp16.h>

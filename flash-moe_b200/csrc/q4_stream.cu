@@ -14,10 +14,17 @@
 // exact; what is left of fp32's accuracy is 2^-30 of a group's largest input.  Scale and bias meet the group's sum in
 // fp32, once per row and group.
 //
-// A unit is 16 rows of one matrix pair (kGateUp: the same rows of gate and up; else 32 rows of one matrix) for one job.
-// The 8 warps of a CTA split the groups of a row among themselves and meet in shared memory at the unit's end; every
-// lane fetches 8 bytes of a row group straight into registers, several groups ahead.  CTAs are persistent and take a
-// contiguous range of units, so that a job's activations are widened once per CTA and not once per unit.
+// A unit is 32 rows per warp that stands alone along the row (kGateUp: 16 of gate and the same 16 of up) for one job.  The 8
+// warps of a CTA split the steps of a row (four groups each) and the unit's rows among themselves, by a cost rule in
+// launch_one, and meet in shared memory at the unit's end; a lane fetches 8 bytes of a row group straight into registers, and
+// refills them as it unpacks them, so that about 60 KB per SM are under way.  CTAs are persistent and take a contiguous range
+// of units, so that a job's activations are widened once per CTA and not once per unit, and the next unit's weights are
+// fetched while this one's sums meet.
+//
+// Measured (B200, weights from HBM): one token x 4096 x 17408 in 12.6 us (40 MB: 3.2 TB/s; 5.3 TB/s in the long run, 4.5 us go
+// into the start and the end), x 8192 x 4096 in 9.5 us; one token through 10 of 512 experts of 4096 x 1024 in 35 us with the
+// weighted sum; 48 tokens through them (2.2 GB) in 450 us, 4.9 TB/s.  Bound by issue slots next to the stream: 31 instructions
+// per 16 rows x 64 inputs, of which the unpacking takes 12.
 #include <math.h>
 
 #include <algorithm>

@@ -305,8 +305,9 @@ fm_status fm_out_proj_norm(FmCtx *ctx, const FmProjWeights *w, int n, const floa
  * shared expert's gate.  Replaces gpu_encode_batch_matvec / BatchMatvecSpec (metal_infer/gpu_dispatch.h) and, at prompt
  * size, dequant_gemm_4bit_batch (metal_infer/shaders.metal); CPU cpu_dequant_matvec (metal_infer/cpu_kernels.h:199-232).
  * x [n][in_dim], y[i] [n][out_dim_i] follow the pointer mode; the array y itself is a host array; weights are device
- * pointers in either mode, 16-byte aligned words.  in_dim a multiple of 64 (up to 65536) and the same for all, out_dim any;
- * n up to max_batch_tokens.
+ * pointers in either mode.  Words and x 16-byte aligned, the rest as its type; in_dim a multiple of 64 (up to 65536) and the
+ * same for all, out_dim any; n up to max_batch_tokens.  Up to 16 tokens nothing is allocated; the first call with more
+ * allocates workspace (so make it before a stream capture: FM_ERR_CAPACITY otherwise).
  * Accuracy is fp32's: the nibbles are exact on the tensor cores, an activation enters them as 22 bits or more, the scale and
  * bias of a group meet its sum in fp32.  A token with an infinity or a NaN among its inputs gets NaN outputs.
  * The outputs must not overlap each other or the inputs. */
@@ -326,7 +327,7 @@ fm_status fm_proj_forward(FmCtx *ctx, int count, const FmProjWeights *w, int n, 
  * shared_expert = 1: the logits have one more column, the shared expert's gate; each token gets one more slot, with id
  * num_experts and weight sigmoid(that logit), so that a shared expert stacked behind the routed ones runs with them.
  * logits [n][num_experts + shared_expert], bias [num_experts], expert_ids and weights [n][top_k + shared_expert] follow the
- * pointer mode.  num_experts <= 1024, top_k <= 32, num_groups <= 32. */
+ * pointer mode.  num_experts <= 1024, top_k + shared_expert <= 32, num_groups <= 32. */
 enum { FM_SCORE_SOFTMAX = 0, FM_SCORE_SIGMOID = 1 };
 typedef struct FmRouteConfig {
     int num_experts;     /* 512 */
@@ -358,7 +359,9 @@ fm_status fm_moe_route(FmCtx *ctx, const FmRouteConfig *rc, int n, const float *
  * An expert that several slots or tokens name is read once for all of them, as far as that pays; the same id twice in a
  * token counts twice.  x [n][hidden], expert_ids and weights [n][top_k] (top_k <= 32), residual, h_out and h_norm [n][hidden]
  * follow the pointer mode; h_out may be the residual itself, and x may be h_out or h_norm.  hidden and inter multiples of 64
- * (up to 65536), num_experts <= 1024, n up to max_batch_tokens.  Accuracy as for fm_proj_forward.
+ * (up to 65536), num_experts <= 1024, n up to max_batch_tokens.  Words, x, residual, h_out and h_norm 16-byte aligned, norm_w
+ * 8-byte, the rest as its type.  Accuracy as for fm_proj_forward; the result does not depend on the order of the tokens or on
+ * the launch.
  * The first call of a size allocates workspace (so make it before a stream capture: FM_ERR_CAPACITY otherwise); graphs
  * captured on one context share that workspace and must not run at the same time. */
 typedef struct FmExpertWeights {

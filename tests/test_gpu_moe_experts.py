@@ -265,7 +265,7 @@ def test_refusals(pkg):
         return e.value.status
     for bad in (dict(format=1), dict(group_size=128), dict(hidden=96), dict(inter=0), dict(inter=65600), dict(num_experts=0), dict(num_experts=1025), dict(top=0), dict(top=33)):
         assert status(**bad) == B.FM_ERR_UNSUPPORTED
-    for bad in (dict(first_expert=-1), dict(expert_stride=-16), dict(expert_stride=24), dict(n=9), dict(n=-1), dict(gate_w=None), dict(down_biases=None), dict(up_w=dev.up_w + 8),
+    for bad in (dict(first_expert=-1), dict(expert_stride=-16), dict(expert_stride=24), dict(n=9), dict(n=-1), dict(gate_w=None), dict(down_biases=None), dict(up_w=dev.up_w + 8), dict(down_scales=dev.down_scales + 1),
                 dict(x_=None), dict(ids_=None), dict(w_=None), dict(out_=None), dict(x_=x.view(-1)[1:129]), dict(out_=out.view(-1)[1:129]), dict(nrm=out.view(-1)[2:130]),
                 dict(res=x.view(-1)[3:131])):
         assert status(**bad) == B.FM_ERR_INVALID

@@ -116,10 +116,10 @@ def test_refusals(pkg):
             c.moe_route(pkg.route_config(**{**BASE, **kw}), n, *args)
         assert e.value.text.startswith("fm_moe_route")
         return e.value.status
-    for bad in (dict(num_experts=0), dict(num_experts=1025), dict(top_k=0), dict(top_k=33), dict(num_groups=0), dict(num_groups=64)):
+    for bad in (dict(num_experts=0), dict(num_experts=1025), dict(top_k=0), dict(top_k=33), dict(num_groups=0), dict(num_groups=64), dict(top_k=32, shared_expert=1)):
         assert status(**bad) == B.FM_ERR_UNSUPPORTED
     for bad in (dict(score=2), dict(top_k=5, num_groups=16, top_groups=1), dict(num_groups=3), dict(top_groups=2), dict(top_groups=0),
-                dict(num_groups=8, top_groups=2, group_best=3), dict(shared_expert=2), dict(n=5), dict(n=-1)):
+                dict(num_groups=8, top_groups=2, group_best=3), dict(shared_expert=2), dict(n=5), dict(n=-1), dict(scale=float("nan"))):
         assert status(**bad) == B.FM_ERR_INVALID
     assert status(args=(None, None, ids, w)) == B.FM_ERR_INVALID and status(args=(x, None, None, w)) == B.FM_ERR_INVALID
     c.moe_route(pkg.route_config(**BASE), 0, x, None, ids, w)

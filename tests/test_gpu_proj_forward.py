@@ -139,6 +139,7 @@ def test_refusals(pkg):
     assert status([changed(a, scales=None)], 1) == B.FM_ERR_INVALID
     assert status([changed(a, w=a.w + 4)], 1) == B.FM_ERR_INVALID
     assert status([a], 1, x_=x.view(-1)[1:129]) == B.FM_ERR_INVALID            # x off its 16-byte boundary
+    assert status([changed(a, scales=a.scales + 1)], 1) == B.FM_ERR_INVALID and status([changed(a, biases=a.biases + 1)], 1) == B.FM_ERR_INVALID
     c.proj_forward([a], 0, x, [y])                                             # no tokens: nothing to do
     c.synchronize()
     assert torch.all(y == 7.0)
