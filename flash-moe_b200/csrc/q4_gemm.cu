@@ -58,19 +58,17 @@ constexpr int kBSlots = 3;
 constexpr int kWSlot = 128 * 128;           // bytes of a weight tile: 128 rows, 4 groups
 constexpr int kWSlots = 4;
 constexpr int kGemmThreads = 20 * 32;
-constexpr int kDBufs = 2;                   // one per tile of a unit
+constexpr int T = 2;                        // row tiles of a unit
+constexpr int kDBufs = T;                   // steps in flight: one per tile
 // Steps whose row factors are kept: the widening warps are at most the operand slots (one to a step at the least), the
 // steps in flight and their own step ahead of the epilogue.
 constexpr int kFSteps = 16;
 constexpr int kHalf = kTok / 2;            // columns of an epilogue warp
 constexpr uint32_t kColStep = 0, kColSum = kDBufs * kTok;  // TMEM columns; operand A behind the sums
 
-template <int T>
-struct Layout {
-    static_assert(T == kDBufs, "a step buffer and an issuing warp per tile");
-    static constexpr uint32_t colA = kColSum + T * kTok;
-    static constexpr int aslots = (512 - (int)colA) / 64;  // of two groups
-};
+constexpr uint32_t kColA = kColSum + T * kTok;
+static_assert(kColA + 128 <= 512, "two operand slots of two groups each");
+constexpr int kA = 2;                       // operand slots
 
 enum Bar { BAR_W_FULL = 0, BAR_W_EMPTY = BAR_W_FULL + kWSlots, BAR_B_FULL = BAR_W_EMPTY + kWSlots, BAR_B_EMPTY = BAR_B_FULL + kBSlots,
            BAR_D_FULL = BAR_B_EMPTY + kBSlots, BAR_D_EMPTY = BAR_D_FULL + kDBufs, BAR_A_FULL = BAR_D_EMPTY + kDBufs,
@@ -132,7 +130,7 @@ struct Unit {
     int start, cnt, ncols; // tokens (kProj) or positions in pair_of; columns of the MMA
 };
 
-template <Q4Mode MODE, int T, bool WARP = true>
+template <Q4Mode MODE, bool WARP = true>
 __device__ __forceinline__ Unit unit_at(const GemmParams &g, int u) {
     Unit r;
     const int job = u / g.units_per_job;
@@ -239,14 +237,12 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
         }
     }
 }
-template <Q4Mode MODE, int T>
+template <Q4Mode MODE>
 __global__ void __launch_bounds__(kGemmThreads, 1)
 q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ GemmParams g) {
     extern __shared__ unsigned char smem_raw[];
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
-    using L = Layout<T>;
-    constexpr int kA = L::aslots;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t sB = base, sW = sB + kBSlots * kBSlot;
     float *s_f = reinterpret_cast<float *>(smem_raw + (sW + kWSlots * kWSlot - smem_u32(smem_raw)));  // [steps][128 rows] power of two of the step
@@ -301,7 +297,7 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
         int count = 0;
         bool ok = true;
         for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x) {
-            const Unit un = unit_at<MODE, T>(g, u);
+            const Unit un = unit_at<MODE>(g, u);
             for (int c = 0; c < nchunks && ok; c++) {
                 const int first = c < nreal ? c * kChunk : G + c - nreal, ng = c < nreal ? min(kChunk, G - first) : 1;  // 64 columns of x each
                 for (int j = 0; j < ng && ok; j += 2) {
@@ -328,7 +324,7 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
             int count = 0;
             bool ok = true;
             for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x) {
-                const Unit un = unit_at<MODE, T, false>(g, u);
+                const Unit un = unit_at<MODE, false>(g, u);
                 for (int c = 0; c < nchunks && ok; c++)
                     for (int i = 0; i < un.tiles && ok; i++) {
                         auto load = [&](const CUtensorMap *map, int x) {  // 128 bytes of each of the tile's rows
@@ -356,7 +352,7 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
         // across the warp (the reductions say so to the compiler), and an MMA costs what the tensor core takes, 57 cycles at
         // N = 96.  Issued by `lane == 0` in divergent code each took 120 to 190.
         const int tile = warp == 17 ? 0 : 1;
-        const uint32_t d = uniform(tmem) + kColStep + (uint32_t)(tile * kTok), a0 = uniform(tmem) + L::colA;
+        const uint32_t d = uniform(tmem) + kColStep + (uint32_t)(tile * kTok), a0 = uniform(tmem) + kColA;
         const uint64_t desc0 = smem_desc(sB, 0, 1024);
         constexpr uint64_t kTile = kBTile >> 4;  // in the descriptor's units of 16 bytes
         Ring<kBSlots> rb;
@@ -365,7 +361,7 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
         uint32_t pairs = 0, mine = 0, steps = 0;
         bool ok = true;
         for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x) {
-            const Unit un = unit_at<MODE, T>(g, u);
+            const Unit un = unit_at<MODE>(g, u);
             const uint32_t idesc = idesc_dense(128, un.ncols, false, 0);
             for (int c = 0; c < nchunks && ok; c++) {
                 const bool real = c < nreal;
@@ -430,7 +426,7 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
     } else if (warp < 8) {
         // ================= widen: weight tiles -> operand A =================
         const int wg = warp >> 2, r = (warp & 3) * 32 + lane;
-        const uint32_t put_at = tmem + ((uint32_t)(warp & 3) << 21) + L::colA + (uint32_t)(wg * 32);  // TMEM lane of the warp's first row in bits 16+
+        const uint32_t put_at = tmem + ((uint32_t)(warp & 3) << 21) + kColA + (uint32_t)(wg * 32);  // TMEM lane of the warp's first row in bits 16+
         // the row's words in a weight tile: this warp group's two groups of a chunk, 16-byte pieces swizzled by the row
         // (the second group four pieces on: bit 2 of the piece's number)
         const uint32_t piece0 = (uint32_t)r * 128u + (uint32_t)(((2 * wg) ^ (r & 7)) << 4), piece1 = (uint32_t)r * 128u + (uint32_t)(((2 * wg + 1) ^ (r & 7)) << 4);
@@ -467,7 +463,7 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
         Unit un;
         int u = blockIdx.x;
         if (u < nunits) {
-            un = unit_at<MODE, T>(g, u);
+            un = unit_at<MODE>(g, u);
             aim(un);
         }
         while (u < nunits && ok) {
@@ -514,7 +510,7 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
             const Unit cur = un;
             u += gridDim.x;
             if (u < nunits) {
-                un = unit_at<MODE, T>(g, u);
+                un = unit_at<MODE>(g, u);
                 aim(un);
             }
             for (int c = 0; c < g.pseudo && ok; c++) {
@@ -582,7 +578,7 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
         Ring<kFSteps> rf;
         bool ok = true;
         for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x) {
-            const Unit un = unit_at<MODE, T>(g, u);
+            const Unit un = unit_at<MODE>(g, u);
             // columns half * 48 + 32 q + lane: the row of the output it goes to, and what takes its token's power of two off again
             int out_row[2] = {0, 0};
             float ts[2] = {0.f, 0.f};
@@ -743,7 +739,7 @@ bool map_rows(CUtensorMap *m, const void *base, long long stride, int rows, int 
                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <Q4Mode MODE, int T>
+template <Q4Mode MODE>
 int launch_gemm(const GemmMaps &maps, GemmParams &g, long long jobs, int sm_count, cudaStream_t st) {
     constexpr int kRows = MODE == kGateUp ? T * 64 : T * 128;
     g.units_per_job = 0;
@@ -753,10 +749,10 @@ int launch_gemm(const GemmMaps &maps, GemmParams &g, long long jobs, int sm_coun
     }
     static unsigned long long configured = 0;
     if (first_use_on_device(&configured) &&
-        cudaFuncSetAttribute(q4_gemm_kernel<MODE, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem) != cudaSuccess)
+        cudaFuncSetAttribute(q4_gemm_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem) != cudaSuccess)
         return -1;
     const int grid = (int)std::min<long long>(jobs * g.units_per_job, sm_count);
-    return launch_dependent(q4_gemm_kernel<MODE, T>, dim3(grid), dim3(kGemmThreads), kGemmSmem, st, maps, g) == cudaSuccess ? 1 : -1;
+    return launch_dependent(q4_gemm_kernel<MODE>, dim3(grid), dim3(kGemmThreads), kGemmSmem, st, maps, g) == cudaSuccess ? 1 : -1;
 }
 
 }  // namespace
@@ -785,9 +781,9 @@ int launch_q4_gemm(Q4Mode mode, const Q4Params &p, const void *xs, int xs_rows, 
     }
     if (!make_map_2d(&maps.x, xs, (uint64_t)xs_rows, (uint64_t)2 * g.kp, 16, false)) return -1;
     const long long jobs = mode == kProj ? (p.n + kTok - 1) / kTok : (long long)p.n * p.top_k;
-    if (mode == kProj) return launch_gemm<kProj, 2>(maps, g, jobs, sm_count, st);
-    if (mode == kGateUp) return launch_gemm<kGateUp, 2>(maps, g, jobs, sm_count, st);
-    return launch_gemm<kDown, 2>(maps, g, jobs, sm_count, st);
+    if (mode == kProj) return launch_gemm<kProj>(maps, g, jobs, sm_count, st);
+    if (mode == kGateUp) return launch_gemm<kGateUp>(maps, g, jobs, sm_count, st);
+    return launch_gemm<kDown>(maps, g, jobs, sm_count, st);
 }
 
 }  // namespace fm

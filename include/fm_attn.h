@@ -360,8 +360,8 @@ fm_status fm_moe_route(FmCtx *ctx, const FmRouteConfig *rc, int n, const float *
  * token counts twice.  x [n][hidden], expert_ids and weights [n][top_k] (top_k <= 32), residual, h_out and h_norm [n][hidden]
  * follow the pointer mode; h_out may be the residual itself, and x may be h_out or h_norm.  hidden and inter multiples of 64
  * (up to 65536), num_experts <= 1024, n up to max_batch_tokens.  Words, x, residual, h_out and h_norm 16-byte aligned, norm_w
- * 8-byte, the rest as its type.  Accuracy as for fm_proj_forward; the result does not depend on the order of the tokens or on
- * the launch.
+ * 8-byte, the rest as its type.  Accuracy as for fm_proj_forward; the same call gives the same bits, whichever order the
+ * launches' blocks take.
  * The first call of a size allocates workspace (so make it before a stream capture: FM_ERR_CAPACITY otherwise); graphs
  * captured on one context share that workspace and must not run at the same time. */
 typedef struct FmExpertWeights {

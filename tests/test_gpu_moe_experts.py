@@ -116,6 +116,29 @@ def test_one_blob_per_expert(pkg, n):
     c.close()
 
 
+@pytest.mark.parametrize("n", [2, 100])
+def test_experts_beyond_four_gigabytes(pkg, n):
+    """One blob per expert, 64 MB apart: the last of 80 lies 5 GB behind the first."""
+    rng = np.random.default_rng(90 + n)
+    c = context(pkg, max_batch=128)
+    E, hidden, inter, stride = 80, 128, 64, 64 << 20
+    few = [0, 31, 63, 64, 79]
+    m = stacks(rng, len(few), hidden, inter)
+    blob = torch.empty(E * stride, dtype=torch.uint8, device="cuda")
+    at, o = [], 0
+    for a in (a for s in m for a in s):
+        at.append(o)
+        flat = np.ascontiguousarray(a.reshape(len(few), -1)).view(np.uint8)
+        for i, e in enumerate(few):
+            blob[e * stride + o: e * stride + o + flat.shape[1]] = torch.from_numpy(flat[i]).cuda()
+        o += (flat.shape[1] + 15) // 16 * 16
+    dev = pkg.binding.FmExpertWeights(0, E, 0, hidden, inter, 64, stride, *(blob.data_ptr() + a for a in at))
+    x, res, ids, w, nw = inputs(rng, n, hidden, len(few), 3)
+    got = run(pkg, c, dev, x, np.array(few, np.int32)[ids], w, res, nw)
+    check(got, m, x, ids, w, res, nw)
+    c.close()
+
+
 def test_in_place_and_host_pointers(pkg):
     rng = np.random.default_rng(30)
     m = stacks(rng, 7, 128, 64)

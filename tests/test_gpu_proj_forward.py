@@ -112,6 +112,46 @@ def test_same_token_gives_the_same_bits_wherever_it_stands(pkg):
     c.close()
 
 
+@pytest.mark.parametrize("n", [1, 18])
+def test_a_matrix_beyond_four_gigabytes(pkg, n):
+    """Offsets past 32 bits: rows at both ends of a 4.4 GB matrix."""
+    out, k = 270000, 32768
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    w = torch.randint(-2 ** 31, 2 ** 31, (out, k // 8), generator=gen, device="cuda", dtype=torch.int32)
+    scales = (0.002 + 0.006 * torch.rand((out, k // 64), generator=gen, device="cuda")).bfloat16()
+    biases = (-7.5 * scales.float()).bfloat16()
+    x = torch.randn((n, k), generator=gen, device="cuda")
+    y = torch.empty((n, out), device="cuda")
+    c = context(pkg)
+    c.proj_forward([pkg.proj_weights(w, scales, biases)], n, x, [y])
+    c.synchronize()
+    rows = torch.tensor([0, 1, 131071, 131072, 262143, 262144, out - 2, out - 1], device="cuda")
+    m = (w[rows].cpu().numpy().view(np.uint32), scales[rows].view(torch.int16).cpu().numpy().view(np.uint16), biases[rows].view(torch.int16).cpu().numpy().view(np.uint16))
+    moe_ref.close(y[:, rows].cpu().numpy(), *moe_ref.product(x.cpu().numpy(), m))
+    c.close()
+
+
+def test_two_contexts_at_once(pkg):
+    """Contexts on streams of their own do not share anything: their calls may overlap."""
+    rng = np.random.default_rng(77)
+    m = moe_ref.weights(rng, 700, 1024)
+    work = []
+    for n in (3, 150):
+        c = context(pkg, max_batch=256)
+        st = torch.cuda.Stream()
+        c.set_stream(st.cuda_stream)
+        x = rng.standard_normal((n, 1024)).astype(np.float32)
+        work.append((c, st, x, torch.from_numpy(x).cuda(), torch.empty((n, 700), device="cuda"), on_device(pkg, m)))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for c, st, x, xd, y, d in work:
+            c.proj_forward([d], len(x), xd, [y])
+    for c, st, x, xd, y, d in work:
+        c.synchronize()
+        moe_ref.close(y.cpu().numpy(), *moe_ref.product(x, m))
+        c.close()
+
+
 def test_refusals(pkg):
     rng = np.random.default_rng(2)
     c = context(pkg, max_batch=8)
