@@ -40,7 +40,7 @@ constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kTiles = 2;        // 16-row tiles per unit
 constexpr int kTokBytes = 256;   // a token's group as bytes: 64 inputs x 4
-constexpr int kFactorBytes = 32; // per group and pair of tokens: (factor, input sum) for each of the four lanes of a quad
+constexpr int kFactorBytes = 32; // (factor, input sum) for each of the four lanes of a quad: per group and pair of tokens, or per two groups
 
 __device__ __forceinline__ void mma_u8s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -57,9 +57,10 @@ __device__ __forceinline__ void mma_u8s8_first(int (&d)[4], uint32_t a0, uint32_
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
 }
 
-// Eight inputs (those of one weight word) of a token -> fixed point bytes in the order of the B fragments.
-// The eight threads of a group of 64 inputs sit in consecutive lanes.
-__device__ __forceinline__ void widen8(const float4 &a, const float4 &b, bool valid, unsigned char *tok_group, float2 *factor, int wi) {
+// Eight inputs (those of one weight word, number wi of the group's) of a token -> fixed point bytes in the order of the B
+// fragments, digit planes kPlane bytes apart.  The eight threads of a group of 64 inputs sit in consecutive lanes.
+template <int kPlane>
+__device__ __forceinline__ void widen8(const float4 &a, const float4 &b, bool valid, unsigned char *o, float2 *factor, int wi) {
     const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
     float am = 0.f, sum = 0.f;
 #pragma unroll
@@ -86,16 +87,15 @@ __device__ __forceinline__ void widen8(const float4 &a, const float4 &b, bool va
         q[i] = ((uint32_t)k + 0x00808080u) ^ 0x00808080u;
     }
     // digit planes: plane p (0 = most significant) of the even inputs and of the odd ones
-    unsigned char *o = tok_group + (wi >> 1) * 16 + (wi & 1) * 8;
 #pragma unroll
     for (int half = 0; half < 2; half++) {
         const uint32_t a = q[half], b = q[2 + half], c = q[4 + half], d = q[6 + half];
         const uint32_t ab_hi = __byte_perm(a, b, 0x7362), cd_hi = __byte_perm(c, d, 0x7362);  // a2 b2 a3 b3
         const uint32_t ab_lo = __byte_perm(a, b, 0x5140), cd_lo = __byte_perm(c, d, 0x5140);  // a0 b0 a1 b1
-        *reinterpret_cast<uint32_t *>(o + 0 * 64 + half * 4) = __byte_perm(ab_hi, cd_hi, 0x7632);  // a3 b3 c3 d3
-        *reinterpret_cast<uint32_t *>(o + 1 * 64 + half * 4) = __byte_perm(ab_hi, cd_hi, 0x5410);  // a2 b2 c2 d2
-        *reinterpret_cast<uint32_t *>(o + 2 * 64 + half * 4) = __byte_perm(ab_lo, cd_lo, 0x7632);  // a1 b1 c1 d1
-        *reinterpret_cast<uint32_t *>(o + 3 * 64 + half * 4) = __byte_perm(ab_lo, cd_lo, 0x5410);  // a0 b0 c0 d0
+        *reinterpret_cast<uint32_t *>(o + 0 * kPlane + half * 4) = __byte_perm(ab_hi, cd_hi, 0x7632);  // a3 b3 c3 d3
+        *reinterpret_cast<uint32_t *>(o + 1 * kPlane + half * 4) = __byte_perm(ab_hi, cd_hi, 0x5410);  // a2 b2 c2 d2
+        *reinterpret_cast<uint32_t *>(o + 2 * kPlane + half * 4) = __byte_perm(ab_lo, cd_lo, 0x7632);  // a1 b1 c1 d1
+        *reinterpret_cast<uint32_t *>(o + 3 * kPlane + half * 4) = __byte_perm(ab_lo, cd_lo, 0x5410);  // a0 b0 c0 d0
     }
     // the pair of upper digits counts 2^16, the pair of lower ones 1; the input sum goes with either (see the loop)
     if (wi < 2) factor[wi] = make_float2(wi == 0 ? down * 65536.f : down, sum);
@@ -104,8 +104,15 @@ __device__ __forceinline__ void widen8(const float4 &a, const float4 &b, bool va
 constexpr int S = 4;             // groups per step
 // A step of a row pair as a lane holds it: 8 bytes of words per group and row, the scales of rows g and g + 8, and the bias of
 // row g (even lanes) or g + 8 (odd lanes).
+template <bool ONE>
 struct Held {
     uint2 w[kTiles][2][S];
+    uint2 sc[kTiles][2], bi[kTiles];
+};
+// One token: 16 bytes of words per two groups and row.  Lanes 0 and 1 of a quad hold the first group, 2 and 3 the second.
+template <>
+struct Held<true> {
+    uint4 w[kTiles][2][S / 2];
     uint2 sc[kTiles][2], bi[kTiles];
 };
 // The bf16 numbers of a step's groups: in one read where a row of them is a multiple of 8 bytes, 8-byte aligned; else one by
@@ -125,19 +132,22 @@ __device__ __forceinline__ float bf16_at(uint2 four, int j) {
     const uint32_t pair = j & 2 ? four.y : four.x;
     return __uint_as_float(j & 1 ? pair & 0xffff0000u : pair << 16);
 }
+// of two groups' bf16 numbers that of the lane's (up: 16 for the first group, 0 for the second)
+__device__ __forceinline__ float bf16_of(uint32_t pair, int up) { return __uint_as_float((pair << up) & 0xffff0000u); }
 // The same value in every lane, and known to the compiler as such (values of at least 0).
 __device__ __forceinline__ int uniform(int v) { return __reduce_max_sync(0xffffffffu, v); }
 
 // Warps: WK of them side by side along a row's steps, 8 / WK along the rows.
 template <Q4Mode MODE, int NTL, bool WIDE>
 __global__ void __launch_bounds__(kThreads, NTL == 4 ? 1 : 2)
-q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units_per_job, int fixed_jobs, int wk_log2) {
+q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units_per_job, int fixed_jobs, int wk_log2, int sms) {
     extern __shared__ __align__(16) unsigned char smem[];
-    constexpr int kTok = 2 * NTL;
+    constexpr bool ONE = NTL == 0;
+    constexpr int kTok = ONE ? 1 : 2 * NTL, NT = ONE ? 1 : NTL;
     constexpr int kAhead = NTL == 4 ? 4 : 1;  // words of activations a thread has under way: as many as fit beside the weights' registers
-    unsigned char *s_b = smem;                                                                      // [NTL][2 tokens][chunk][256]
-    float2 *s_f = reinterpret_cast<float2 *>(smem + (size_t)kTok * chunk_groups * kTokBytes);       // [NTL][chunk][4]
-    float *s_red = reinterpret_cast<float *>(reinterpret_cast<unsigned char *>(s_f) + (size_t)NTL * chunk_groups * kFactorBytes);  // [2][warp][tok][32 rows]
+    unsigned char *s_b = smem;                                                                      // [tokens][chunk][256]
+    float2 *s_f = reinterpret_cast<float2 *>(smem + (size_t)kTok * chunk_groups * kTokBytes);       // [NT][chunk][4], or [chunk / 2][4]
+    float *s_red = reinterpret_cast<float *>(reinterpret_cast<unsigned char *>(s_f) + (size_t)NT * chunk_groups * kFactorBytes);  // [2][warp][tok][32 rows]
     const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int WK = 1 << wk_log2, wk = warp & (WK - 1), wr = warp >> wk_log2, rows_unit = (MODE == kGateUp ? 16 : 32) * (kWarps >> wk_log2);
     const int G = p.in_dim / 64;
@@ -149,7 +159,9 @@ q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     const int njobs = p.plan.njobs != nullptr ? uniform(*p.plan.njobs) : fixed_jobs;
     const long long units = (long long)njobs * units_per_job;
-    const long long u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1) / gridDim.x;
+    // Ranges differ by a unit; those of the CTAs that share an SM (b, b + sms) are neighbours, so that no SM gets the longer ones only.
+    const int range = gridDim.x % sms == 0 ? (int)(blockIdx.x % sms * (gridDim.x / sms) + blockIdx.x / sms) : (int)blockIdx.x;
+    const long long u0 = units * range / gridDim.x, u1 = units * (range + 1) / gridDim.x;
 
     struct Unit {
         int job, expert, start, cnt, mat, row0;
@@ -169,7 +181,7 @@ q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units
         }
     };
 
-    Held h;
+    Held<ONE> h;
     // where the lane's rows start: offsets of rows g and g + 8 of each tile (rows without a place read the last one there is)
     const unsigned char *bw[kTiles], *bs[kTiles], *bb[kTiles];
     uint32_t ow[kTiles][2], os[kTiles][2], ob[kTiles];
@@ -194,7 +206,7 @@ q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units
             bs[i] = m.scales + (size_t)un.expert * m.s_stride + (size_t)first * s_pitch;
             bb[i] = m.biases + (size_t)un.expert * m.s_stride + (size_t)first * s_pitch;
             const uint32_t l0 = min(g, last), l1 = min(g + 8, last);
-            ow[i][0] = l0 * w_pitch + t * 8; ow[i][1] = l1 * w_pitch + t * 8;
+            ow[i][0] = l0 * w_pitch + t * (ONE ? 16 : 8); ow[i][1] = l1 * w_pitch + t * (ONE ? 16 : 8);
             os[i][0] = l0 * s_pitch; os[i][1] = l1 * s_pitch;
             ob[i] = t & 1 ? os[i][1] : os[i][0];
         }
@@ -208,11 +220,19 @@ q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units
             for (int q = 0; q < 2; q++) pw[i][q] = bw[i] + (ow[i][q] + (uint32_t)step * (S * 32u));
         if constexpr (!WIDE) left = G - step * S;
     };
-    auto fetch_words = [&](int j) {  // group j of the step (behind the row's end: its last group again)
+    auto fetch_words = [&](int j) {  // group j of the step; ONE: groups 2 j and 2 j + 1 (behind the row's end: its last group again)
+        if constexpr (ONE) {
+            const int at = WIDE ? j * 64 : j * 64 - 32 * max(0, 2 * j + (t >> 1) - (left - 1));
 #pragma unroll
-        for (int i = 0; i < kTiles; i++)
+            for (int i = 0; i < kTiles; i++)
 #pragma unroll
-            for (int q = 0; q < 2; q++) h.w[i][q][j] = __ldg(reinterpret_cast<const uint2 *>(pw[i][q] + (WIDE ? j : min(j, left - 1)) * 32));
+                for (int q = 0; q < 2; q++) h.w[i][q][j] = __ldg(reinterpret_cast<const uint4 *>(pw[i][q] + at));
+        } else {
+#pragma unroll
+            for (int i = 0; i < kTiles; i++)
+#pragma unroll
+                for (int q = 0; q < 2; q++) h.w[i][q][j] = __ldg(reinterpret_cast<const uint2 *>(pw[i][q] + (WIDE ? j : min(j, left - 1)) * 32));
+        }
     };
     auto fetch_scales = [&](int step) {
 #pragma unroll
@@ -254,7 +274,7 @@ q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units
     auto fetch_first = [&]() {
         point(wk);
 #pragma unroll
-        for (int j = 0; j < S; j++) fetch_words(j);
+        for (int j = 0; j < (ONE ? S / 2 : S); j++) fetch_words(j);
         fetch_scales(wk);
     };
     const bool has_first = wk < (min(chunk_groups, G) + S - 1) / S;  // this warp has a step in a unit's first chunk
@@ -263,10 +283,14 @@ q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units
         if (has_first) fetch_first();
     }
     if constexpr (MODE == kDown) asm volatile("griddepcontrol.wait;\n" ::: "memory");
-    const unsigned char *lane_b = s_b + (size_t)(g >> 2) * chunk_groups * kTokBytes + ((g & 3) * 4 + t) * 16;
+    // B fragments: two tokens -- column g is digit g & 3 of token g / 4 of the pair.  One token: column g is digit g & 3 of group g / 4
+    // of two, and only the lanes that hold that group's words have anything in it; so a row is read 64 bytes at a time.
+    const bool mine = (g >> 2) == (t >> 1);
+    const int up = t < 2 ? 16 : 0;  // bf16_of: which of two scales is the lane's
+    const unsigned char *lane_b = ONE ? s_b + (t * 4 + (g & 3)) * 32 : s_b + (size_t)(g >> 2) * chunk_groups * kTokBytes + ((g & 3) * 4 + t) * 16;
     while (u < u1) {
         const int ntl = (un.cnt + 1) / 2;
-        float acc[kTiles][2][NTL] = {}, accb[kTiles][NTL] = {};
+        float acc[kTiles][2][NT] = {}, accb[kTiles][NT] = {};
         Unit nx = un;
         long long v = u;
         for (int c = 0; c < nchunks; c++) {
@@ -298,14 +322,21 @@ q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units
                     }
 #pragma unroll
                     for (int k = 0; k < kAhead; k++) {
-                        unsigned char *tb = s_b + ((size_t)who[k] * chunk_groups + (at[k] >> 3)) * kTokBytes;
-                        float2 *f = s_f + ((size_t)(who[k] >> 1) * chunk_groups + (at[k] >> 3)) * 4 + (who[k] & 1) * 2;
-                        widen8(xa[k], xb[k], who[k] < un.cnt, tb, f, at[k] & 7);
+                        const int grp = at[k] >> 3, wi = at[k] & 7;
+                        if constexpr (ONE) {  // two groups' sixteen words in fours, a lane of the quad each
+                            const int w = (grp & 1) * 8 + wi;
+                            widen8<32>(xa[k], xb[k], who[k] < un.cnt, s_b + (size_t)(grp >> 1) * 2 * kTokBytes + (w >> 2) * 128 + (w & 3) * 8, s_f + (size_t)grp * 2, wi);
+                        } else {
+                            widen8<64>(xa[k], xb[k], who[k] < un.cnt, s_b + ((size_t)who[k] * chunk_groups + grp) * kTokBytes + (wi >> 1) * 16 + (wi & 1) * 8,
+                                       s_f + ((size_t)(who[k] >> 1) * chunk_groups + grp) * 4 + (who[k] & 1) * 2, wi);
+                        }
                     }
                 }
-                for (int i = tid; i < NTL * 4 * (steps * S - cgn); i += kThreads) {  // the last step's groups behind the row's end
-                    const int nt = i / (4 * (steps * S - cgn)), q = i - nt * 4 * (steps * S - cgn);
-                    s_f[((size_t)nt * chunk_groups + cgn) * 4 + q] = make_float2(0.f, 0.f);
+                // the last step's groups behind the row's end count nothing
+                constexpr int kPer = ONE ? 2 : 4;  // factors of a group
+                for (int i = tid; i < NT * kPer * (steps * S - cgn); i += kThreads) {
+                    const int nt = i / (kPer * (steps * S - cgn)), q = i - nt * kPer * (steps * S - cgn);
+                    s_f[((size_t)nt * chunk_groups + cgn) * kPer + q] = make_float2(0.f, 0.f);
                 }
                 held_start = source; held_job = kind;
                 __syncthreads();
@@ -330,33 +361,69 @@ q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units
                 for (int i = 0; i < kTiles; i++) { sc[i][0] = h.sc[i][0]; sc[i][1] = h.sc[i][1]; bi[i] = h.bi[i]; }
                 if (more >= 0) { fetch_scales(more); point(more); }
                 const unsigned char *fb = lane_b + (size_t)st * S * kTokBytes;
-                const float2 *ff = s_f + (size_t)st * S * 4 + t;
+                const float2 *ff = s_f + (size_t)st * S * (ONE ? 2 : 4) + t;
+                if constexpr (ONE) {
 #pragma unroll
-                for (int j = 0; j < S; j++) {
-                    uint32_t a[kTiles][2][4];  // nibbles as bytes: [tile][word of the lane's two][fragment register]
+                    for (int b = 0; b < S / 2; b++) {
+                        uint4 b01 = make_uint4(0, 0, 0, 0), b23 = b01;
+                        if (mine) {
+                            const uint4 *src = reinterpret_cast<const uint4 *>(fb + b * 2 * kTokBytes);
+                            b01 = src[0]; b23 = src[1];
+                        }
+                        const float2 f = ff[b * 4];
+                        uint32_t a[kTiles][4][4];  // nibbles as bytes: [tile][word of the lane's four][fragment register]
 #pragma unroll
-                    for (int i = 0; i < kTiles; i++) {
-                        const uint2 w0 = h.w[i][0][j], w1 = h.w[i][1][j];
-                        a[i][0][0] = w0.x & 0x0F0F0F0Fu; a[i][0][1] = w1.x & 0x0F0F0F0Fu;
-                        a[i][0][2] = (w0.x >> 4) & 0x0F0F0F0Fu; a[i][0][3] = (w1.x >> 4) & 0x0F0F0F0Fu;
-                        a[i][1][0] = w0.y & 0x0F0F0F0Fu; a[i][1][1] = w1.y & 0x0F0F0F0Fu;
-                        a[i][1][2] = (w0.y >> 4) & 0x0F0F0F0Fu; a[i][1][3] = (w1.y >> 4) & 0x0F0F0F0Fu;
-                    }
-                    if (more >= 0) fetch_words(j);
+                        for (int i = 0; i < kTiles; i++) {
+                            const uint4 w0 = h.w[i][0][b], w1 = h.w[i][1][b];
+                            const uint32_t r0[4] = {w0.x, w0.y, w0.z, w0.w}, r1[4] = {w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
-                    for (int nt = 0; nt < NTL; nt++) {
-                        if (nt >= ntl) break;
-                        const uint4 bf = *reinterpret_cast<const uint4 *>(fb + (size_t)nt * 2 * chunk_groups * kTokBytes + j * kTokBytes);
-                        const float2 f = ff[(size_t)nt * chunk_groups * 4 + j * 4];
+                            for (int w = 0; w < 4; w++) {
+                                a[i][w][0] = r0[w] & 0x0F0F0F0Fu; a[i][w][1] = r1[w] & 0x0F0F0F0Fu;
+                                a[i][w][2] = (r0[w] >> 4) & 0x0F0F0F0Fu; a[i][w][3] = (r1[w] >> 4) & 0x0F0F0F0Fu;
+                            }
+                        }
+                        if (more >= 0) fetch_words(b);
 #pragma unroll
                         for (int i = 0; i < kTiles; i++) {
                             int d[4];
-                            mma_u8s8_first(d, a[i][0][0], a[i][0][1], a[i][0][2], a[i][0][3], bf.x, bf.y);
-                            mma_u8s8(d, a[i][1][0], a[i][1][1], a[i][1][2], a[i][1][3], bf.z, bf.w);
-                            // |d| <= 64 * 15 * 128, so two digits still fit an int; lane t holds the digit pair t & 1 of token t / 2
-                            acc[i][0][nt] = fmaf(bf16_at(sc[i][0], j) * f.x, (float)(d[0] * 256 + d[1]), acc[i][0][nt]);
-                            acc[i][1][nt] = fmaf(bf16_at(sc[i][1], j) * f.x, (float)(d[2] * 256 + d[3]), acc[i][1][nt]);
-                            accb[i][nt] = fmaf(bf16_at(bi[i], j), f.y, accb[i][nt]);
+                            mma_u8s8_first(d, a[i][0][0], a[i][0][1], a[i][0][2], a[i][0][3], b01.x, b01.y);
+                            mma_u8s8(d, a[i][1][0], a[i][1][1], a[i][1][2], a[i][1][3], b01.z, b01.w);
+                            mma_u8s8(d, a[i][2][0], a[i][2][1], a[i][2][2], a[i][2][3], b23.x, b23.y);
+                            mma_u8s8(d, a[i][3][0], a[i][3][1], a[i][3][2], a[i][3][3], b23.z, b23.w);
+                            // |d| <= 64 * 15 * 128, so two digits still fit an int; lane t holds the digit pair t & 1 of group t / 2
+                            acc[i][0][0] = fmaf(bf16_of(b ? sc[i][0].y : sc[i][0].x, up) * f.x, (float)(d[0] * 256 + d[1]), acc[i][0][0]);
+                            acc[i][1][0] = fmaf(bf16_of(b ? sc[i][1].y : sc[i][1].x, up) * f.x, (float)(d[2] * 256 + d[3]), acc[i][1][0]);
+                            accb[i][0] = fmaf(bf16_of(b ? bi[i].y : bi[i].x, up), f.y, accb[i][0]);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < S; j++) {
+                        uint32_t a[kTiles][2][4];  // nibbles as bytes: [tile][word of the lane's two][fragment register]
+#pragma unroll
+                        for (int i = 0; i < kTiles; i++) {
+                            const uint2 w0 = h.w[i][0][j], w1 = h.w[i][1][j];
+                            a[i][0][0] = w0.x & 0x0F0F0F0Fu; a[i][0][1] = w1.x & 0x0F0F0F0Fu;
+                            a[i][0][2] = (w0.x >> 4) & 0x0F0F0F0Fu; a[i][0][3] = (w1.x >> 4) & 0x0F0F0F0Fu;
+                            a[i][1][0] = w0.y & 0x0F0F0F0Fu; a[i][1][1] = w1.y & 0x0F0F0F0Fu;
+                            a[i][1][2] = (w0.y >> 4) & 0x0F0F0F0Fu; a[i][1][3] = (w1.y >> 4) & 0x0F0F0F0Fu;
+                        }
+                        if (more >= 0) fetch_words(j);
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) {
+                            if (nt >= ntl) break;
+                            const uint4 bf = *reinterpret_cast<const uint4 *>(fb + (size_t)nt * 2 * chunk_groups * kTokBytes + j * kTokBytes);
+                            const float2 f = ff[(size_t)nt * chunk_groups * 4 + j * 4];
+#pragma unroll
+                            for (int i = 0; i < kTiles; i++) {
+                                int d[4];
+                                mma_u8s8_first(d, a[i][0][0], a[i][0][1], a[i][0][2], a[i][0][3], bf.x, bf.y);
+                                mma_u8s8(d, a[i][1][0], a[i][1][1], a[i][1][2], a[i][1][3], bf.z, bf.w);
+                                // |d| <= 64 * 15 * 128, so two digits still fit an int; lane t holds the digit pair t & 1 of token t / 2
+                                acc[i][0][nt] = fmaf(bf16_at(sc[i][0], j) * f.x, (float)(d[0] * 256 + d[1]), acc[i][0][nt]);
+                                acc[i][1][nt] = fmaf(bf16_at(sc[i][1], j) * f.x, (float)(d[2] * 256 + d[3]), acc[i][1][nt]);
+                                accb[i][nt] = fmaf(bf16_at(bi[i], j), f.y, accb[i][nt]);
+                            }
                         }
                     }
                 }
@@ -375,11 +442,17 @@ q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units
 #pragma unroll
         for (int i = 0; i < kTiles; i++)
 #pragma unroll
-            for (int nt = 0; nt < NTL; nt++) {
+            for (int nt = 0; nt < NT; nt++) {
                 float v0 = acc[i][0][nt] + (t & 1 ? 0.f : accb[i][nt]), v1 = acc[i][1][nt] + (t & 1 ? accb[i][nt] : 0.f);
                 v0 += __shfl_xor_sync(0xffffffffu, v0, 1);
                 v1 += __shfl_xor_sync(0xffffffffu, v1, 1);
-                red[((size_t)warp * kTok + nt * 2 + (t >> 1)) * 32 + i * 16 + g + (t & 1) * 8] = t & 1 ? v1 : v0;
+                if constexpr (ONE) {  // and the two groups
+                    v0 += __shfl_xor_sync(0xffffffffu, v0, 2);
+                    v1 += __shfl_xor_sync(0xffffffffu, v1, 2);
+                    if (t < 2) red[(size_t)warp * 32 + i * 16 + g + t * 8] = t ? v1 : v0;
+                } else {
+                    red[((size_t)warp * kTok + nt * 2 + (t >> 1)) * 32 + i * 16 + g + (t & 1) * 8] = t & 1 ? v1 : v0;
+                }
             }
         __syncthreads();  // (the other half of s_red is free again once everyone is here)
         for (int e = warp; e < un.cnt * (kWarps >> wk_log2); e += kWarps) {  // 32 rows of one token per warp
@@ -402,7 +475,8 @@ q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units
 constexpr int kMaxSmem = 200 * 1024;
 
 size_t smem_bytes(int ntl, int chunk) {
-    return (size_t)2 * ntl * chunk * kTokBytes + (size_t)ntl * chunk * kFactorBytes + (size_t)2 * kWarps * 2 * ntl * 32 * 4;
+    const int tokens = ntl == 0 ? 1 : 2 * ntl;
+    return (size_t)tokens * chunk * kTokBytes + (size_t)std::max(1, ntl) * chunk * kFactorBytes + (size_t)2 * kWarps * tokens * 32 * 4;
 }
 
 template <Q4Mode MODE, int NTL, bool WIDE>
@@ -416,20 +490,21 @@ int launch_one(const Q4Params &p, int jobs, int sm_count, cudaStream_t st) {
         cudaFuncSetAttribute(q4_stream_kernel<MODE, NTL, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem) != cudaSuccess)
         return -1;
     const int grid_max = sm_count * std::max(1, std::min(NTL == 4 ? 1 : 2, (int)((220 * 1024) / (smem + 1024))));
-    // Warps along a row, the others side by side on more rows.  A unit costs its steps and an end worth about 1 1/3 of a step of
-    // two tokens (the warps meet, the next unit's addresses); a CTA takes whole units: the cheapest split.
+    // Warps along a row, the others side by side on more rows.  An SM's time is its units' steps, plus a unit's end worth about
+    // 0.6 of a step (the warps meet, the next unit's addresses), and it takes whole units: the cheapest split.  (One token x 4096
+    // x 20480: 8, 4, 2 warps along a row take 16.7, 18.3 and 20.2 us; x 18944, where the last two come out even, 13.0, 12.7, 12.6.)
     int wk_log2 = 0, per_job = 0;
     double best = 0.0;
     for (int k = 0; k <= 3; k++) {
         const int rows = (MODE == kGateUp ? 16 : 32) * (kWarps >> k);
         int n = 0;
         for (int i = 0; i < (MODE == kGateUp ? 1 : p.nmat); i++) n += (p.mat[i].rows + rows - 1) / rows;
-        const long long waves = ((long long)jobs * n + grid_max - 1) / grid_max;
-        const double cost = (double)waves * ((double)(((G + S - 1) / S + (1 << k) - 1) >> k) + 2.66 / (1 + NTL));
+        const long long most = ((long long)jobs * n + sm_count - 1) / sm_count;
+        const double cost = (double)most * ((double)(((G + S - 1) / S + (1 << k) - 1) >> k) + 0.6);
         if (k == 0 || cost < best) { best = cost; wk_log2 = k; per_job = n; }
     }
     const int grid = (int)std::min<long long>((long long)jobs * per_job, grid_max);
-    return launch_dependent(q4_stream_kernel<MODE, NTL, WIDE>, dim3(grid), dim3(kThreads), smem, st, p, chunk, per_job, jobs, wk_log2) == cudaSuccess ? 1 : -1;
+    return launch_dependent(q4_stream_kernel<MODE, NTL, WIDE>, dim3(grid), dim3(kThreads), smem, st, p, chunk, per_job, jobs, wk_log2, sm_count) == cudaSuccess ? 1 : -1;
 }
 
 template <Q4Mode MODE, int NTL>
@@ -445,12 +520,13 @@ int launch_steps(const Q4Params &p, int jobs, int sm_count, cudaStream_t st) {
 int launch_q4_stream(Q4Mode mode, const Q4Params &p, int sm_count, cudaStream_t st) {
     if (mode == kProj) {
         // tokens per pass over the weights: as many as there are, up to 8; more take more passes, which find the weights in L2
-        if (p.n <= 2) return launch_steps<kProj, 1>(p, 1, sm_count, st);
+        if (p.n == 1) return launch_steps<kProj, 0>(p, 1, sm_count, st);
+        if (p.n == 2) return launch_steps<kProj, 1>(p, 1, sm_count, st);
         if (p.n <= 4) return launch_steps<kProj, 2>(p, 1, sm_count, st);
         return launch_steps<kProj, 4>(p, (p.n + 7) / 8, sm_count, st);
     }
     const int pairs = p.n * p.top_k;  // an upper bound of the jobs; with a plan the device knows how many there are
-    if (p.plan.njobs == nullptr) return mode == kGateUp ? launch_steps<kGateUp, 1>(p, pairs, sm_count, st) : launch_steps<kDown, 1>(p, pairs, sm_count, st);
+    if (p.plan.njobs == nullptr) return mode == kGateUp ? launch_steps<kGateUp, 0>(p, pairs, sm_count, st) : launch_steps<kDown, 0>(p, pairs, sm_count, st);
     return mode == kGateUp ? launch_steps<kGateUp, 2>(p, pairs, sm_count, st) : launch_steps<kDown, 2>(p, pairs, sm_count, st);
 }
 
