@@ -6,25 +6,26 @@
 // down chain of the same file.
 //     y[r] = sum over groups g of 64 inputs:  s[r][g] * sum_k nibble[r][k] x[k]  +  b[r][g] * X[g],   X[g] = sum_k x[k]
 //
-// Bound by the weights' stream, 0.5625 bytes per weight, and close behind it by the instructions that widen them.  So
-// the nibbles are never turned into floating point: they are multiplied as they are, unsigned bytes, on the integer
+// The weights' stream, 0.5625 bytes per weight, is what it cannot do without; next to it stand the instructions that widen
+// them.  So the nibbles are never turned into floating point: they are multiplied as they are, unsigned bytes, on the integer
 // tensor cores (mma.sync m16n8k32, measured at twice the fp16 rate), which takes 3 instructions per word of eight.  The
 // activations are the other factor, as 32-bit fixed point relative to the largest of their group of 64, cut into four
-// signed bytes, which are four of the eight columns of the product: two tokens per instruction.  The integer sums are
-// exact; what is left of fp32's accuracy is 2^-30 of a group's largest input.  Scale and bias meet the group's sum in
-// fp32, once per row and group.
+// signed bytes, which are four of the eight columns of the product.  The other four are a second token; or, for one token,
+// a second group, so that a row is read 64 bytes at a time and not 32.  The integer sums are exact; what is left of fp32's
+// accuracy is 2^-30 of a group's largest input.  Scale and bias meet the group's sum in fp32, once per row and group.
 //
-// A unit is 32 rows per warp that stands alone along the row (kGateUp: 16 of gate and the same 16 of up) for one job.  The 8
-// warps of a CTA split the steps of a row (four groups each) and the unit's rows among themselves, by a cost rule in
-// launch_one, and meet in shared memory at the unit's end; a lane fetches 8 bytes of a row group straight into registers, and
-// refills them as it unpacks them, so that about 60 KB per SM are under way.  CTAs are persistent and take a contiguous range
-// of units, so that a job's activations are widened once per CTA and not once per unit, and the next unit's weights are
-// fetched while this one's sums meet.
+// A unit is 32 rows (kGateUp: 16 of gate and the same 16 of up) per warp along the rows, for one job.  The 8 warps of a CTA
+// split the steps of a row (four groups each) and the unit's rows among themselves, by a cost rule in launch_one, and meet in
+// shared memory at the unit's end; a lane fetches its words straight into registers, and refills them as it unpacks them, so
+// that about 60 KB per SM are under way.  CTAs are persistent and take a contiguous range of units, so that a job's
+// activations are widened once per CTA and not once per unit, and the next unit's weights are fetched while this one's sums
+// meet.
 //
-// Measured (B200, weights from HBM): one token x 4096 x 17408 in 12.6 us (40 MB: 3.2 TB/s; 5.3 TB/s in the long run, 4.5 us go
-// into the start and the end), x 8192 x 4096 in 9.5 us; one token through 10 of 512 experts of 4096 x 1024 in 35 us with the
-// weighted sum; 48 tokens through them (2.2 GB) in 450 us, 4.9 TB/s.  Bound by issue slots next to the stream: 31 instructions
-// per 16 rows x 64 inputs, of which the unpacking takes 12.
+// Measured (B200): one token x 4096 x 17408 in 11.2 us (40 MB: 3.6 TB/s; 5.3 TB/s in the long run, 4.5 us go into the start and
+// the end), x 8192 x 4096 in 9 us; one token through 10 of 512 experts of 4096 x 1024 in 29 us with the weighted sum; 48 tokens
+// through them (2.2 GB) in 450 us, 4.9 TB/s.  In the long run it is bound by the L1 cache's wavefronts (72 % of their peak): a
+// request of a warp touches 8 rows, 64 or 32 bytes of each, and the scales and biases cost as many as the words.
+// One token in the two-token form: 12.5 and 35 us; the one-token form for 3 or more tokens takes 1.3 to 1.8 times as long.
 #include <math.h>
 
 #include <algorithm>
