@@ -162,18 +162,48 @@ __device__ __forceinline__ int tile_mat(const Unit &u, int tile) {
     return MODE == kGateUp ? tile & 1 : u.mat;
 }
 
-// The four scales of a row's chunk as bf16 bits (zero beyond the last group).
-__device__ __forceinline__ uint2 chunk_scales(const unsigned char *row, int c, int G, bool wide) {
-    uint2 v = make_uint2(0, 0);
-    if (wide) {  // volatile: the load stays where it is written, a step ahead of its use
-        asm volatile("ld.global.nc.v2.u32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "l"(reinterpret_cast<const uint2 *>(row) + c));
-        return v;
-    }
-    const uint16_t *s = reinterpret_cast<const uint16_t *>(row) + c * kChunk;
-    const int left = G - c * kChunk;
-    v.x = (uint32_t)__ldg(s) | (left > 1 ? (uint32_t)__ldg(s + 1) << 16 : 0u);
-    v.y = (left > 2 ? (uint32_t)__ldg(s + 2) : 0u) | (left > 3 ? (uint32_t)__ldg(s + 3) << 16 : 0u);
+// The four scales of a row's chunk as bf16 bits, where scales are wide.  Volatile: the load stays where it is written, a step
+// ahead of its use.
+__device__ __forceinline__ uint2 chunk_scales(const unsigned char *row, int c) {
+    uint2 v;
+    asm volatile("ld.global.nc.v2.u32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "l"(reinterpret_cast<const uint2 *>(row) + c));
     return v;
+}
+// Where they are not, a row begins at any even address.  It is read in aligned windows, each once, and its pieces are cut out
+// of two of them.  Read 2 bytes at a time (a sector of 32 per load and row, next to no L1 beside the tiles) 4160 inputs took
+// 2.4 times as long as 4096 (4096 rows, 20 tokens: 89 and 36 us), so they take 49.  A window that reaches beyond the matrix is
+// read by the 2 bytes that belong to it.
+struct Bytes { const unsigned char *begin, *end; };
+__device__ __forceinline__ uint2 window8(const unsigned char *at, Bytes m) {
+    uint2 v = make_uint2(0, 0);
+    if (at >= m.begin && at + 8 <= m.end) return chunk_scales(at, 0);
+    const uint16_t *h = reinterpret_cast<const uint16_t *>(at);
+    const uint16_t *lo = reinterpret_cast<const uint16_t *>(m.begin), *hi = reinterpret_cast<const uint16_t *>(m.end);
+    if (h >= lo && h < hi) v.x = __ldg(h);
+    if (h + 1 >= lo && h + 1 < hi) v.x |= (uint32_t)__ldg(h + 1) << 16;
+    if (h + 2 >= lo && h + 2 < hi) v.y = __ldg(h + 2);
+    if (h + 3 >= lo && h + 3 < hi) v.y |= (uint32_t)__ldg(h + 3) << 16;
+    return v;
+}
+// Eight bytes from `by` (0, 2, 4 or 6) bytes into two windows, of which the first `left` halves are kept.
+__device__ __forceinline__ uint2 cut8(uint2 a, uint2 b, uint32_t by, int left) {
+    const uint32_t w0 = by & 4 ? a.y : a.x, w1 = by & 4 ? b.x : a.y, w2 = by & 4 ? b.y : b.x, s = (by & 2) * 8;
+    uint2 v = make_uint2(__funnelshift_r(w0, w1, s), __funnelshift_r(w1, w2, s));
+    if (left < 4) v.y &= left < 3 ? 0u : 0xffffu;
+    if (left < 2) v.x &= 0xffffu;
+    return v;
+}
+__device__ __forceinline__ uint4 window16(const unsigned char *at) {
+    uint4 v;
+    asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(at));
+    return v;
+}
+// The same of 16-byte windows.
+__device__ __forceinline__ uint4 cut16(uint4 a, uint4 b, uint32_t by) {
+    const bool p = by & 8, q = by & 4;
+    const uint32_t t0 = p ? a.z : a.x, t1 = p ? a.w : a.y, t2 = p ? b.x : a.z, t3 = p ? b.y : a.w, t4 = p ? b.z : b.x, t5 = p ? b.w : b.y;
+    const uint32_t w0 = q ? t1 : t0, w1 = q ? t2 : t1, w2 = q ? t3 : t2, w3 = q ? t4 : t3, w4 = q ? t5 : t4, s = (by & 2) * 8;
+    return make_uint4(__funnelshift_r(w0, w1, s), __funnelshift_r(w1, w2, s), __funnelshift_r(w2, w3, s), __funnelshift_r(w3, w4, s));
 }
 // Exponent field of the largest of them, kept where the powers of two made of it are normal numbers.
 __device__ __forceinline__ int chunk_exponent(uint2 v) {
@@ -289,6 +319,12 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
         const int first = tile_row<MODE>(u, tile);
         const unsigned char *tile0 = (biases ? m.biases : m.scales) + (size_t)u.expert * m.s_stride + (size_t)first * s_pitch;  // uniform
         return tile0 + (uint32_t)min(r, m.rows - 1 - first) * (uint32_t)s_pitch;
+    };
+
+    auto matrix_bytes = [&](const Unit &u, int tile, bool biases) {
+        const Q4View &m = g.p.mat[tile_mat<MODE>(u, tile)];
+        const unsigned char *first = (biases ? m.biases : m.scales) + (size_t)u.expert * m.s_stride;
+        return Bytes{first, first + (size_t)m.rows * s_pitch};
     };
 
     if (warp == 16) {
@@ -452,12 +488,18 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
         };
         // scales of the next chunk, a tile's row each: fetched a chunk ahead, those of a unit's first one before the bias block
         const unsigned char *sp[T];
-        uint2 sc[T];
+        uint2 sc[T], sd[T];  // (not wide: two windows that hold the scales)
+        auto window = [&](const Unit &un, int i, int c) { return window8((const unsigned char *)((uintptr_t)sp[i] & ~(uintptr_t)7) + 8 * c, matrix_bytes(un, i, false)); };
         auto aim = [&](const Unit &un) {
 #pragma unroll
             for (int i = 0; i < T; i++) {
-                sp[i] = row_ptr(un, i < un.tiles ? i : 0, r, false);
-                sc[i] = chunk_scales(sp[i], 0, G, g.wide);
+                const int t = i < un.tiles ? i : 0;
+                sp[i] = row_ptr(un, t, r, false);
+                if (g.wide) sc[i] = chunk_scales(sp[i], 0);
+                else {
+                    sc[i] = window(un, t, 0);
+                    sd[i] = window(un, t, 1);
+                }
             }
         };
         Unit un;
@@ -471,10 +513,19 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
                 const int na = min(kChunk, G - c * kChunk);
 #pragma unroll 1  // (one copy of the loop's body: the four roles' code has to fit the instruction cache)
                 for (int i = 0; i < un.tiles && ok; i++) {
-                    const uint2 s = i ? sc[1] : sc[0];
+                    uint2 s = i ? sc[1] : sc[0];
+                    if (!g.wide) s = cut8(s, i ? sd[1] : sd[0], (uint32_t)(uintptr_t)(i ? sp[1] : sp[0]) & 7u, na);
                     if (c + 1 < nreal) {  // (in place: a copy of the result would wait for it)
-                        if (i) sc[1] = chunk_scales(sp[1], c + 1, G, g.wide);
-                        else sc[0] = chunk_scales(sp[0], c + 1, G, g.wide);
+                        if (g.wide) {
+                            if (i) sc[1] = chunk_scales(sp[1], c + 1);
+                            else sc[0] = chunk_scales(sp[0], c + 1);
+                        } else if (i) {
+                            sc[1] = sd[1];
+                            sd[1] = window(un, 1, c + 2);
+                        } else {
+                            sc[0] = sd[0];
+                            sd[0] = window(un, 0, c + 2);
+                        }
                     }
                     const int e = chunk_exponent(s);
                     const float up = pow2(127 + 141 - e);  // the largest scale comes to [2^14, 2^15)
@@ -543,10 +594,37 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
                             }
                         }
                     } else {
-                        const uint16_t *ps = reinterpret_cast<const uint16_t *>(row_ptr(cur, i, r, false)) + c * 64;
-                        const uint16_t *pb = reinterpret_cast<const uint16_t *>(row_ptr(cur, i, r, true)) + c * 64;
+                        const unsigned char *ps = row_ptr(cur, i, r, false) + c * 128, *pb = row_ptr(cur, i, r, true) + c * 128;
+                        const unsigned char *ws = (const unsigned char *)((uintptr_t)ps & ~(uintptr_t)15), *wb = (const unsigned char *)((uintptr_t)pb & ~(uintptr_t)15);
+                        const uint32_t os = (uint32_t)(ps - ws), ob = (uint32_t)(pb - wb);
+                        const int ns = (int)(os + 2 * gn + 15) >> 4, nb = (int)(ob + 2 * gn + 15) >> 4;  // windows, at most 9
+                        const Bytes ms = matrix_bytes(cur, i, false), mb = matrix_bytes(cur, i, true);
+                        if (ws >= ms.begin && ws + 16 * ns <= ms.end && wb >= mb.begin && wb + 16 * nb <= mb.end) {
 #pragma unroll
-                        for (int q = 0; q < 64; q++) v[q] = q < gn ? fmaf(8.f, bf16_bits_to_float(__ldg(ps + q)), bf16_bits_to_float(__ldg(pb + q))) : 0.f;
+                            for (int h = 0; h < 2; h++) {  // 32 groups at a time: ten loads on their way together
+                                uint4 s4[5], b4[5];
+#pragma unroll
+                                for (int q = 0; q < 5; q++) {
+                                    s4[q] = 4 * h + q < ns ? window16(ws + 16 * (4 * h + q)) : make_uint4(0, 0, 0, 0);
+                                    b4[q] = 4 * h + q < nb ? window16(wb + 16 * (4 * h + q)) : make_uint4(0, 0, 0, 0);
+                                }
+#pragma unroll
+                                for (int q = 0; q < 4; q++) {
+                                    const uint4 s8 = cut16(s4[q], s4[q + 1], os), b8 = cut16(b4[q], b4[q + 1], ob);
+                                    const uint32_t sw[4] = {s8.x, s8.y, s8.z, s8.w}, bw[4] = {b8.x, b8.y, b8.z, b8.w};
+#pragma unroll
+                                    for (int k = 0; k < 4; k++) {
+                                        const int at = 32 * h + 8 * q + 2 * k;
+                                        v[at] = at < gn ? fmaf(8.f, __uint_as_float(sw[k] << 16), __uint_as_float(bw[k] << 16)) : 0.f;
+                                        v[at + 1] = at + 1 < gn ? fmaf(8.f, __uint_as_float(sw[k] & 0xffff0000u), __uint_as_float(bw[k] & 0xffff0000u)) : 0.f;
+                                    }
+                                }
+                            }
+                        } else {  // a row at the matrix's edge
+                            const uint16_t *hs = reinterpret_cast<const uint16_t *>(ps), *hb = reinterpret_cast<const uint16_t *>(pb);
+#pragma unroll
+                            for (int q = 0; q < 64; q++) v[q] = q < gn ? fmaf(8.f, bf16_bits_to_float(__ldg(hs + q)), bf16_bits_to_float(__ldg(hb + q))) : 0.f;
+                        }
                     }
                     float m = 0.f;
 #pragma unroll

@@ -51,6 +51,46 @@ def test_products(pkg, n, k, outs):
     c.close()
 
 
+LONG_SHAPES = [  # many tokens, rows enough that the weights are widened once for all of them
+    (300, 64, [1300]), (513, 128, [400, 300, 1]), (301, 192, [1025]), (257, 576, [1281, 3]), (400, 1088, [900]), (320, 2112, [1000, 100]),
+    (290, 4096, [1100]), (97, 4160, [2850]), (300, 8192, [1100]), (289, 8256, [1024, 1, 127]), (304, 12352, [960])]
+
+
+@pytest.mark.parametrize("n,k,outs", LONG_SHAPES)
+def test_products_of_many_tokens(pkg, n, k, outs):
+    rng = np.random.default_rng(7000 + n * 7 + k)
+    c = context(pkg, max_batch=1024)
+    mats = [moe_ref.weights(rng, o, k) for o in outs]
+    x = rng.standard_normal((n, k)).astype(np.float32)
+    for got, m in zip(run(pkg, c, mats, x), mats):
+        moe_ref.close(got, *moe_ref.product(x, m))
+    c.close()
+
+
+@pytest.mark.parametrize("k", [64, 192, 512, 1088, 4096, 4160])
+@pytest.mark.parametrize("n,out", [(1, 130), (5, 130), (40, 130), (300, 1100)])
+def test_scales_at_every_even_address(pkg, n, k, out):
+    """Scales and biases need no more than their type's alignment, and what stands around them is not used."""
+    rng = np.random.default_rng(n + k)
+    c = context(pkg, max_batch=512)
+    mat = moe_ref.weights(rng, out, k)
+    x = rng.standard_normal((n, k)).astype(np.float32)
+    want, bound = moe_ref.product(x, mat)
+    xd, words = torch.from_numpy(x).cuda(), torch.from_numpy(mat[0].view(np.int32)).cuda()
+    size = out * (k // 64)
+    for s_at, b_at in [(0, 0), (1, 0), (2, 7), (5, 3), (4, 4), (7, 6)]:
+        views = []
+        for at, part in ((s_at, mat[1]), (b_at, mat[2])):
+            block = torch.full((size + 32,), float("nan"), device="cuda", dtype=torch.bfloat16)
+            views.append(block[8 + at: 8 + at + size].view(out, k // 64))
+            views[-1].copy_(torch.from_numpy(part.view(np.int16)).cuda().view(torch.bfloat16).view(out, k // 64))
+        y = torch.full((n, out), 7.0, device="cuda")
+        c.proj_forward([pkg.proj_weights(words, *views)], n, xd, [y])
+        c.synchronize()
+        moe_ref.close(y.cpu().numpy(), want, bound)
+    c.close()
+
+
 @pytest.mark.parametrize("n", [1, 4, 13, 40])
 def test_inputs_of_every_size(pkg, n):
     """Outliers beside small values, groups of zeros, values at both ends of fp32's range: no group loses its own."""
