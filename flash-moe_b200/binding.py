@@ -74,7 +74,7 @@ class FmExpertWeights(C.Structure):
                 ("group_size", C.c_int), ("expert_stride", C.c_int64),
                 ("gate_w", C.c_void_p), ("gate_scales", C.c_void_p), ("gate_biases", C.c_void_p),
                 ("up_w", C.c_void_p), ("up_scales", C.c_void_p), ("up_biases", C.c_void_p),
-                ("down_w", C.c_void_p), ("down_scales", C.c_void_p), ("down_biases", C.c_void_p)]
+                ("down_w", C.c_void_p), ("down_scales", C.c_void_p), ("down_biases", C.c_void_p), ("total_experts", C.c_int)]
 
 
 class FmError(RuntimeError):
@@ -154,13 +154,14 @@ def proj_weights(w, scales, biases) -> FmProjWeights:
     return r
 
 
-def expert_weights(gate, up, down, first_expert: int = 0) -> FmExpertWeights:
+def expert_weights(gate, up, down, first_expert: int = 0, total_experts: int = 0) -> FmExpertWeights:
     """Stacks of 4-bit affine matrices in device memory, each a (w, scales, biases) of CUDA tensors: gate and up
-    [experts][inter][hidden / 8], down [experts][hidden][inter / 8] int32 words, [..][in / 64] bf16 scales and biases."""
+    [experts][inter][hidden / 8], down [experts][hidden][inter / 8] int32 words, [..][in / 64] bf16 scales and biases.
+    total_experts: how many the model has, where these are a part of them (0: all)."""
     experts, inter, hidden = gate[0].shape[0], gate[0].shape[1], down[0].shape[1]
     for (w, s, b), (rows, cols) in ((gate, (inter, hidden)), (up, (inter, hidden)), (down, (hidden, inter))):
         assert w.shape == (experts, rows, cols // 8) and s.shape == b.shape == (experts, rows, cols // 64)
-    r = FmExpertWeights(FM_W_Q4_AFFINE, experts, first_expert, hidden, inter, 64, 0, *(_ptr(t) for m in (gate, up, down) for t in m))
+    r = FmExpertWeights(FM_W_Q4_AFFINE, experts, first_expert, hidden, inter, 64, 0, *(_ptr(t) for m in (gate, up, down) for t in m), total_experts)
     r.keep = (gate, up, down)
     return r
 

@@ -6,6 +6,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <cmath>
 #include <new>
 
 #include <cstdlib>
@@ -1050,10 +1051,37 @@ struct Carver {  // pieces of a block, 256-byte aligned; base null: only counts
     }
 };
 
-// Up to this many tokens (projections) or pairs per expert held (experts) the weights stream past the activations on the
-// integer tensor cores; beyond, the prompt form takes over.
-constexpr int kProjStreamTokens = 16;
-constexpr int kExpertStreamPairs = 3;
+// Which form a product of 4-bit weights takes, by what each is expected to take (us).  The stream form reads the weights once
+// per 8 tokens (experts: once per job of up to 4 pairs), the later passes mostly from L2; the prompt form widens a tile of 256
+// rows once per 96 tokens, and a tile takes about as long for one token as for 96, so it is bound by the tiles an SM gets.
+// Measured, stream form then prompt form: 4096 inputs, 20480 rows, 8 tokens 26 and 36 us, 9 tokens 42 and 36; 4096 rows, 64
+// tokens 36 and 40, 512 rows 12 and 40; 128 inputs, 8191 rows, 923 tokens 107 and 29; 1408 inputs, 32 rows, 967 tokens 8 and 20.
+// Over 109 sizes (5 to 1024 tokens, 64 to 8192 inputs, 16 to 16384 rows) the choice costs 0.2 % against always the better one.
+static bool proj_streams(const FmProjWeights *w, int count, int n, int sm_count) {
+    double rows = 0, tiles = 0;
+    for (int i = 0; i < count; i++) {
+        rows += (w[i].out_dim + 15) / 16 * 16;
+        tiles += (w[i].out_dim + 255) / 256;
+    }
+    const double k = w[0].in_dim, passes = (n + 7) / 8, waves = std::ceil(tiles * ((n + kGemmTokens - 1) / kGemmTokens) / sm_count);
+    return passes * rows * k / 4.2e6 <= waves * k * 9e-3;
+}
+// Experts have a third form for few pairs, one job per pair straight from the ids: no plan to wait for (5 us), but an expert is
+// read again for each of its pairs.  Tokens are taken to choose evenly among the model's experts.
+// Measured, straight, stream and prompt form: 512 experts of 4096 x 1024, 10 per token, 1 token 29, 38 and 118 us, 48 tokens -,
+// 447 and 773, 208 tokens -, 1170 and 1298, 320 tokens -, 1687 and 1428; 16 experts of 1024 x 512, one per token, 16 tokens 11,
+// 17 and 34, 128 tokens 31, 25 and 41.  Over 110 sizes the choice costs 2 % against always the best one.
+enum class ExpertForm { kStraight, kStream, kPrompt };
+static ExpertForm expert_form(const FmExpertWeights *w, int n, int top_k, int sm_count) {
+    const double all = std::max(w->total_experts, w->num_experts), held = w->num_experts, pairs = (double)n * top_k, here = pairs * held / all;
+    const double used = std::min(here, held * (1 - std::pow(1 - std::min(1.0, top_k / all), n)));  // experts
+    auto jobs = [&](double tile) { return std::max(used, here / tile + used * (tile - 1) / (2 * tile)); };
+    const double h = w->hidden, i = w->inter, size = 3 * h * i, many = std::ceil(jobs(kGemmTokens));
+    const double straight = pairs * size / 8.5e6, stream = 5 + jobs(4) * size / 8e6;
+    const double prompt = 22 + (std::ceil(many * std::ceil(i / 128) / sm_count) * h + std::ceil(many * std::ceil(h / 256) / sm_count) * i) * 11e-3;
+    if (straight <= stream && straight <= prompt) return ExpertForm::kStraight;
+    return stream <= prompt ? ExpertForm::kStream : ExpertForm::kPrompt;
+}
 
 static bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 static bool aligned2(const void *a, const void *b) { return (((uintptr_t)a | (uintptr_t)b) & 1) == 0; }
@@ -1087,7 +1115,7 @@ extern "C" fm_status fm_proj_forward(FmCtx *ctx, int count, const FmProjWeights 
     }
     if (!ok) return fail(ctx, FM_ERR_INVALID, "fm_proj_forward: staging buffer too small (raise max_batch_tokens)");
     if (!aligned16(p.x)) return fail(ctx, FM_ERR_INVALID, "fm_proj_forward: x is not 16-byte aligned");
-    const bool gemm = n > kProjStreamTokens;
+    const bool gemm = !proj_streams(w, count, n, ctx->sm_count);
     void *xs = nullptr;
     float *tscale = nullptr;
     fm_status st;
@@ -1175,6 +1203,8 @@ extern "C" fm_status fm_moe_experts(FmCtx *ctx, const FmExpertWeights *w, int n,
                     w->format, w->group_size, w->num_experts, w->hidden, w->inter, top_k);
     if (w->first_expert < 0 || w->expert_stride < 0 || w->expert_stride % 16)
         return fail(ctx, FM_ERR_INVALID, "fm_moe_experts: first_expert %d, expert_stride %lld (0 or a multiple of 16)", w->first_expert, (long long)w->expert_stride);
+    if (w->total_experts < 0 || (w->total_experts > 0 && w->total_experts < (long long)w->first_expert + w->num_experts))
+        return fail(ctx, FM_ERR_INVALID, "fm_moe_experts: total_experts %d (0 or at least first_expert + num_experts)", w->total_experts);
     if (n < 0 || n > ctx->cfg.max_batch_tokens) return fail(ctx, FM_ERR_INVALID, "fm_moe_experts: n=%d exceeds max_batch_tokens=%d", n, ctx->cfg.max_batch_tokens);
     if (!aligned16(w->gate_w) || !aligned16(w->up_w) || !aligned16(w->down_w) || !aligned2(w->gate_scales, w->gate_biases) || !aligned2(w->up_scales, w->up_biases) ||
         !aligned2(w->down_scales, w->down_biases) || !aligned4(expert_ids) || !aligned4(weights))
@@ -1196,7 +1226,8 @@ extern "C" fm_status fm_moe_experts(FmCtx *ctx, const FmExpertWeights *w, int n,
         return fail(ctx, FM_ERR_INVALID, "fm_moe_experts: x, residual, h_out and h_norm have to be 16-byte aligned, norm_w 8-byte");
 
     MoePlan plan = {};
-    const bool gemm = pairs > (size_t)kExpertStreamPairs * w->num_experts && pairs > 16;
+    const ExpertForm form = expert_form(w, n, top_k, ctx->sm_count);
+    const bool gemm = form == ExpertForm::kPrompt;
     float *hbuf = nullptr, *ybuf = nullptr, *xscale = nullptr, *hscale = nullptr;
     void *xs = nullptr, *hs = nullptr;
     auto carve = [&](Carver cv) {
@@ -1232,7 +1263,7 @@ extern "C" fm_status fm_moe_experts(FmCtx *ctx, const FmExpertWeights *w, int n,
     gu.mat[1] = view(w->up_w, w->up_scales, w->up_biases, I, H);
     dn.in_dim = w->inter; dn.x = hbuf; dn.nmat = 1; dn.out[0] = ybuf;
     dn.mat[0] = view(w->down_w, w->down_scales, w->down_biases, H, I);
-    if (pairs > 16) {  // fewer: one job per pair, straight from the ids
+    if (form != ExpertForm::kStraight) {
         st = launched(ctx, launch_moe_plan(d_ids, (int)pairs, w->first_expert, w->num_experts, gemm ? kGemmTokens : 4, plan, ctx->stream), "moe_plan");
         if (st) return st;
         gu.plan = dn.plan = plan;

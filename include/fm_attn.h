@@ -355,7 +355,8 @@ fm_status fm_moe_route(FmCtx *ctx, const FmRouteConfig *rc, int n, const float *
  * FmProjWeights.  expert_stride = 0: each of the nine arrays is packed by itself; else it is the distance in bytes (a multiple
  * of 16) from one expert to the next in all nine (one blob per expert).
  * Experts [first_expert, first_expert + num_experts) are the ones held here; slots with any other id (-1, another rank's) add
- * nothing, so the ranks of an expert-sharded model sum their h_out (with the residual on one of them).
+ * nothing, so the ranks of an expert-sharded model sum their h_out (with the residual on one of them).  total_experts says
+ * how many the model has (0: those held are all); only the choice of kernels depends on it.
  * An expert that several slots or tokens name is read once for all of them, as far as that pays; the same id twice in a
  * token counts twice.  x [n][hidden], expert_ids and weights [n][top_k] (top_k <= 32), residual, h_out and h_norm [n][hidden]
  * follow the pointer mode; h_out may be the residual itself, and x may be h_out or h_norm.  hidden and inter multiples of 64
@@ -376,6 +377,7 @@ typedef struct FmExpertWeights {
     const uint16_t *up_scales, *up_biases;
     const uint32_t *down_w;
     const uint16_t *down_scales, *down_biases;
+    int total_experts;           /* of the whole model; 0 = num_experts */
 } FmExpertWeights;
 fm_status fm_moe_experts(FmCtx *ctx, const FmExpertWeights *w, int n, int top_k, const float *x, const int *expert_ids,
                          const float *weights, const float *residual, const uint16_t *norm_w, float *h_out, float *h_norm);

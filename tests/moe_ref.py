@@ -116,21 +116,21 @@ def experts(gate, up, down, x, ids, weights, residual, norm_w, first=0, eps=1e-6
     held = gate[0].shape[0]
     h = np.zeros((n, hidden)) if residual is None else np.asarray(residual, np.float64).copy()
     bound = np.abs(h) * 4 * EPS
-    for t in range(n):
-        for j, e in enumerate(ids[t]):
-            e = int(e) - first
-            if not 0 <= e < held:
-                continue
-            g, bg = product(x[t:t + 1], [m[e] for m in gate])
-            u, bu = product(x[t:t + 1], [m[e] for m in up])
-            sil = g / (1 + np.exp(-g))
-            a = sil * u
-            ba = 1.1 * bg * np.abs(u) + np.abs(sil) * bu + 1.1 * bg * bu + 16 * EPS * np.abs(a)
-            y, by = product(a, [m[e] for m in down])
-            by = by + ba @ np.abs(matrix(*[m[e] for m in down])).T
-            w = abs(float(weights[t, j]))
-            h[t] += float(weights[t, j]) * y[0]
-            bound[t] += w * (by[0] + (ids.shape[1] + 4) * EPS * np.abs(y[0]))
+    ids = np.asarray(ids, np.int64) - first
+    for e in range(held):
+        t, j = np.nonzero(ids == e)
+        if len(t) == 0:
+            continue
+        g, bg = product(x[t], [m[e] for m in gate])
+        u, bu = product(x[t], [m[e] for m in up])
+        sil = g / (1 + np.exp(-g))
+        a = sil * u
+        ba = 1.1 * bg * np.abs(u) + np.abs(sil) * bu + 1.1 * bg * bu + 16 * EPS * np.abs(a)
+        y, by = product(a, [m[e] for m in down])
+        by = by + ba @ np.abs(matrix(*[m[e] for m in down])).T
+        w = np.asarray(weights, np.float64)[t, j][:, None]
+        np.add.at(h, t, w * y)
+        np.add.at(bound, t, np.abs(w) * (by + (ids.shape[1] + 4) * EPS * np.abs(y)))
     inv = 1 / np.sqrt((h * h).mean(1, keepdims=True) + eps)
     nw = np.ones(hidden) if norm_w is None else f32(norm_w).astype(np.float64)
     return h, h * inv * nw, bound

@@ -292,6 +292,7 @@ def test_refusals(pkg):
                 dict(x_=None), dict(ids_=None), dict(w_=None), dict(out_=None), dict(x_=x.view(-1)[1:129]), dict(out_=out.view(-1)[1:129]), dict(nrm=out.view(-1)[2:130]),
                 dict(res=x.view(-1)[3:131])):
         assert status(**bad) == B.FM_ERR_INVALID
+    assert status(total_experts=-1) == status(total_experts=2) == status(total_experts=5, first_expert=3) == B.FM_ERR_INVALID
     c.moe_experts(dev, 0, 2, x, ids, w, None, None, out, None)
     c.synchronize()
     assert torch.all(out == 7.0)
