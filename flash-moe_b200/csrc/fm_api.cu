@@ -1286,7 +1286,7 @@ extern "C" fm_status fm_moe_experts(FmCtx *ctx, const FmExpertWeights *w, int n,
     }
     if (st) return st;
     st = launched(ctx, launch_moe_combine(ybuf, d_ids, d_w, n, top_k, w->first_expert, w->num_experts, w->hidden, d_res, d_nw, ctx->cfg.rms_norm_eps, d_out,
-                                          d_norm, ctx->stream), "moe_combine");
+                                          d_norm, ctx->sm_count, ctx->stream), "moe_combine");
     if (st) return st;
     if (sg.host && gemm) FM_CUDA(ctx, cudaMemcpyAsync(ctx->h_err, ctx->d_err, sizeof(int), cudaMemcpyDeviceToHost, ctx->stream));
     FM_CUDA(ctx, sg.pull(h_out, w_out, n * H));

@@ -331,7 +331,7 @@ int launch_q4_gemm(Q4Mode mode, const Q4Params &p, const void *xs, int xs_rows, 
 int launch_moe_plan(const int *ids, int pairs, int first_expert, int num_experts, int tile, const MoePlan &plan, cudaStream_t st);
 // h = residual + sum over the slots of weight * y[pair]; h_norm = rms-norm(h) * norm_w (moe_plan.cu)
 int launch_moe_combine(const float *y, const int *ids, const float *weights, int n, int top_k, int first_expert, int num_experts, int hidden,
-                       const float *residual, const uint16_t *norm_w, float eps, float *h_out, float *h_norm, cudaStream_t st);
+                       const float *residual, const uint16_t *norm_w, float eps, float *h_out, float *h_norm, int sm_count, cudaStream_t st);
 
 struct PrefillWork {
     void *q16, *k16, *v16;

@@ -73,8 +73,11 @@ moe_plan_kernel(const int *__restrict__ ids, int pairs, int first_expert, int nu
 }
 
 // One CTA per token.  The slots are summed in their order, so the result does not depend on the launch; eight of their loads
-// are in flight at a time.  A few tokens get four columns per thread (the row at once: 7 us for 10 slots of 4096), many get
-// small CTAs, four to an SM, which cover each other's meeting points (4096 tokens: 180 -> 150 us, 4.9 TB/s).
+// are in flight at a time.  Up to two tokens per SM get four columns per thread (the row at once), more get small CTAs, four
+// to an SM, which cover each other's meeting points.  Measured, large then small CTAs, whole calls with 8 slots of 4096 columns
+// and experts of 64 inputs: 148 tokens 92 and 97 us, 296 tokens 117 and 118, 400 tokens 133 and 130, 1000 tokens 234 and 222;
+// 4096 tokens with 10 slots, by itself: 180 and 150 us (4.9 TB/s).  A row split over a cluster of CTAs, with the ids fetched
+// before the products end, took the same time at one token.
 constexpr int kCombineThreads = 1024, kCombineThreadsMany = 256;
 constexpr int kCombineBatch = 8;
 
@@ -145,9 +148,9 @@ int launch_moe_plan(const int *ids, int pairs, int first_expert, int num_experts
 }
 
 int launch_moe_combine(const float *y, const int *ids, const float *weights, int n, int top_k, int first_expert, int num_experts, int hidden,
-                       const float *residual, const uint16_t *norm_w, float eps, float *h_out, float *h_norm, cudaStream_t st) {
-    return launch_dependent(moe_combine_kernel, dim3(n), dim3(std::min(n > 296 ? kCombineThreadsMany : kCombineThreads, (hidden / 4 + 31) / 32 * 32)), 0, st, y, ids, weights, top_k, first_expert, num_experts, hidden, residual, norm_w, eps,
-                            h_out, h_norm) == cudaSuccess ? 1 : -1;
+                       const float *residual, const uint16_t *norm_w, float eps, float *h_out, float *h_norm, int sm_count, cudaStream_t st) {
+    return launch_dependent(moe_combine_kernel, dim3(n), dim3(std::min(n > 2 * sm_count ? kCombineThreadsMany : kCombineThreads, (hidden / 4 + 31) / 32 * 32)), 0, st, y, ids,
+                            weights, top_k, first_expert, num_experts, hidden, residual, norm_w, eps, h_out, h_norm) == cudaSuccess ? 1 : -1;
 }
 
 }  // namespace fm
