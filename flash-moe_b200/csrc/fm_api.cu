@@ -1054,17 +1054,20 @@ struct Carver {  // pieces of a block, 256-byte aligned; base null: only counts
 // Which form a product of 4-bit weights takes, by what each is expected to take (us).  The stream form reads the weights once
 // per 8 tokens (experts: once per job of up to 4 pairs), the later passes mostly from L2; the prompt form widens a tile of 256
 // rows once per 96 tokens, and a tile takes about as long for one token as for 96, so it is bound by the tiles an SM gets.
-// Measured, stream form then prompt form: 4096 inputs, 20480 rows, 8 tokens 26 and 36 us, 9 tokens 42 and 36; 4096 rows, 64
-// tokens 36 and 40, 512 rows 12 and 40; 128 inputs, 8191 rows, 923 tokens 107 and 29; 1408 inputs, 32 rows, 967 tokens 8 and 20.
-// Over 109 sizes (5 to 1024 tokens, 64 to 8192 inputs, 16 to 16384 rows) the choice costs 0.2 % against always the better one.
+// Measured, stream form then prompt form: 4096 inputs, 20480 rows, 8 tokens 26 and 38 us, 9 tokens 42 and 38; 4096 rows, 48
+// tokens 28.5 and 28.7, 512 rows, 64 tokens 12 and 33; 128 inputs, 8191 rows, 923 tokens 107 and 29; 1408 inputs, 32 rows, 967
+// tokens 8 and 19.  Over 149 sizes (5 to 1024 tokens, 64 to 8192 inputs, 16 to 20480 rows) the choice costs less than 0.1 %
+// against always the better one.
 static bool proj_streams(const FmProjWeights *w, int count, int n, int sm_count) {
     double rows = 0, tiles = 0;
     for (int i = 0; i < count; i++) {
         rows += (w[i].out_dim + 15) / 16 * 16;
         tiles += (w[i].out_dim + 255) / 256;
     }
-    const double k = w[0].in_dim, passes = (n + 7) / 8, waves = std::ceil(tiles * ((n + kGemmTokens - 1) / kGemmTokens) / sm_count);
-    return passes * rows * k / 4.2e6 <= waves * k * 9e-3;
+    const double k = w[0].in_dim, passes = (n + 7) / 8, units = tiles * ((n + kGemmTokens - 1) / kGemmTokens);
+    const double whole = std::floor(units / sm_count), rest = units - whole * sm_count;
+    const double waves = whole + (rest == 0 ? 0 : 2 * rest <= sm_count ? 0.7 : 1);  // (a last wave of few units is cut in two)
+    return passes * rows * k / 4.2e6 <= waves * k * 8e-3;
 }
 // Experts have a third form for few pairs, one job per pair straight from the ids: no plan to wait for (5 us), but an expert is
 // read again for each of its pairs.  Tokens are taken to choose evenly among the model's experts.

@@ -126,13 +126,18 @@ struct Ring {
 struct Unit {
     int mat, row0, rows;   // matrix, first row, rows of the matrix
     int expert;
-    int tiles;             // row tiles that hold rows
+    int tiles;             // row tiles that hold rows; none: the second half of a cut unit of one tile, its CTA's last
     int start, cnt, ncols; // tokens (kProj) or positions in pair_of; columns of the MMA
 };
 
 template <Q4Mode MODE, bool WARP = true>
-__device__ __forceinline__ Unit unit_at(const GemmParams &g, int u) {
+__device__ __forceinline__ Unit unit_at(const GemmParams &g, int u, int whole) {
     Unit r;
+    int half = -1;
+    if (MODE == kProj && u >= whole) {
+        half = (u - whole) & 1;
+        u = whole + ((u - whole) >> 1);
+    }
     const int job = u / g.units_per_job;
     int mu = u - job * g.units_per_job;
     r.mat = 0; r.expert = 0;
@@ -146,9 +151,9 @@ __device__ __forceinline__ Unit unit_at(const GemmParams &g, int u) {
         else { r.expert = j.x; r.start = j.y; r.cnt = j.z; }
     }
     constexpr int kRows = MODE == kGateUp ? T * 64 : T * 128;
-    r.row0 = mu * kRows;
+    r.row0 = mu * kRows + (half > 0 ? 128 : 0);
     r.rows = g.p.mat[r.mat].rows;
-    const int t = (min(kRows, r.rows - r.row0) + 127) / 128;
+    const int t = (min(half >= 0 ? 128 : kRows, r.rows - r.row0) + 127) / 128;
     r.tiles = MODE == kGateUp ? 2 * t : t;
     r.ncols = (r.cnt + 15) / 16 * 16;
     return r;
@@ -272,7 +277,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ GemmParams g) {
     extern __shared__ unsigned char smem_raw[];
     __shared__ uint32_t s_tmem;
-    __shared__ int s_abort;
+    __shared__ int s_abort, s_whole, s_units;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t sB = base, sW = sB + kBSlots * kBSlot;
     float *s_f = reinterpret_cast<float *>(smem_raw + (sW + kWSlots * kWSlot - smem_u32(smem_raw)));  // [steps][128 rows] power of two of the step
@@ -301,8 +306,23 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
 
     const int G = g.G, nreal = (G + kChunk - 1) / kChunk, nchunks = nreal + g.pseudo;
-    const int njobs = MODE == kProj ? (g.p.n + kTok - 1) / kTok : uniform(*g.p.plan.njobs);
-    const int nunits = njobs * g.units_per_job;
+    // The units left for a last, partly filled wave are cut into their tiles where every tile then gets an SM of its own; a tile by
+    // itself takes 0.6 (20 tokens) to 0.8 (96) of the two's time.  Measured, 4096 inputs, whole then cut: 17408 rows, 20 tokens 39
+    // and 27 us, 96 tokens 50 and 45; 28608 rows, 300 tokens (3 waves and 4 units) 133 and 119; more units than half of the SMs are
+    // left whole, since the tiles would take two turns.  The counts stay in shared memory: registers are short, and a unit is long.
+    // (Not for the experts: what it adds to a unit cost more there, units being short, than the last wave of many gives.)
+    const int all = (MODE == kProj ? (g.p.n + kTok - 1) / kTok : uniform(*g.p.plan.njobs)) * g.units_per_job;
+    if (MODE == kProj) {
+        if (tid == 0) {
+            const int rest = all % (int)gridDim.x;
+            const bool cut = 2 * rest <= (int)gridDim.x;
+            s_whole = cut ? all - rest : all;
+            s_units = cut ? all + rest : all;
+        }
+        __syncthreads();
+    }
+    auto units = [&]() { return MODE == kProj ? *(volatile int *)&s_units : all; };
+    auto whole = [&]() { return MODE == kProj ? *(volatile int *)&s_whole : all; };
     const size_t s_pitch = (size_t)G * 2;
     // after a wait that ran out: the copies in flight land before the CTA goes (a ring's last `count` loads)
     auto drain = [&](int first, int n, int slot, uint32_t phase, int count) {
@@ -332,8 +352,9 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
         Ring<kBSlots> rb;
         int count = 0;
         bool ok = true;
-        for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x) {
-            const Unit un = unit_at<MODE>(g, u);
+        for (int u = blockIdx.x; u < units() && ok; u += gridDim.x) {
+            const Unit un = unit_at<MODE>(g, u, whole());
+            if (MODE == kProj && un.tiles == 0) break;
             for (int c = 0; c < nchunks && ok; c++) {
                 const int first = c < nreal ? c * kChunk : G + c - nreal, ng = c < nreal ? min(kChunk, G - first) : 1;  // 64 columns of x each
                 for (int j = 0; j < ng && ok; j += 2) {
@@ -359,8 +380,9 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
             Ring<kWSlots> rw;
             int count = 0;
             bool ok = true;
-            for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x) {
-                const Unit un = unit_at<MODE, false>(g, u);
+            for (int u = blockIdx.x; u < units() && ok; u += gridDim.x) {
+                const Unit un = unit_at<MODE, false>(g, u, whole());
+                if (MODE == kProj && un.tiles == 0) break;
                 for (int c = 0; c < nchunks && ok; c++)
                     for (int i = 0; i < un.tiles && ok; i++) {
                         auto load = [&](const CUtensorMap *map, int x) {  // 128 bytes of each of the tile's rows
@@ -396,8 +418,9 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
         // warp never waits on a phase it is two behind), steps of this tile
         uint32_t pairs = 0, mine = 0, steps = 0;
         bool ok = true;
-        for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x) {
-            const Unit un = unit_at<MODE>(g, u);
+        for (int u = blockIdx.x; u < units() && ok; u += gridDim.x) {
+            const Unit un = unit_at<MODE>(g, u, whole());
+            if (MODE == kProj && un.tiles == 0) break;
             const uint32_t idesc = idesc_dense(128, un.ncols, false, 0);
             for (int c = 0; c < nchunks && ok; c++) {
                 const bool real = c < nreal;
@@ -504,11 +527,12 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
         };
         Unit un;
         int u = blockIdx.x;
-        if (u < nunits) {
-            un = unit_at<MODE>(g, u);
-            aim(un);
+        if (u < units()) {
+            un = unit_at<MODE>(g, u, whole());
+            if (MODE == kProj && un.tiles == 0) u = units();
+            else aim(un);
         }
-        while (u < nunits && ok) {
+        while (u < units() && ok) {
             for (int c = 0; c < nreal && ok; c++) {
                 const int na = min(kChunk, G - c * kChunk);
 #pragma unroll 1  // (one copy of the loop's body: the four roles' code has to fit the instruction cache)
@@ -560,9 +584,10 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
             }
             const Unit cur = un;
             u += gridDim.x;
-            if (u < nunits) {
-                un = unit_at<MODE>(g, u);
-                aim(un);
+            if (u < units()) {
+                un = unit_at<MODE>(g, u, whole());
+                if (MODE == kProj && un.tiles == 0) u = units();
+                else aim(un);
             }
             for (int c = 0; c < g.pseudo && ok; c++) {
                 const int gn = min(64, G - c * 64);
@@ -655,8 +680,9 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
         uint32_t seen = 0;  // bit i: parity of tile i's next step
         Ring<kFSteps> rf;
         bool ok = true;
-        for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x) {
-            const Unit un = unit_at<MODE>(g, u);
+        for (int u = blockIdx.x; u < units() && ok; u += gridDim.x) {
+            const Unit un = unit_at<MODE>(g, u, whole());
+            if (MODE == kProj && un.tiles == 0) break;
             // columns half * 48 + 32 q + lane: the row of the output it goes to, and what takes its token's power of two off again
             int out_row[2] = {0, 0};
             float ts[2] = {0.f, 0.f};
@@ -829,7 +855,9 @@ int launch_gemm(const GemmMaps &maps, GemmParams &g, long long jobs, int sm_coun
     if (first_use_on_device(&configured) &&
         cudaFuncSetAttribute(q4_gemm_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem) != cudaSuccess)
         return -1;
-    const int grid = (int)std::min<long long>(jobs * g.units_per_job, sm_count);
+    // (fewer units than SMs: as many CTAs as there are units or, cut, tiles; idle ones would crowd the others onto half of the GPU)
+    const long long units = jobs * g.units_per_job;
+    const int grid = (int)std::min<long long>(MODE == kProj && 2 * units <= sm_count ? 2 * units : units, sm_count);
     return launch_dependent(q4_gemm_kernel<MODE>, dim3(grid), dim3(kGemmThreads), kGemmSmem, st, maps, g) == cudaSuccess ? 1 : -1;
 }
 
