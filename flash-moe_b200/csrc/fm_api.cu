@@ -1057,8 +1057,10 @@ struct Carver {  // pieces of a block, 256-byte aligned; base null: only counts
 // Measured, stream form then prompt form: 4096 inputs, 20480 rows, 8 tokens 26 and 38 us, 9 tokens 42 and 38; 4096 rows, 48
 // tokens 28.5 and 28.7, 512 rows, 64 tokens 12 and 33; 128 inputs, 8191 rows, 923 tokens 107 and 29; 1408 inputs, 32 rows, 967
 // tokens 8 and 19.  Over 149 sizes (5 to 1024 tokens, 64 to 8192 inputs, 16 to 20480 rows) the choice costs less than 0.1 %
-// against always the better one.
+// against always the better one.  Up to 8 tokens it is one pass, and the stream form takes less time at any size (248320 rows of
+// 4096 inputs, 1 token 119 and 240, 8 tokens 204 and 243).
 static bool proj_streams(const FmProjWeights *w, int count, int n, int sm_count) {
+    if (n <= 8) return true;
     double rows = 0, tiles = 0;
     for (int i = 0; i < count; i++) {
         rows += (w[i].out_dim + 15) / 16 * 16;

@@ -65,6 +65,28 @@ def test_projection_host_pointers_and_bits(pkg, many, n, k, out):
     c.close()
 
 
+@pytest.mark.parametrize("n", [1, 8])
+def test_a_few_tokens_are_captured_without_a_call_before(pkg, n):
+    """Up to 8 tokens nothing is allocated, however many rows there are."""
+    rng = np.random.default_rng(515 + n)
+    c = context(pkg)
+    m = moe_ref.weights(rng, 40000, 128)
+    d = on_device(pkg, m)
+    x, y = torch.zeros((n, 128), device="cuda"), torch.empty((n, 40000), device="cuda")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        c.set_stream(torch.cuda.current_stream().cuda_stream)
+        c.proj_forward([d], n, x, [y])
+    c.set_stream(torch.cuda.current_stream().cuda_stream)
+    values = rng.standard_normal((n, 128)).astype(np.float32)
+    x.copy_(torch.from_numpy(values))
+    g.replay()
+    torch.cuda.synchronize()
+    moe_ref.close(y.cpu().numpy(), *moe_ref.product(values, m))
+    del g
+    c.close()
+
+
 def test_projections_of_two_contexts_at_once(pkg):
     rng = np.random.default_rng(520)
     work = []
