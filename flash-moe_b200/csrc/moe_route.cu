@@ -15,7 +15,7 @@
 //
 // Borders.  Which expert is the k-th best is a whole number, so a rounding must not decide it.  The chain therefore takes
 // every expert that the lost bits, or the error of a 32-bit choice, leave possible -- one or two more than asked for -- and
-// these few, one per lane, are put in their exact order: softmax without a bias by the logits themselves, sigmoid by
+// these few, one per lane, are put in their exact order wherever two neighbours leave a doubt: softmax without a bias by the logits themselves, sigmoid by
 // choices in 64 bits.  Where that does not settle it (softmax with a bias, whose denominator would be needed in 64 bits;
 // two groups at the border; more than 32 candidates) the warp takes the whole row again in 64 bits.
 #include <math.h>
@@ -61,6 +61,24 @@ __device__ uint32_t best_groups(T total, int groups, int top, int lane, T *gap, 
     *border = last;
     *gap = next == -INFINITY ? (T)INFINITY : last - next;
     return keep;
+}
+
+// Keys of a lane, largest first: Batcher's odd-even merge sort.
+template <int N>
+__device__ __forceinline__ void sort_down(uint32_t (&k)[N]) {
+#pragma unroll
+    for (int p = 1; p < N; p *= 2)
+#pragma unroll
+        for (int q = p; q >= 1; q /= 2)
+#pragma unroll
+            for (int j = q % p; j + q < N; j += 2 * q)
+#pragma unroll
+                for (int i = 0; i < q; i++)
+                    if (i + j + q < N && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+                        const uint32_t a = k[i + j], b = k[i + j + q];
+                        k[i + j] = max(a, b);
+                        k[i + j + q] = min(a, b);
+                    }
 }
 
 // The same row in 64 bits, taken where 32 cannot tell neighbours apart.  Returns the lane's slot's expert (-1: none).
@@ -250,51 +268,78 @@ moe_route_kernel(const __grid_constant__ RouteParams p) {
 #pragma unroll
     for (int j = 0; j < VPL; j++)
         if (key[j] != 0u) key[j] = (key[j] & ~kIndex) | (kIndex - (uint32_t)(j * 32 + lane));
-    uint32_t mine = 0, last = 0;
-    int nc = 0;
-    if (!unsure) {
-        while (true) {
-            uint32_t best = 0;
+    if constexpr (VPL <= 8) sort_down(key);
+    auto take = [&]() {  // the largest key of all, which leaves its lane
+        uint32_t best = key[0];
+        if constexpr (VPL > 8)
 #pragma unroll
-            for (int j = 0; j < VPL; j++) best = max(best, key[j]);
-            best = __reduce_max_sync(kFull, best);
-            if (best == 0u) break;
-            if (nc >= p.top_k && value_of(best | kIndex) + 2.f * tol_score * (by_logit ? 0.f : 1.f) + (by_logit ? 0.f : 2.4e-7f * fabsf(value_of(best))) < value_of(last & ~kIndex)) break;
-            if (nc == 32) { unsure = true; break; }
-            if (lane == nc) mine = best;
-            nc++;
-            if (nc == p.top_k) last = best;
+            for (int j = 1; j < VPL; j++) best = max(best, key[j]);
+        best = __reduce_max_sync(kFull, best);
+        if constexpr (VPL <= 8) {
+            const bool won = key[0] == best;
+#pragma unroll
+            for (int j = 0; j + 1 < VPL; j++) key[j] = won ? key[j + 1] : key[j];
+            key[VPL - 1] = won ? 0u : key[VPL - 1];
+        } else {
 #pragma unroll
             for (int j = 0; j < VPL; j++) key[j] = key[j] == best ? 0u : key[j];
         }
+        return best;
+    };
+    // whether a candidate's choice is below another's, whatever the lost bits and the choices' errors are
+    auto below = [&](uint32_t a, uint32_t b) {
+        return value_of(a | kIndex) + (by_logit ? 0.f : 2.f * tol_score + 2.4e-7f * fabsf(value_of(a))) < value_of(b & ~kIndex);
+    };
+    uint32_t mine = 0;
+    int nc = 0;
+    if (!unsure) {
+        uint32_t last = 0, best = 0;
+        for (; nc < p.top_k; nc++) {
+            best = take();
+            if (best == 0u) break;
+            if (lane == nc) mine = best;
+            last = best;
+        }
+        while (best != 0u) {
+            best = take();
+            if (best == 0u || below(best, last)) break;
+            if (nc == 32) { unsure = true; break; }
+            if (lane == nc) mine = best;
+            nc++;
+        }
     }
-    // Their exact order: logits as they are, choices in 64 bits (softmax with a bias: in 32, where that decides).
-    int id = lane < nc ? (int)(kIndex - (mine & kIndex)) : -1, rank = 0;
-    const float v0 = id >= 0 ? __ldg(row + id) : -INFINITY;
-    if (by_logit) {
-        for (int j = 0; j < nc; j++) {
-            const float o = __shfl_sync(kFull, v0, j);
-            const int oe = __shfl_sync(kFull, id, j);
-            rank += (o > v0 || (o == v0 && oe < id)) ? 1 : 0;
+    // Their exact order, where two neighbours leave a doubt: logits as they are, choices in 64 bits (softmax with a bias: in 32,
+    // where that decides).
+    int id = lane < nc ? (int)(kIndex - (mine & kIndex)) : -1, rank = lane;
+    const uint32_t before = __shfl_up_sync(kFull, mine, 1);
+    if (__any_sync(kFull, lane > 0 && lane < nc && !below(mine, before))) {
+        const float v0 = id >= 0 ? __ldg(row + id) : -INFINITY;
+        rank = 0;
+        if (by_logit) {
+            for (int j = 0; j < nc; j++) {
+                const float o = __shfl_sync(kFull, v0, j);
+                const int oe = __shfl_sync(kFull, id, j);
+                rank += (o > v0 || (o == v0 && oe < id)) ? 1 : 0;
+            }
+        } else if (!softmax) {
+            double c = -INFINITY;
+            if (id >= 0) c = 1.0 / (1.0 + exp(-(double)v0)) + (p.bias != nullptr ? (double)__ldg(p.bias + id) : 0.0);
+            for (int j = 0; j < nc; j++) {
+                const double o = __shfl_sync(kFull, c, j);
+                const int oe = __shfl_sync(kFull, id, j);
+                rank += (o > c || (o == c && oe < id)) ? 1 : 0;
+            }
+        } else {
+            const float c = id >= 0 ? (v0 == m ? 1.f : expf(v0 - m)) * inv + __ldg(p.bias + id) : -INFINITY;
+            bool near = false;
+            for (int j = 0; j < nc; j++) {
+                const float o = __shfl_sync(kFull, c, j);
+                const int oe = __shfl_sync(kFull, id, j);
+                rank += (o > c || (o == c && oe < id)) ? 1 : 0;
+                near |= oe != id && !(fabsf(o - c) > 2.f * tol_score + 2.4e-7f * fabsf(c));
+            }
+            unsure |= __any_sync(kFull, near && id >= 0);
         }
-    } else if (!softmax) {
-        double c = -INFINITY;
-        if (id >= 0) c = 1.0 / (1.0 + exp(-(double)v0)) + (p.bias != nullptr ? (double)__ldg(p.bias + id) : 0.0);
-        for (int j = 0; j < nc; j++) {
-            const double o = __shfl_sync(kFull, c, j);
-            const int oe = __shfl_sync(kFull, id, j);
-            rank += (o > c || (o == c && oe < id)) ? 1 : 0;
-        }
-    } else {
-        const float c = id >= 0 ? (v0 == m ? 1.f : expf(v0 - m)) * inv + __ldg(p.bias + id) : -INFINITY;
-        bool near = false;
-        for (int j = 0; j < nc; j++) {
-            const float o = __shfl_sync(kFull, c, j);
-            const int oe = __shfl_sync(kFull, id, j);
-            rank += (o > c || (o == c && oe < id)) ? 1 : 0;
-            near |= oe != id && !(fabsf(o - c) > 2.f * tol_score + 2.4e-7f * fabsf(c));
-        }
-        unsure |= __any_sync(kFull, near && id >= 0);
     }
     if (unsure) {
         id = select_in_double<VPL>(p, row, lane);
