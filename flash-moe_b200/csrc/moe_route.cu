@@ -15,8 +15,8 @@
 //
 // Borders.  Which expert is the k-th best is a whole number, so a rounding must not decide it.  The chain therefore takes
 // every expert that the lost bits, or the error of a 32-bit choice, leave possible -- one or two more than asked for -- and
-// these few, one per lane, are put in their exact order wherever two neighbours leave a doubt: softmax without a bias by the logits themselves, sigmoid by
-// choices in 64 bits.  Where that does not settle it (softmax with a bias, whose denominator would be needed in 64 bits;
+// these few, one per lane, are put in their exact order wherever two neighbours leave a doubt: softmax without a
+// bias by the logits themselves, sigmoid by choices in 64 bits.  Where that does not settle it (softmax with a bias, whose denominator would be needed in 64 bits;
 // two groups at the border; more than 32 candidates) the warp takes the whole row again in 64 bits.
 #include <math.h>
 
@@ -206,26 +206,19 @@ moe_route_kernel(const __grid_constant__ RouteParams p) {
 
     if (p.groups > 1) {
         const int size = p.experts / p.groups;
-        float mine = -INFINITY;  // lane g: the total of group g
-        auto total_of = [&](int g, uint32_t m1, uint32_t m2) {  // each lane's best two of the group
+        // lane g gets the best two of group g, from each lane's best two of it; free of branches, so that the groups' chains overlap
+        uint32_t g1 = 0, g2 = 0;
+        auto best_two = [&](int g, uint32_t m1, uint32_t m2) {
             const uint32_t a = __reduce_max_sync(kFull, m1);
-            float total = -INFINITY;
-            if (a != 0u) {
-                // by_logit: the group's best scores are those of its best logits; of one best, compare the logits themselves
-                const float va = value_of(a);
-                total = by_logit && p.group_best == 2 ? (va == m ? 1.f : expf(va - m)) * inv : va;
-                if (p.group_best == 2) {
-                    const uint32_t at = __ballot_sync(kFull, m1 == a);
-                    const uint32_t b = __popc(at) > 1 ? a : __reduce_max_sync(kFull, m1 == a ? m2 : m1);
-                    if (b != 0u) {
-                        const float vb = value_of(b);
-                        total += by_logit ? (vb == m ? 1.f : expf(vb - m)) * inv : vb;
-                    }
-                }
-            }
-            if (lane == g) mine = total;
+            const int holder = __ffs(__ballot_sync(kFull, m1 == a)) - 1;
+            const uint32_t b = __reduce_max_sync(kFull, lane == holder ? m2 : m1);
+            g1 = lane == g ? a : g1;
+            g2 = lane == g ? b : g2;
         };
-        if (size % 32 == 0) {  // whole registers per group
+        if (size == 32) {  // a register per group
+#pragma unroll
+            for (int j = 0; j < VPL; j++) best_two(j, key[j], 0u);
+        } else if (size % 32 == 0) {  // whole registers per group
             const int regs = size / 32;
             uint32_t m1 = 0, m2 = 0;
             int left = regs, g = 0;
@@ -233,8 +226,8 @@ moe_route_kernel(const __grid_constant__ RouteParams p) {
             for (int j = 0; j < VPL; j++) {
                 m2 = max(m2, min(m1, key[j]));
                 m1 = max(m1, key[j]);
-                if (--left == 0 && g < p.groups) {
-                    total_of(g++, m1, m2);
+                if (--left == 0) {
+                    best_two(g++, m1, m2);
                     m1 = m2 = 0; left = regs;
                 }
             }
@@ -249,8 +242,19 @@ moe_route_kernel(const __grid_constant__ RouteParams p) {
                     m2 = max(m2, min(m1, k));
                     m1 = max(m1, k);
                 }
-                total_of(g, m1, m2);
+                best_two(g, m1, m2);
             }
+        }
+        // lane g: the total of group g.  by_logit: the group's best scores are those of its best logits; of one best, compare the
+        // logits themselves
+        float mine = -INFINITY;
+        if (lane < p.groups && g1 != 0u) {
+            auto score = [&](uint32_t k) {
+                const float v = value_of(k);
+                return by_logit && p.group_best == 2 ? (v == m ? 1.f : expf(v - m)) * inv : v;
+            };
+            mine = score(g1);
+            if (p.group_best == 2 && g2 != 0u) mine += score(g2);
         }
         float gap, border;
         const uint32_t keep = best_groups<float>(mine, p.groups, p.top_groups, lane, &gap, &border);
