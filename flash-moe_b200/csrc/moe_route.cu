@@ -10,14 +10,15 @@
 // One warp per token, expert j * 32 + lane in register j: the row is read once, coalesced, and nothing leaves the
 // registers.  Selection works on order-preserving 32-bit keys whose low bits make room for the expert's index, one redux
 // per slot for value and holder together.  What bounds it is that chain (a redux and a pass over the lane's keys per slot),
-// not the bytes: one token of 512 experts takes 4 us, all of it latency; 8192 tokens of 256 experts 10 us by softmax, 12 us by
-// sigmoid, 20 us with a bias and 8 groups (8.9 MB: the memory would take 1.4 us).
+// not the bytes: one token of 512 experts takes 4 us, all of it latency; 8192 tokens of 256 experts 8 us by softmax, 9.7 us by
+// sigmoid, 11.8 us with a bias, 15.1 us with a bias and 8 groups (8.9 MB: the memory would take 1.4 us).
 //
 // Borders.  Which expert is the k-th best is a whole number, so a rounding must not decide it.  The chain therefore takes
 // every expert that the lost bits, or the error of a 32-bit choice, leave possible -- one or two more than asked for -- and
 // these few, one per lane, are put in their exact order wherever two neighbours leave a doubt: softmax without a
 // bias by the logits themselves, sigmoid by choices in 64 bits.  Where that does not settle it (softmax with a bias, whose denominator would be needed in 64 bits;
-// two groups at the border; more than 32 candidates) the warp takes the whole row again in 64 bits.
+// more than 32 candidates) the warp takes the whole row again in 64 bits; likewise the groups' totals, where two groups are
+// at the border.
 #include <math.h>
 
 #include "fm_device.cuh"
@@ -81,11 +82,31 @@ __device__ __forceinline__ void sort_down(uint32_t (&k)[N]) {
                     }
 }
 
-// The same row in 64 bits, taken where 32 cannot tell neighbours apart.  Returns the lane's slot's expert (-1: none).
+// Order-preserving map of doubles that are not NaN; 0 stands below every value.  The largest of the warp by its two halves: two
+// dependent redux, where a butterfly of doubles takes five rounds.
+__device__ __forceinline__ unsigned long long key_of(double d) {
+    const long long b = __double_as_longlong(d);
+    return (unsigned long long)(b ^ (b >> 63 | (long long)0x8000000000000000ull));
+}
+__device__ __forceinline__ double value_of(unsigned long long k) {
+    return __longlong_as_double((long long)(k & 0x8000000000000000ull ? k ^ 0x8000000000000000ull : ~k));
+}
+__device__ __forceinline__ unsigned long long warp_max_key(unsigned long long k) {
+    const uint32_t hi = __reduce_max_sync(kFull, (uint32_t)(k >> 32));
+    const uint32_t lo = __reduce_max_sync(kFull, (uint32_t)(k >> 32) == hi ? (uint32_t)k : 0u);
+    return (unsigned long long)hi << 32 | lo;
+}
+
+// Longer rows keep their doubles in local memory: in registers they would cost every warp its share (512 experts, 8192 tokens
+// 14.5 us, with 158 registers 17.6).
 template <int VPL>
-__device__ __noinline__ int select_in_double(const RouteParams &p, const float *row, int lane) {
-    double c[VPL];
+constexpr int kDoubleUnroll = VPL <= 8 ? VPL : 1;
+
+// A row's choices in 64 bits (-inf: not available).
+template <int VPL>
+__device__ __forceinline__ void choices_in_double(const RouteParams &p, const float *row, int lane, double (&c)[VPL]) {
     double m = -INFINITY, sum = 0.0;
+#pragma unroll(kDoubleUnroll<VPL>)
     for (int j = 0; j < VPL; j++) {
         const int e = j * 32 + lane;
         const float x = e < p.experts ? row[e] : -INFINITY;
@@ -94,37 +115,57 @@ __device__ __noinline__ int select_in_double(const RouteParams &p, const float *
         m = fmax(m, c[j]);
     }
     m = warp_max_d(m);
+#pragma unroll(kDoubleUnroll<VPL>)
     for (int j = 0; j < VPL; j++) {
         if (c[j] == -INFINITY) continue;
         c[j] = p.score == FM_SCORE_SOFTMAX ? (c[j] == m ? 1.0 : exp(c[j] - m)) : 1.0 / (1.0 + exp(-c[j]));
         sum += c[j];
     }
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+    if (p.score == FM_SCORE_SOFTMAX)
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+#pragma unroll(kDoubleUnroll<VPL>)
     for (int j = 0; j < VPL; j++) {
         if (c[j] == -INFINITY) continue;
         if (p.score == FM_SCORE_SOFTMAX) c[j] /= sum;
         if (p.bias != nullptr) c[j] += (double)p.bias[j * 32 + lane];
     }
+}
+
+// The groups that survive, where the 32-bit totals do not tell.  A few warps of thousands come here, and a launch waits for them:
+// 8192 tokens of 256 experts in 8 groups take 14.6 us without and 15.1 with them (20 when they took the whole row this way).
+template <int VPL>
+__device__ __noinline__ uint32_t groups_in_double(const RouteParams &p, const float *row, int lane) {
+    double c[VPL];
+    choices_in_double<VPL>(p, row, lane, c);
+    const int size = p.experts / p.groups;
+    unsigned long long g1 = 0, g2 = 0;
+    for (int g = 0; g < p.groups; g++) {
+        unsigned long long m1 = 0, m2 = 0;
+#pragma unroll(kDoubleUnroll<VPL>)
+        for (int j = 0; j < VPL; j++) {
+            if (j * 32 + 31 < g * size || j * 32 >= (g + 1) * size) continue;  // uniform
+            const int e = j * 32 + lane;
+            const unsigned long long k = e >= g * size && e < (g + 1) * size && c[j] > -INFINITY ? key_of(c[j]) : 0ull;
+            m2 = max(m2, min(m1, k));
+            m1 = max(m1, k);
+        }
+        const unsigned long long a = warp_max_key(m1);
+        const int holder = __ffs(__ballot_sync(kFull, m1 == a)) - 1;
+        const unsigned long long b = p.group_best == 2 ? warp_max_key(lane == holder ? m2 : m1) : 0ull;
+        if (lane == g) { g1 = a; g2 = b; }
+    }
+    const double mine = g1 == 0 ? -INFINITY : g2 == 0 ? value_of(g1) : value_of(g1) + value_of(g2);
+    double gap, border;
+    return best_groups<double>(mine, p.groups, p.top_groups, lane, &gap, &border);
+}
+
+// The whole choice in 64 bits, taken where 32 cannot tell neighbours apart.  Returns the lane's slot's expert (-1: none).
+template <int VPL>
+__device__ __noinline__ int select_in_double(const RouteParams &p, const float *row, int lane, uint32_t keep) {
+    double c[VPL];
+    choices_in_double<VPL>(p, row, lane, c);
     if (p.groups > 1) {
         const int size = p.experts / p.groups;
-        double mine = -INFINITY;
-        for (int g = 0; g < p.groups; g++) {
-            double m1 = -INFINITY, m2 = -INFINITY;
-            for (int j = 0; j < VPL; j++) {
-                if ((j * 32 + lane) / size != g) continue;
-                if (c[j] > m1) { m2 = m1; m1 = c[j]; } else if (c[j] > m2) m2 = c[j];
-            }
-            const double a = warp_max_d(m1);
-            double t = a;
-            if (p.group_best == 2) {
-                const uint32_t at = __ballot_sync(kFull, m1 == a);
-                const double b = __popc(at) > 1 ? a : warp_max_d(m1 == a ? m2 : m1);
-                if (b > -INFINITY) t += b;
-            }
-            if (lane == g) mine = t;
-        }
-        double gap, border;
-        const uint32_t keep = best_groups<double>(mine, p.groups, p.top_groups, lane, &gap, &border);
         for (int j = 0; j < VPL; j++)
             if (j * 32 + lane < p.experts && !((keep >> ((j * 32 + lane) / size)) & 1)) c[j] = -INFINITY;
         if (p.score == FM_SCORE_SOFTMAX && p.bias == nullptr)  // within the groups the logits decide, as in the kernel
@@ -202,7 +243,7 @@ moe_route_kernel(const __grid_constant__ RouteParams p) {
             key[j] = x[j] > -INFINITY ? key_of(p.bias != nullptr ? s + __ldg(p.bias + min(j * 32 + lane, p.experts - 1)) : s) : 0u;
         }
     }
-    bool unsure = false;
+    uint32_t keep = 0;  // groups
 
     if (p.groups > 1) {
         const int size = p.experts / p.groups;
@@ -257,9 +298,9 @@ moe_route_kernel(const __grid_constant__ RouteParams p) {
             if (p.group_best == 2 && g2 != 0u) mine += score(g2);
         }
         float gap, border;
-        const uint32_t keep = best_groups<float>(mine, p.groups, p.top_groups, lane, &gap, &border);
-        if (!(by_logit && p.group_best == 1))
-            unsure = !(gap > (by_logit ? 1.6e-5f * border : 4.f * tol_score + 4.8e-7f * fabsf(border)));
+        keep = best_groups<float>(mine, p.groups, p.top_groups, lane, &gap, &border);
+        if (!(by_logit && p.group_best == 1) && !(gap > (by_logit ? 1.6e-5f * border : 4.f * tol_score + 4.8e-7f * fabsf(border))))
+            keep = groups_in_double<VPL>(p, row, lane);
         const uint32_t per = ((1u << 20) + size - 1) / size;  // e / size = e * per >> 20 for e < 1024
 #pragma unroll
         for (int j = 0; j < VPL; j++)
@@ -294,23 +335,21 @@ moe_route_kernel(const __grid_constant__ RouteParams p) {
     auto below = [&](uint32_t a, uint32_t b) {
         return value_of(a | kIndex) + (by_logit ? 0.f : 2.f * tol_score + 2.4e-7f * fabsf(value_of(a))) < value_of(b & ~kIndex);
     };
-    uint32_t mine = 0;
+    uint32_t mine = 0, last = 0, best = 0;
     int nc = 0;
-    if (!unsure) {
-        uint32_t last = 0, best = 0;
-        for (; nc < p.top_k; nc++) {
-            best = take();
-            if (best == 0u) break;
-            if (lane == nc) mine = best;
-            last = best;
-        }
-        while (best != 0u) {
-            best = take();
-            if (best == 0u || below(best, last)) break;
-            if (nc == 32) { unsure = true; break; }
-            if (lane == nc) mine = best;
-            nc++;
-        }
+    for (; nc < p.top_k; nc++) {
+        best = take();
+        if (best == 0u) break;
+        if (lane == nc) mine = best;
+        last = best;
+    }
+    bool unsure = false;
+    while (best != 0u) {
+        best = take();
+        if (best == 0u || below(best, last)) break;
+        if (nc == 32) { unsure = true; break; }
+        if (lane == nc) mine = best;
+        nc++;
     }
     // Their exact order, where two neighbours leave a doubt: logits as they are, choices in 64 bits (softmax with a bias: in 32,
     // where that decides).
@@ -346,7 +385,7 @@ moe_route_kernel(const __grid_constant__ RouteParams p) {
         }
     }
     if (unsure) {
-        id = select_in_double<VPL>(p, row, lane);
+        id = select_in_double<VPL>(p, row, lane, keep);
         rank = lane;
     }
     const bool chosen = id >= 0 && rank < p.top_k;
