@@ -70,6 +70,24 @@ def test_borders_that_fp32_cannot_decide(pkg, score):
 
 
 @pytest.mark.parametrize("score", [0, 1])
+@pytest.mark.parametrize("best", [1, 2])
+@pytest.mark.parametrize("experts,groups", [(256, 8), (512, 8), (256, 4), (1024, 32), (120, 5), (18, 6)])
+def test_groups_that_fp32_cannot_order(pkg, score, best, experts, groups):
+    """Rows whose groups' best choices lie closer than fp32 tells, beside ordinary ones; whole and part registers per group."""
+    rc = {**BASE, "num_experts": experts, "top_k": 3, "score": score, "num_groups": groups, "top_groups": groups // 2, "group_best": best}
+    rng = np.random.default_rng(experts + groups)
+    logits = rng.standard_normal((48, experts)).astype(np.float32)
+    tight = (2.0 + 1e-6 * rng.integers(-2, 3, size=(24, experts))).astype(np.float32)
+    logits[::2] = np.where(rng.random((24, experts)) < 0.3, tight, logits[::2] - 3.0)
+    logits[4:12, : experts // groups] = -np.inf  # a group without an expert
+    bias = (1e-7 * rng.standard_normal(experts)).astype(np.float32)
+    c = context(pkg)
+    for b in (None, bias):
+        check(run(pkg, c, rc, logits, b), moe_ref.route(logits, b, rc))
+    c.close()
+
+
+@pytest.mark.parametrize("score", [0, 1])
 @pytest.mark.parametrize("groups", [1, 4])
 def test_experts_that_are_not_available(pkg, score, groups):
     rc = {**BASE, "num_experts": 40, "top_k": 6, "score": score, "num_groups": groups, "top_groups": min(groups, 2), "group_best": 2, "shared_expert": 1}
