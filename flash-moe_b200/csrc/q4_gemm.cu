@@ -77,14 +77,13 @@ constexpr int kGemmSmem = kBSlots * kBSlot + kWSlots * kWSlot + kFSteps * 128 * 
 
 struct GemmMaps {
     CUtensorMap w[kMaxProj];  // words: [matrix][rows][K / 8] (kGateUp: 0 gate, 1 up)
-    CUtensorMap s[kMaxProj], b[kMaxProj];  // scales and biases [matrix][rows][K / 64], where GemmParams.wide
+    CUtensorMap s[kMaxProj], b[kMaxProj];  // scales and biases [matrix][rows][K / 64], where wide (groups a multiple of 8, 16-byte aligned)
     CUtensorMap x;            // fp16 [rows][hi | lo]
 };
 struct GemmParams {
     Q4Params p;
     int G, pseudo, units_per_job, kp;  // groups, blocks of 64 groups, row units, columns of one term of x
     int m_units[kMaxProj];             // kProj: row units of each matrix
-    int wide;                          // groups a multiple of 8, scales and biases 16-byte aligned
     const float *tscale;               // what a row of x has to be multiplied with
     int *err;
 };
@@ -272,7 +271,7 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
         }
     }
 }
-template <Q4Mode MODE>
+template <Q4Mode MODE, bool WIDE>
 __global__ void __launch_bounds__(kGemmThreads, 1)
 q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ GemmParams g) {
     extern __shared__ unsigned char smem_raw[];
@@ -394,7 +393,7 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
                         };
                         const int m = tile_mat<MODE>(un, i);
                         if (c < nreal) load(&maps.w[m], c * 32);
-                        else if (g.wide) {
+                        else if (WIDE) {
                             load(&maps.s[m], (c - nreal) * 64);
                             if (ok) load(&maps.b[m], (c - nreal) * 64);
                         }
@@ -518,7 +517,7 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
             for (int i = 0; i < T; i++) {
                 const int t = i < un.tiles ? i : 0;
                 sp[i] = row_ptr(un, t, r, false);
-                if (g.wide) sc[i] = chunk_scales(sp[i], 0);
+                if (WIDE) sc[i] = chunk_scales(sp[i], 0);
                 else {
                     sc[i] = window(un, t, 0);
                     sd[i] = window(un, t, 1);
@@ -538,9 +537,9 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
 #pragma unroll 1  // (one copy of the loop's body: the four roles' code has to fit the instruction cache)
                 for (int i = 0; i < un.tiles && ok; i++) {
                     uint2 s = i ? sc[1] : sc[0];
-                    if (!g.wide) s = cut8(s, i ? sd[1] : sd[0], (uint32_t)(uintptr_t)(i ? sp[1] : sp[0]) & 7u, na);
+                    if (!WIDE) s = cut8(s, i ? sd[1] : sd[0], (uint32_t)(uintptr_t)(i ? sp[1] : sp[0]) & 7u, na);
                     if (c + 1 < nreal) {  // (in place: a copy of the result would wait for it)
-                        if (g.wide) {
+                        if (WIDE) {
                             if (i) sc[1] = chunk_scales(sp[1], c + 1);
                             else sc[0] = chunk_scales(sp[0], c + 1);
                         } else if (i) {
@@ -595,7 +594,7 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
                     // b + 8 s of the row's groups; warps 0-3 take the first fp16 term, the others the second
                     float v[64];
                     uint32_t pw[32];
-                    if (g.wide) {  // both tiles came like weight tiles, 64 bf16 to a row
+                    if (WIDE) {  // both tiles came like weight tiles, 64 bf16 to a row
                         Ring<kWSlots> rs = rw;
                         ok = __all_sync(0xffffffffu, bar_wait(bar(BAR_W_FULL + rs.slot), rs.phase, abortp));
                         const uint32_t srow = sW + (uint32_t)rs.slot * kWSlot + (uint32_t)r * 128u;
@@ -665,7 +664,7 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
                     }
                     if (wg == 0) s_f[rf.slot * 128 + r] = pow2(127 + e - 135);
                     put(pw, i);
-                    for (int k = 0; k < (g.wide ? 2 : 0); k++) {
+                    for (int k = 0; k < (WIDE ? 2 : 0); k++) {
                         if (lane == 0) mbar_arrive(bar(BAR_W_EMPTY + rw.slot));
                         rw.next();
                     }
@@ -843,7 +842,7 @@ bool map_rows(CUtensorMap *m, const void *base, long long stride, int rows, int 
                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <Q4Mode MODE>
+template <Q4Mode MODE, bool WIDE>
 int launch_gemm(const GemmMaps &maps, GemmParams &g, long long jobs, int sm_count, cudaStream_t st) {
     constexpr int kRows = MODE == kGateUp ? T * 64 : T * 128;
     g.units_per_job = 0;
@@ -853,12 +852,12 @@ int launch_gemm(const GemmMaps &maps, GemmParams &g, long long jobs, int sm_coun
     }
     static unsigned long long configured = 0;
     if (first_use_on_device(&configured) &&
-        cudaFuncSetAttribute(q4_gemm_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem) != cudaSuccess)
+        cudaFuncSetAttribute(q4_gemm_kernel<MODE, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem) != cudaSuccess)
         return -1;
     // (fewer units than SMs: as many CTAs as there are units or, cut, tiles; idle ones would crowd the others onto half of the GPU)
     const long long units = jobs * g.units_per_job;
     const int grid = (int)std::min<long long>(MODE == kProj && 2 * units <= sm_count ? 2 * units : units, sm_count);
-    return launch_dependent(q4_gemm_kernel<MODE>, dim3(grid), dim3(kGemmThreads), kGemmSmem, st, maps, g) == cudaSuccess ? 1 : -1;
+    return launch_dependent(q4_gemm_kernel<MODE, WIDE>, dim3(grid), dim3(kGemmThreads), kGemmSmem, st, maps, g) == cudaSuccess ? 1 : -1;
 }
 
 }  // namespace
@@ -876,20 +875,20 @@ int launch_q4_gemm(Q4Mode mode, const Q4Params &p, const void *xs, int xs_rows, 
     GemmParams g = {};
     g.p = p; g.G = p.in_dim / 64; g.pseudo = (g.G + 63) / 64; g.kp = q4_split_columns(p.in_dim); g.tscale = tscale; g.err = err;
     const int matrices = mode == kProj ? 1 : p.num_experts;
-    g.wide = g.G % 8 == 0;
-    for (int i = 0; i < p.nmat; i++) g.wide = g.wide && (((uintptr_t)p.mat[i].scales | (uintptr_t)p.mat[i].biases) & 15) == 0;
+    bool wide = g.G % 8 == 0;  // scales and biases then start on 16 bytes in every row
+    for (int i = 0; i < p.nmat; i++) wide = wide && (((uintptr_t)p.mat[i].scales | (uintptr_t)p.mat[i].biases) & 15) == 0;
     for (int i = 0; i < p.nmat; i++) {
         const Q4View &m = p.mat[i];
         if (!map_rows(&maps.w[i], m.w, m.w_stride, m.rows, p.in_dim / 2, matrices, true)) return -1;
-        if (g.wide && (!map_rows(&maps.s[i], m.scales, m.s_stride, m.rows, g.G * 2, matrices, false) ||
+        if (wide && (!map_rows(&maps.s[i], m.scales, m.s_stride, m.rows, g.G * 2, matrices, false) ||
                        !map_rows(&maps.b[i], m.biases, m.s_stride, m.rows, g.G * 2, matrices, false)))
             return -1;
     }
     if (!make_map_2d(&maps.x, xs, (uint64_t)xs_rows, (uint64_t)2 * g.kp, 16, false)) return -1;
     const long long jobs = mode == kProj ? (p.n + kTok - 1) / kTok : (long long)p.n * p.top_k;
-    if (mode == kProj) return launch_gemm<kProj>(maps, g, jobs, sm_count, st);
-    if (mode == kGateUp) return launch_gemm<kGateUp>(maps, g, jobs, sm_count, st);
-    return launch_gemm<kDown>(maps, g, jobs, sm_count, st);
+    if (mode == kProj) return wide ? launch_gemm<kProj, true>(maps, g, jobs, sm_count, st) : launch_gemm<kProj, false>(maps, g, jobs, sm_count, st);
+    if (mode == kGateUp) return wide ? launch_gemm<kGateUp, true>(maps, g, jobs, sm_count, st) : launch_gemm<kGateUp, false>(maps, g, jobs, sm_count, st);
+    return wide ? launch_gemm<kDown, true>(maps, g, jobs, sm_count, st) : launch_gemm<kDown, false>(maps, g, jobs, sm_count, st);
 }
 
 }  // namespace fm
