@@ -270,3 +270,25 @@ def test_total_experts_changes_the_choice_and_not_the_answer(pkg):
         counts.append(count)
     assert counts == [6, 4]
     c.close()
+
+
+@pytest.mark.parametrize("many,n,out", [(1, 1, 33), (1, 8, 33), (1, 17, 33), (2, 600, 330)])
+def test_projection_of_the_longest_input(pkg, many, n, out):
+    rng = np.random.default_rng(600 + n)
+    c = context(pkg, max_batch=1024)
+    m = moe_ref.weights(rng, out, 65536)
+    x = rng.standard_normal((n, 65536)).astype(np.float32)
+    count, got = launches(c, lambda: run_proj(pkg, c, [m], x)[0])
+    assert count == many
+    moe_ref.close(got, *moe_ref.product(x, m))
+    c.close()
+
+
+@pytest.mark.parametrize("n,hidden,inter", [(2, 65536, 64), (2, 64, 65536), (40, 65536, 64), (40, 64, 65536), (900, 8192, 64), (900, 64, 8192)])
+def test_experts_of_the_longest_rows(pkg, n, hidden, inter):
+    rng = np.random.default_rng(610 + n)
+    c = context(pkg, max_batch=1024)
+    m = stacks(rng, 2, hidden, inter)
+    x, res, ids, w, nw = inputs(rng, n, hidden, 2, 2)
+    check(run_experts(pkg, c, device_stacks(pkg, m), x, ids, w, res, nw), m, x, ids, w, res, nw)
+    c.close()
