@@ -28,8 +28,8 @@
 // and the MMA's start-up counts more, at 128 the steps could not be double-buffered.
 //
 // Measured (B200, 1.9 GHz; the tensor work is twice the product's, because of the two terms): 4096 tokens x 4096 x 8192 in
-// 520 us, 530 TFLOP/s of products (the tensor core is busy 73 % of the time in MMAs of 57 cycles, ideal 48); 300 tokens through
-// qkv + z + beta + alpha of 4096 in 130 us; 4096 tokens through 10 of 512 experts of 4096 x 1024: gate / up 1.8 ms, down 1.0 ms.
+// 514 us, 535 TFLOP/s of products (the tensor core is busy 73 % of the time in MMAs of 57 cycles, ideal 48); 300 tokens through
+// qkv + z + beta + alpha of 4096 in 120 us; 4096 tokens through 10 of 512 experts of 4096 x 1024: gate / up 1.72 ms, down 0.96 ms.
 // What bounds it: the issue slots.  Widening, the epilogue and the hand-overs between the roles take 2000 to 2300 instructions
 // per operand slot of 915 tensor cycles; below 64 tokens a unit takes about 950 cycles per slot whatever its tokens.
 // Tried and not kept: 16 widening warps (the same time), the two issuing warps as one (+10 %), operand slots of one group
