@@ -1,4 +1,4 @@
-"""The 64-bit reference of the mixture-of-experts tests against the CPU checker, and the structs' ctypes mirrors (no GPU)."""
+"""The 64-bit reference of the mixture-of-experts tests against the CPU oracle, and the structs' ctypes mirrors (no GPU)."""
 import re
 from pathlib import Path
 
@@ -9,7 +9,7 @@ import moe_ref
 ROOT = Path(__file__).resolve().parents[1]
 
 
-def test_product_is_the_checkers(port):
+def test_product_is_the_oracles(port):
     rng = np.random.default_rng(0)
     m = moe_ref.weights(rng, 40, 512)
     x = rng.standard_normal((3, 512)).astype(np.float32)
