@@ -163,14 +163,19 @@ __device__ __noinline__ uint32_t groups_in_double(const RouteParams &p, const fl
 template <int VPL>
 __device__ __noinline__ int select_in_double(const RouteParams &p, const float *row, int lane, uint32_t keep) {
     double c[VPL];
-    choices_in_double<VPL>(p, row, lane, c);
+    if (p.score == FM_SCORE_SOFTMAX && p.bias == nullptr) {  // the logits decide, as in the kernel: scores underflow, or round to one value
+#pragma unroll(kDoubleUnroll<VPL>)
+        for (int j = 0; j < VPL; j++) {
+            const float x = j * 32 + lane < p.experts ? row[j * 32 + lane] : -INFINITY;
+            c[j] = x > -INFINITY ? (double)x : -INFINITY;
+        }
+    } else {
+        choices_in_double<VPL>(p, row, lane, c);
+    }
     if (p.groups > 1) {
         const int size = p.experts / p.groups;
         for (int j = 0; j < VPL; j++)
             if (j * 32 + lane < p.experts && !((keep >> ((j * 32 + lane) / size)) & 1)) c[j] = -INFINITY;
-        if (p.score == FM_SCORE_SOFTMAX && p.bias == nullptr)  // within the groups the logits decide, as in the kernel
-            for (int j = 0; j < VPL; j++)
-                if (c[j] > -INFINITY) c[j] = (double)row[j * 32 + lane];
     }
     int id = -1;
     for (int s = 0; s < p.top_k; s++) {

@@ -87,6 +87,37 @@ def test_groups_that_fp32_cannot_order(pkg, score, best, experts, groups):
     c.close()
 
 
+def rows_of_close_logits_far_below_the_best(rng, experts):
+    """More than 32 logits that share all but the last bits, beside larger ones whose distance leaves them without a score."""
+    up = np.arange(experts) * 2.0 ** -23
+    rows = np.zeros((8, experts), np.float32)
+    rows[0] = 1.0 + up; rows[0, 0] = 1000.0
+    rows[1] = 1.0 + up; rows[1, 3] = np.inf
+    rows[2] = 1.0 + up[rng.permutation(experts)]; rows[2, experts // 2] = 800.0
+    rows[3] = np.arange(experts) * 2.0 ** -149; rows[3, 1] = 1.0   # numbers that are lost beside the largest
+    for row, mask in ((4, -1e4), (5, -1e5), (6, -3e38)):            # a mask that is added and finite, few experts without it
+        rows[row] = rng.standard_normal(experts) + (mask if row < 6 else 0)
+        rows[row] = rows[row] if row < 6 else mask
+        free = rng.permutation(experts)[:2]
+        rows[row, free] = rng.standard_normal(2)
+    rows[7] = -2000.0 + up; rows[7, :5] = np.nan; rows[7, 9] = 0.0
+    return rows
+
+
+@pytest.mark.parametrize("groups", [1, 4])
+@pytest.mark.parametrize("experts", [64, 256, 512, 1024])
+def test_softmax_without_a_bias_goes_by_the_logits(pkg, experts, groups):
+    """However far below the largest logit the border lies: there are no ties by underflow."""
+    rng = np.random.default_rng(experts + groups)
+    logits = rows_of_close_logits_far_below_the_best(rng, experts)
+    c = context(pkg)
+    for top in (3, 10, 32 if experts > 64 else 16):
+        for renorm in (0, 1):
+            rc = {**BASE, "num_experts": experts, "top_k": top, "num_groups": groups, "top_groups": max(1, groups - 1), "renormalize": renorm}
+            check(run(pkg, c, rc, logits), moe_ref.route(logits, None, rc))
+    c.close()
+
+
 @pytest.mark.parametrize("score", [0, 1])
 @pytest.mark.parametrize("groups", [1, 4])
 def test_experts_that_are_not_available(pkg, score, groups):
