@@ -293,18 +293,26 @@ moe_route_kernel(const __grid_constant__ RouteParams p) {
         }
         // lane g: the total of group g.  by_logit: the group's best scores are those of its best logits; of one best, compare the
         // logits themselves
-        float mine = -INFINITY;
+        float mine = -INFINITY, size_of = 0.f;  // (size_of: what the total's roundings are relative to)
         if (lane < p.groups && g1 != 0u) {
             auto score = [&](uint32_t k) {
                 const float v = value_of(k);
                 return by_logit && p.group_best == 2 ? (v == m ? 1.f : expf(v - m)) * inv : v;
             };
             mine = score(g1);
-            if (p.group_best == 2 && g2 != 0u) mine += score(g2);
+            size_of = fabsf(mine);
+            if (p.group_best == 2 && g2 != 0u) {
+                const float second = score(g2);
+                mine += second;
+                size_of += fabsf(second);
+            }
         }
         float gap, border;
         keep = best_groups<float>(mine, p.groups, p.top_groups, lane, &gap, &border);
-        if (!(by_logit && p.group_best == 1) && !(gap > (by_logit ? 1.6e-5f * border : 4.f * tol_score + 4.8e-7f * fabsf(border))))
+        // Two choices of a group may cancel, so their roundings are taken from their sizes, the largest of any group.  Scores alone
+        // (by_logit) do not cancel.
+        const float largest = __uint_as_float(__reduce_max_sync(kFull, __float_as_uint(size_of)));
+        if (!(by_logit && p.group_best == 1) && !(gap > (by_logit ? 1.6e-5f * border : 4.f * tol_score + 4.8e-7f * largest)))
             keep = groups_in_double<VPL>(p, row, lane);
         const uint32_t per = ((1u << 20) + size - 1) / size;  // e / size = e * per >> 20 for e < 1024
 #pragma unroll

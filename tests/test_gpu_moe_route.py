@@ -119,6 +119,20 @@ def test_softmax_without_a_bias_goes_by_the_logits(pkg, experts, groups):
 
 
 @pytest.mark.parametrize("score", [0, 1])
+@pytest.mark.parametrize("experts,groups", [(32, 4), (256, 8), (512, 8), (60, 6)])
+def test_groups_whose_choices_cancel(pkg, score, experts, groups):
+    """A group's best two add up to about 1 while each is a thousand: their roundings are those of the thousands."""
+    rc = {**BASE, "num_experts": experts, "top_k": 2, "score": score, "num_groups": groups, "top_groups": groups // 2, "group_best": 2}
+    rng = np.random.default_rng(experts + score)
+    logits = (1e-3 * rng.standard_normal((64, experts))).astype(np.float32)
+    bias = np.full(experts, -1000.0, np.float32)
+    bias[:: experts // groups] = 1000.0
+    c = context(pkg)
+    check(run(pkg, c, rc, logits, bias), moe_ref.route(logits, bias, rc))
+    c.close()
+
+
+@pytest.mark.parametrize("score", [0, 1])
 @pytest.mark.parametrize("groups", [1, 4])
 def test_experts_that_are_not_available(pkg, score, groups):
     rc = {**BASE, "num_experts": 40, "top_k": 6, "score": score, "num_groups": groups, "top_groups": min(groups, 2), "group_best": 2, "shared_expert": 1}
