@@ -310,9 +310,9 @@ moe_route_kernel(const __grid_constant__ RouteParams p) {
         float gap, border;
         keep = best_groups<float>(mine, p.groups, p.top_groups, lane, &gap, &border);
         // Two choices of a group may cancel, so their roundings are taken from their sizes, the largest of any group.  Scores alone
-        // (by_logit) do not cancel.
+        // (by_logit) do not cancel; below fp32's normal numbers their rounding is absolute.
         const float largest = __uint_as_float(__reduce_max_sync(kFull, __float_as_uint(size_of)));
-        if (!(by_logit && p.group_best == 1) && !(gap > (by_logit ? 1.6e-5f * border : 4.f * tol_score + 4.8e-7f * largest)))
+        if (!(by_logit && p.group_best == 1) && !(gap > (by_logit ? 1.6e-5f * border + 1.2e-38f : 4.f * tol_score + 4.8e-7f * largest)))
             keep = groups_in_double<VPL>(p, row, lane);
         const uint32_t per = ((1u << 20) + size - 1) / size;  // e / size = e * per >> 20 for e < 1024
 #pragma unroll

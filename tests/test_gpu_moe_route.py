@@ -132,6 +132,19 @@ def test_groups_whose_choices_cancel(pkg, score, experts, groups):
     c.close()
 
 
+@pytest.mark.parametrize("experts,groups", [(32, 4), (256, 8), (512, 8), (60, 6)])
+def test_groups_whose_scores_are_subnormal(pkg, experts, groups):
+    """Two experts of one group hold all of the weight, the others' scores are a few of fp32's smallest steps."""
+    rc = {**BASE, "num_experts": experts, "top_k": 6, "num_groups": groups, "top_groups": 2, "group_best": 2}
+    rng = np.random.default_rng(experts)
+    logits = (-99.0 + 0.05 * rng.standard_normal((64, experts))).astype(np.float32)
+    logits[:, :2] += 99.0
+    logits[:, 2: experts // groups] = -np.inf
+    c = context(pkg)
+    check(run(pkg, c, rc, logits), moe_ref.route(logits, None, rc))
+    c.close()
+
+
 @pytest.mark.parametrize("score", [0, 1])
 @pytest.mark.parametrize("groups", [1, 4])
 def test_experts_that_are_not_available(pkg, score, groups):
