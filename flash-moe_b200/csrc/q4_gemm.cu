@@ -6,8 +6,9 @@
 // with X[t][g] the sum of the group's 64 inputs.
 //
 // Exactness.  A scale is bf16 (8 bits) and |nibble - 8| is 8 or has 3 bits, so s * (nibble - 8) has 11 bits at most: it
-// IS an fp16 number, once a power of two per row and 256 inputs has brought the scales into range (those below 1/256 of
-// the largest keep an absolute error of 2^-18 of its weights).  An activation enters
+// IS an fp16 number, once a power of two per row and 256 inputs has brought the scales into range.  Scales down to 1/128 of the
+// largest of their 256 inputs take one multiply-add; where a warp has smaller ones, a second multiplication takes them in down to
+// 2^-23, and what lies below keeps an absolute error of 2^-31 of the largest per weight.  An activation enters
 // as two fp16 terms, hi + lo (22 bits, a power of two per token).  The second sum is one more block of 64 columns, per 64
 // groups, with both factors in two terms.  The tensor cores add into fp32 by truncation, which shrinks a long sum by a
 // few 2^-24 per addition; so TMEM accumulates over 256 inputs only, and the parts are added in fp32 by the epilogue
@@ -209,10 +210,26 @@ __device__ __forceinline__ uint4 cut16(uint4 a, uint4 b, uint32_t by) {
     const uint32_t w0 = q ? t1 : t0, w1 = q ? t2 : t1, w2 = q ? t3 : t2, w3 = q ? t4 : t3, w4 = q ? t5 : t4, s = (by & 2) * 8;
     return make_uint4(__funnelshift_r(w0, w1, s), __funnelshift_r(w1, w2, s), __funnelshift_r(w2, w3, s), __funnelshift_r(w3, w4, s));
 }
-// Exponent field of the largest of them, kept where the powers of two made of it are normal numbers.
-__device__ __forceinline__ int chunk_exponent(uint2 v) {
-    const uint32_t a = max(v.x & 0x7fff0000u, v.x << 16 & 0x7fff0000u), b = max(v.y & 0x7fff0000u, v.y << 16 & 0x7fff0000u);
-    return min(max((int)(max(a, b) >> 23), 16), 244);
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("max.u16x2 %0, %1, %2;\n" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ uint32_t min_u16x2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("min.u16x2 %0, %1, %2;\n" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+// Exponent field of a chunk's largest scale, kept where the powers of two made of it are normal numbers; *far: whether one of
+// the four lies below 1/128 of it.  Looking for those costs ordinary matrices 1 % (4096 tokens x 4096 x 8192) to 2 % (4096 tokens
+// through 10 of 512 experts); a branch around the whole of the widening cost the experts 3 %.
+__device__ __forceinline__ int chunk_exponent(uint2 v, bool *far) {
+    const uint32_t a = v.x & 0x7fff7fffu, b = v.y & 0x7fff7fffu;
+    uint32_t hi = max_u16x2(a, b), lo = min_u16x2(a, b);
+    hi = max(max_u16x2(hi, __byte_perm(hi, 0, 0x1032)), 0x08000800u);  // the same in both halves from here on
+    lo = min_u16x2(lo, __byte_perm(lo, 0, 0x1032));
+    *far = (int)(hi - lo) > 0x03800380;
+    return min((int)(hi >> 23), 244);
 }
 __device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
     uint4 v;
@@ -224,7 +241,9 @@ __device__ __forceinline__ uint32_t h2_bits(__half2 v) { return *reinterpret_cas
 
 // (n_q - 8, n_{q+4} - 8) * m * 2^-24 for q = 0..3 of a weight word.  A nibble in the low bits of a half is the subnormal
 // fp16 number n * 2^-24 (16 n * 2^-24 one nibble up), so one fused multiply-add takes the 8 off and the scale on, exactly: m
-// is the scale as an integer below 2^15 with 8 bits.
+// is the scale as an integer below 2^15 with 8 bits.  A scale below 1/128 of its chunk's largest has less than 8 bits left as
+// such an integer.  Where a warp has one, m is 2^15 for all of them, which leaves (n - 8) * 2^-9, and a second multiplication
+// takes the scale on.
 __device__ __forceinline__ uint32_t fma_h2(uint32_t a, uint32_t b, uint32_t c) {
     uint32_t d;
     asm("fma.rn.f16x2 %0, %1, %2, %3;\n" : "=r"(d) : "r"(a), "r"(b), "r"(c));
@@ -236,6 +255,11 @@ __device__ __forceinline__ void widen_word(uint32_t w, uint32_t m, uint32_t m16,
     out[1] = fma_h2(w & 0x00F000F0u, m16, c);
     out[2] = fma_h2(v & 0x000F000Fu, m, c);
     out[3] = fma_h2(v & 0x00F000F0u, m16, c);
+}
+__device__ __forceinline__ uint32_t mul_h2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("mul.rn.f16x2 %0, %1, %2;\n" : "=r"(d) : "r"(a), "r"(b));
+    return d;
 }
 // x as fp16 in both halves
 __device__ __forceinline__ uint32_t dup_h2(float x) {
@@ -550,10 +574,12 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
                             sd[0] = window(un, 0, c + 2);
                         }
                     }
-                    const int e = chunk_exponent(s);
+                    bool far;
+                    const int e = chunk_exponent(s, &far);
+                    far = __any_sync(0xffffffffu, far);  // (both groups of warps see the scales of the same rows, so they agree)
                     const float up = pow2(127 + 141 - e);  // the largest scale comes to [2^14, 2^15)
                     // for the epilogue: what the step's sums have to be multiplied with (seen through A_FULL, the MMAs and D_FULL)
-                    if (wg == 0) s_f[rf.slot * 128 + r] = pow2(127 + e - 141 + 24);
+                    if (wg == 0) s_f[rf.slot * 128 + r] = pow2(127 + e - 141 + (far ? 8 : 24));
                     ok = __all_sync(0xffffffffu, bar_wait(bar(BAR_W_FULL + rw.slot), rw.phase, abortp));
                     if (!ok) break;
                     const uint32_t tile = sW + (uint32_t)rw.slot * kWSlot;
@@ -564,7 +590,8 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
                         const uint4 w0 = ws[q][0], w1 = ws[q][1];
                         const uint32_t bits = q ? s.y : s.x;
                         const float mf = __uint_as_float(wg ? bits & 0xffff0000u : bits << 16) * up;
-                        const uint32_t m = dup_h2(mf), m16 = dup_h2(mf * 0.0625f), mc = dup_h2(mf * -0x1p-21f);
+                        const float mq = far ? 0x1p15f : mf;
+                        const uint32_t m = dup_h2(mq), m16 = dup_h2(mq * 0.0625f), mc = dup_h2(mq * -0x1p-21f);
                         uint32_t a[32];
                         widen_word(w0.x, m, m16, mc, a);
                         widen_word(w0.y, m, m16, mc, a + 4);
@@ -574,6 +601,11 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
                         widen_word(w1.y, m, m16, mc, a + 20);
                         widen_word(w1.z, m, m16, mc, a + 24);
                         widen_word(w1.w, m, m16, mc, a + 28);
+                        if (far) {
+                            const uint32_t mh = dup_h2(mf + mf);
+#pragma unroll
+                            for (int k = 0; k < 32; k++) a[k] = mul_h2(a[k], mh);
+                        }
                         put(a, i);
                     }
                     if (lane == 0) mbar_arrive(bar(BAR_W_EMPTY + rw.slot));  // (the last put brought the warp together)

@@ -12,6 +12,15 @@ def weights(rng, out_dim, in_dim, lead=()):
     return w, scales, biases
 
 
+def spread(rng, mat, ratio):
+    """The matrix with three of every four groups of 64 inputs scaled down by `ratio` (some of those to nothing but a bias)."""
+    w, scales, biases = mat
+    small = np.arange(scales.shape[-1]) % 4 != 1
+    s, b = (np.where(small, f32(a) * ratio, f32(a)) for a in (scales, biases))
+    s[..., small] *= rng.random(s[..., small].shape) > 0.1
+    return w, bf16(s), bf16(b)
+
+
 def bf16(x):
     u = np.ascontiguousarray(x, np.float32).view(np.uint32).astype(np.uint64)
     return ((u + 0x7FFF + ((u >> 16) & 1)) >> 16).astype(np.uint16)

@@ -46,6 +46,43 @@ def test_projection_inputs_of_every_size(pkg, many, n, k, out):
     c.close()
 
 
+WIDE_AND_NOT = [(1, 8, 1024, 48), (1, 40, 1024, 48), (2, 300, 1024, 1000), (2, 300, 832, 1000)]  # launches, tokens, inputs, outputs
+RATIOS = [1e-2, 1e-3, 1e-4, 2.0 ** -7, 2.0 ** -8, 2.0 ** -12, 2.0 ** -16, 2.0 ** -20]
+
+
+@pytest.mark.parametrize("ratio", RATIOS)
+@pytest.mark.parametrize("many,n,k,out", WIDE_AND_NOT)
+def test_groups_whose_scales_lie_far_apart(pkg, many, n, k, out, ratio):
+    """Every group keeps its weights, however small its scale is beside its neighbours': with inputs of one size, with none but
+    in the groups of small scales, and with inputs that make up for the scales."""
+    rng = np.random.default_rng(620 + n + k)
+    c = context(pkg, max_batch=512)
+    m = moe_ref.spread(rng, moe_ref.weights(rng, out, k), ratio)
+    big = np.repeat(np.arange(k // 64) % 4 == 1, 64)
+    x = rng.standard_normal((n, k)).astype(np.float32)
+    for xs in (x, np.where(big, 0, x), np.where(big, x * 64 * ratio, x)):
+        xs = xs.astype(np.float32)
+        count, got = launches(c, lambda: run_proj(pkg, c, [m], xs)[0])
+        assert count == many
+        moe_ref.close(got, *moe_ref.product(xs, m))
+    c.close()
+
+
+@pytest.mark.parametrize("ratio", [1e-3, 2.0 ** -20])
+@pytest.mark.parametrize("many,n,hidden,inter", EXPERTS)
+def test_experts_whose_scales_lie_far_apart(pkg, many, n, hidden, inter, ratio):
+    rng = np.random.default_rng(640 + n)
+    c = context(pkg, max_batch=1024)
+    m = [moe_ref.spread(rng, a, ratio) for a in stacks(rng, 6, hidden, inter)]
+    x, res, ids, w, nw = inputs(rng, n, hidden, 6, 3)
+    x[:, np.repeat(np.arange(hidden // 64) % 4 == 1, 64)] = 0.0
+    x /= np.float32(ratio)  # gate and up come out as large as usual
+    count, got = launches(c, lambda: run_experts(pkg, c, device_stacks(pkg, m), x, ids, w, None, nw))
+    assert count == many
+    check(got, m, x, ids, w, None, nw)
+    c.close()
+
+
 @pytest.mark.parametrize("many,n,k,out", PROJ)
 def test_projection_host_pointers_and_bits(pkg, many, n, k, out):
     """Host pointers give the bits that device pointers give, and equal tokens of a call equal rows."""
