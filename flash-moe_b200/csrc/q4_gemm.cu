@@ -10,7 +10,9 @@
 // largest of their 256 inputs take one multiply-add; where a warp has smaller ones, a second multiplication takes them in down to
 // 2^-23, and what lies below keeps an absolute error of 2^-31 of the largest per weight.  An activation enters
 // as two fp16 terms, hi + lo (22 bits, a power of two per token).  The second sum is one more block of 64 columns, per 64
-// groups, with both factors in two terms.  The tensor cores add into fp32 by truncation, which shrinks a long sum by a
+// groups, with both factors in two terms: b + 8 s keeps 22 bits down to 2^-16 of the largest of its row's 64, below that an
+// absolute error of 2^-39 of it.  (b and 8 s by themselves would be exact further down, but that block needs both at once, and the
+// registers it spilled cost the experts 2 %.)  The tensor cores add into fp32 by truncation, which shrinks a long sum by a
 // few 2^-24 per addition; so TMEM accumulates over 256 inputs only, and the parts are added in fp32 by the epilogue
 // warps, which apply the row's power of two in the same fused multiply-add.
 //
@@ -686,7 +688,7 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
 #pragma unroll
                     for (int q = 0; q < 64; q++) m = fmaxf(m, fabsf(v[q]));
                     const int e = max((int)(__float_as_uint(m) >> 23), 16);
-                    const float up = pow2(127 + 135 - e);
+                    const float up = pow2(127 + 141 - e);  // the largest comes to [2^14, 2^15): as far up as fp16 goes
 #pragma unroll
                     for (int q = 0; q < 32; q++) {
                         const float a0 = v[2 * q] * up, a1 = v[2 * q + 1] * up;
@@ -694,7 +696,7 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
                         const float2 hf = __half22float2(h);
                         pw[q] = h2_bits(wg == 0 ? h : __floats2half2_rn(a0 - hf.x, a1 - hf.y));
                     }
-                    if (wg == 0) s_f[rf.slot * 128 + r] = pow2(127 + e - 135);
+                    if (wg == 0) s_f[rf.slot * 128 + r] = pow2(127 + e - 141);
                     put(pw, i);
                     for (int k = 0; k < (WIDE ? 2 : 0); k++) {
                         if (lane == 0) mbar_arrive(bar(BAR_W_EMPTY + rw.slot));

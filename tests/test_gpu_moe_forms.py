@@ -68,6 +68,23 @@ def test_groups_whose_scales_lie_far_apart(pkg, many, n, k, out, ratio):
     c.close()
 
 
+@pytest.mark.parametrize("ratio", [2.0 ** -20, 2.0 ** -24, 2.0 ** -28])
+@pytest.mark.parametrize("many,n,k,out", [(1, 8, 4096, 48), (2, 300, 4096, 1000), (2, 300, 4160, 1000)])
+def test_rows_whose_biases_lie_far_apart(pkg, many, n, k, out, ratio):
+    """Every other 256 inputs have small scales and biases, and only those have inputs, all of one sign: the biases' share is
+    what it takes the share of the nibbles to cancel."""
+    rng = np.random.default_rng(660 + n + k)
+    c = context(pkg, max_batch=512)
+    w, s, b = moe_ref.weights(rng, out, k)
+    small = np.arange(k // 64) // 4 % 2 == 1
+    m = (w, *(moe_ref.bf16(np.where(small, moe_ref.f32(a) * ratio, moe_ref.f32(a))) for a in (s, b)))
+    x = np.where(np.repeat(small, 64), np.abs(rng.standard_normal((n, k))), 0).astype(np.float32)
+    count, got = launches(c, lambda: run_proj(pkg, c, [m], x)[0])
+    assert count == many
+    moe_ref.close(got, *moe_ref.product(x, m))
+    c.close()
+
+
 @pytest.mark.parametrize("ratio", [1e-3, 2.0 ** -20])
 @pytest.mark.parametrize("many,n,hidden,inter", EXPERTS)
 def test_experts_whose_scales_lie_far_apart(pkg, many, n, hidden, inter, ratio):
