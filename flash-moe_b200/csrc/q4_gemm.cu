@@ -9,10 +9,11 @@
 // IS an fp16 number, once a power of two per row and 256 inputs has brought the scales into range.  Scales down to 1/128 of the
 // largest of their 256 inputs take one multiply-add; where a warp has smaller ones, a second multiplication takes them in down to
 // 2^-23, and what lies below keeps an absolute error of 2^-31 of the largest per weight.  An activation enters
-// as two fp16 terms, hi + lo (22 bits, a power of two per token).  The second sum is one more block of 64 columns, per 64
-// groups, with both factors in two terms: b + 8 s keeps 22 bits down to 2^-16 of the largest of its row's 64, below that an
-// absolute error of 2^-39 of it.  (b and 8 s by themselves would be exact further down, but that block needs both at once, and the
-// registers it spilled cost the experts 2 %.)  The tensor cores add into fp32 by truncation, which shrinks a long sum by a
+// as two fp16 terms, hi + lo, under a power of two per token: 22 bits down to 2^-16 of the token's largest, below that an absolute
+// error of 2^-39 of it (a sum X: 2^-33).  The second sum is one more block of 64 columns, per 64 groups, with both factors in two
+// terms: b + 8 s keeps 22 bits down to 2^-16 of the largest of its row's 64, below that an absolute error of 2^-39 of it.  (b and
+// 8 s by themselves would be exact further down, but that block needs both at once, and the registers it spilled cost the experts
+// 2 %.)  The tensor cores add into fp32 by truncation, which shrinks a long sum by a
 // few 2^-24 per addition; so TMEM accumulates over 256 inputs only, and the parts are added in fp32 by the epilogue
 // warps, which apply the row's power of two in the same fused multiply-add.
 //
@@ -62,6 +63,7 @@ constexpr int kWSlot = 128 * 128;           // bytes of a weight tile: 128 rows,
 constexpr int kWSlots = 4;
 constexpr int kGemmThreads = 20 * 32;
 constexpr int T = 2;                        // row tiles of a unit
+constexpr float kSumScale = 0x1p-6f;        // of the stored sums of 64 inputs
 constexpr int kDBufs = T;                   // steps in flight: one per tile
 // Steps whose row factors are kept: the widening warps are at most the operand slots (one to a step at the least), the
 // steps in flight and their own step ahead of the epilogue.
@@ -696,7 +698,7 @@ q4_gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ Ge
                         const float2 hf = __half22float2(h);
                         pw[q] = h2_bits(wg == 0 ? h : __floats2half2_rn(a0 - hf.x, a1 - hf.y));
                     }
-                    if (wg == 0) s_f[rf.slot * 128 + r] = pow2(127 + e - 141);
+                    if (wg == 0) s_f[rf.slot * 128 + r] = pow2(127 + e - 141) / kSumScale;
                     put(pw, i);
                     for (int k = 0; k < (WIDE ? 2 : 0); k++) {
                         if (lane == 0) mbar_arrive(bar(BAR_W_EMPTY + rw.slot));
@@ -825,11 +827,12 @@ q4_split_kernel(const float *__restrict__ x, int K, int kp, const int *count, co
 #pragma unroll
     for (int w = 0; w < 8; w++) { am = fmaxf(am, s_red[w]); sum += s_sum[w]; }
     const bool bad = !(sum == 0.f);
-    // am in [2^e, 2^(e+1)) becomes [2^8, 2^9): the sum of 64 inputs stays below fp16's largest number
+    // am in [2^e, 2^(e+1)) becomes [2^14, 2^15), as far up as fp16 goes, so that small inputs beside it keep their bits; the sums of
+    // 64 inputs are stored 2^-6 times as large, which the widening warps make up for
     int e = max((int)(__float_as_uint(am) >> 23), 16);
-    if (bad) e = 135;
-    const float up = __uint_as_float((uint32_t)(127 + 135 - e) << 23);
-    if (tid == 0) tscale[row] = bad ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)(127 + e - 135) << 23);
+    if (bad) e = 141;
+    const float up = __uint_as_float((uint32_t)(127 + 141 - e) << 23);
+    if (tid == 0) tscale[row] = bad ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)(127 + e - 141) << 23);
     __half *hi = xs + row * 2 * kp, *lo = hi + kp;
     const int G = K / 64;
     for (int i0 = 0; i0 < K / 8; i0 += 256) {  // eight inputs per thread; the eight threads of a group are neighbours
@@ -851,6 +854,7 @@ q4_split_kernel(const float *__restrict__ x, int K, int kp, const int *count, co
         float s = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
 #pragma unroll
         for (int o = 1; o < 8; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        s *= kSumScale;
         if (valid) {
             *reinterpret_cast<uint4 *>(hi + 8 * i) = make_uint4(h[0], h[1], h[2], h[3]);
             *reinterpret_cast<uint4 *>(lo + 8 * i) = make_uint4(l[0], l[1], l[2], l[3]);

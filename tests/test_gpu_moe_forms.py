@@ -85,6 +85,22 @@ def test_rows_whose_biases_lie_far_apart(pkg, many, n, k, out, ratio):
     c.close()
 
 
+@pytest.mark.parametrize("ratio", [2.0 ** -12, 2.0 ** -16, 2.0 ** -20, 2.0 ** -22])
+@pytest.mark.parametrize("many,n,k,out", WIDE_AND_NOT)
+def test_small_inputs_beside_large_ones_without_weight(pkg, many, n, k, out, ratio):
+    """Inputs that lie `ratio` below their token's largest, where the large ones meet weights of zero."""
+    rng = np.random.default_rng(680 + n + k)
+    c = context(pkg, max_batch=512)
+    w, s, b = moe_ref.weights(rng, out, k)
+    large = np.arange(k // 64) % 4 == 2
+    m = (w, np.where(large, 0, s).astype(np.uint16), np.where(large, 0, b).astype(np.uint16))
+    x = (rng.standard_normal((n, k)) * np.where(np.repeat(large, 64), 1, ratio)).astype(np.float32)
+    count, got = launches(c, lambda: run_proj(pkg, c, [m], x)[0])
+    assert count == many
+    moe_ref.close(got, *moe_ref.product(x, m))
+    c.close()
+
+
 @pytest.mark.parametrize("ratio", [1e-3, 2.0 ** -20])
 @pytest.mark.parametrize("many,n,hidden,inter", EXPERTS)
 def test_experts_whose_scales_lie_far_apart(pkg, many, n, hidden, inter, ratio):
