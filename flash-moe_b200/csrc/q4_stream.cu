@@ -43,6 +43,9 @@ constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kTiles = 2;        // 16-row tiles per unit
 constexpr int kTokBytes = 256;   // a token's group as bytes: 64 inputs x 4
+// What the running sums count: 2^16, so that inputs up to fp32's largest number do not take a group's sums beyond it, where its
+// scale is that of a weight.  (Sums below fp32's normal numbers are exact multiples of 2^-149 * 2^16 until a scale meets them.)
+constexpr float kUnit = 65536.f;
 constexpr int kFactorBytes = 32; // (factor, input sum) for each of the four lanes of a quad: per group and pair of tokens, or per two groups
 
 __device__ __forceinline__ void mma_u8s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -68,7 +71,8 @@ __device__ __forceinline__ void widen8(const float4 &a, const float4 &b, bool va
     float am = 0.f, sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; i++) am = fmaxf(am, fabsf(v[i]));
-    sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+    constexpr float u = 1.f / kUnit;
+    sum = (fmaf(v[0], u, v[1] * u) + fmaf(v[2], u, v[3] * u)) + (fmaf(v[4], u, v[5] * u) + fmaf(v[6], u, v[7] * u));
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) {
         am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, o));
@@ -76,7 +80,8 @@ __device__ __forceinline__ void widen8(const float4 &a, const float4 &b, bool va
     }
     if (!valid) return;
     // am in [2^e, 2^(e+1)): inputs as integers of 2^(e-29), so that |q| < 2^30; groups below 2^-97 keep a fixed step.
-    // A group with an infinity or a NaN (the maximum passes NaN by, the sum does not) makes its token's results NaN.
+    // A group with an infinity or a NaN (the maximum passes NaN by, the sum does not; of finite inputs it stays finite) makes its
+    // token's results NaN.
     int e = (int)(__float_as_uint(am) >> 23) - 127;
     e = max(e, -97);
     const bool bad = !(fabsf(sum) <= 3.4028235e38f) || e > 127;
@@ -101,7 +106,7 @@ __device__ __forceinline__ void widen8(const float4 &a, const float4 &b, bool va
         *reinterpret_cast<uint32_t *>(o + 3 * kPlane + half * 4) = __byte_perm(ab_lo, cd_lo, 0x5410);  // a0 b0 c0 d0
     }
     // the pair of upper digits counts 2^16, the pair of lower ones 1; the input sum goes with either (see the loop)
-    if (wi < 2) factor[wi] = make_float2(wi == 0 ? down * 65536.f : down, sum);
+    if (wi < 2) factor[wi] = make_float2(wi == 0 ? down * (65536.f / kUnit) : down / kUnit, sum);
 }
 
 constexpr int S = 4;             // groups per step
@@ -394,8 +399,9 @@ q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units
                             mma_u8s8(d, a[i][2][0], a[i][2][1], a[i][2][2], a[i][2][3], b23.x, b23.y);
                             mma_u8s8(d, a[i][3][0], a[i][3][1], a[i][3][2], a[i][3][3], b23.z, b23.w);
                             // |d| <= 64 * 15 * 128, so two digits still fit an int; lane t holds the digit pair t & 1 of group t / 2
-                            acc[i][0][0] = fmaf(bf16_of(b ? sc[i][0].y : sc[i][0].x, up) * f.x, (float)(d[0] * 256 + d[1]), acc[i][0][0]);
-                            acc[i][1][0] = fmaf(bf16_of(b ? sc[i][1].y : sc[i][1].x, up) * f.x, (float)(d[2] * 256 + d[3]), acc[i][1][0]);
+                            // (the factor is a power of two and goes to the integer, exactly; a small one would leave a scale few bits)
+                            acc[i][0][0] = fmaf(bf16_of(b ? sc[i][0].y : sc[i][0].x, up), f.x * (float)(d[0] * 256 + d[1]), acc[i][0][0]);
+                            acc[i][1][0] = fmaf(bf16_of(b ? sc[i][1].y : sc[i][1].x, up), f.x * (float)(d[2] * 256 + d[3]), acc[i][1][0]);
                             accb[i][0] = fmaf(bf16_of(b ? bi[i].y : bi[i].x, up), f.y, accb[i][0]);
                         }
                     }
@@ -423,8 +429,8 @@ q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units
                                 mma_u8s8_first(d, a[i][0][0], a[i][0][1], a[i][0][2], a[i][0][3], bf.x, bf.y);
                                 mma_u8s8(d, a[i][1][0], a[i][1][1], a[i][1][2], a[i][1][3], bf.z, bf.w);
                                 // |d| <= 64 * 15 * 128, so two digits still fit an int; lane t holds the digit pair t & 1 of token t / 2
-                                acc[i][0][nt] = fmaf(bf16_at(sc[i][0], j) * f.x, (float)(d[0] * 256 + d[1]), acc[i][0][nt]);
-                                acc[i][1][nt] = fmaf(bf16_at(sc[i][1], j) * f.x, (float)(d[2] * 256 + d[3]), acc[i][1][nt]);
+                                acc[i][0][nt] = fmaf(bf16_at(sc[i][0], j), f.x * (float)(d[0] * 256 + d[1]), acc[i][0][nt]);
+                                acc[i][1][nt] = fmaf(bf16_at(sc[i][1], j), f.x * (float)(d[2] * 256 + d[3]), acc[i][1][nt]);
                                 accb[i][nt] = fmaf(bf16_at(bi[i], j), f.y, accb[i][nt]);
                             }
                         }
@@ -462,6 +468,7 @@ q4_stream_kernel(const __grid_constant__ Q4Params p, int chunk_groups, int units
             const int wq = e / un.cnt, tok = e - wq * un.cnt;
             float y = 0.f;
             for (int w = 0; w < WK; w++) y += red[((size_t)(wq * WK + w) * kTok + tok) * 32 + lane];
+            y *= kUnit;
             const size_t pr = (size_t)pair_at(un.start, tok);
             const int row = un.row0 + (MODE == kGateUp ? wq * 16 : wq * 32) + lane;
             if constexpr (MODE == kGateUp) {

@@ -101,6 +101,24 @@ def test_small_inputs_beside_large_ones_without_weight(pkg, many, n, k, out, rat
     c.close()
 
 
+@pytest.mark.parametrize("many,n,k,out", [(1, 1, 768, 48), (1, 2, 832, 48), (1, 4, 768, 48), *PROJ])
+def test_inputs_next_to_the_largest_number(pkg, many, n, k, out):
+    """Finite inputs whose sums leave fp32's range do not make outputs that lie within it infinite or NaN."""
+    rng = np.random.default_rng(700 + n)
+    c = context(pkg, max_batch=512)
+    w, s, b = moe_ref.weights(rng, out, k)
+    m = (w, *(moe_ref.bf16(moe_ref.f32(a) / 128) for a in (s, b)))
+    x = rng.uniform(2.0e38, 3.4e38, size=(n, k)).astype(np.float32)
+    x[0, : k // 2] *= -1
+    x[-1, ::3] = np.finfo(np.float32).max
+    want, bound = moe_ref.product(x, m)
+    assert np.abs(want).max() < 1e38
+    count, got = launches(c, lambda: run_proj(pkg, c, [m], x)[0])
+    assert count == many
+    moe_ref.close(got, want, bound)
+    c.close()
+
+
 @pytest.mark.parametrize("ratio", [1e-3, 2.0 ** -20])
 @pytest.mark.parametrize("many,n,hidden,inter", EXPERTS)
 def test_experts_whose_scales_lie_far_apart(pkg, many, n, hidden, inter, ratio):
