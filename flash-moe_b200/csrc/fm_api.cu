@@ -588,6 +588,26 @@ struct Stager {
     }
 };
 
+// Staging for the tensors of one call, where they are not among those that fm_create counts (stage_need).  Grows, and waits for
+// what may still be under way through the old buffers.
+static size_t staged(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
+static fm_status stage_reserve(FmCtx *ctx, const char *fn, size_t need) {
+    if (ctx->ptr_mode != FM_PTR_HOST || need <= ctx->stage_bytes) return FM_OK;
+    FM_CUDA(ctx, cudaDeviceSynchronize());
+    need = std::max(need, ctx->stage_bytes + ctx->stage_bytes / 4);
+    char *h = nullptr, *d = nullptr;
+    cudaError_t e = cudaMallocHost(&h, need);
+    if (e == cudaSuccess && (e = cudaMalloc(&d, need)) != cudaSuccess) cudaFreeHost(h);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return fail(ctx, FM_ERR_NOMEM, "%s: %zu bytes of staging: %s", fn, need, cudaGetErrorString(e));
+    }
+    cudaFreeHost(ctx->h_stage);
+    cudaFree(ctx->d_stage);
+    ctx->h_stage = h; ctx->d_stage = d; ctx->stage_bytes = need;
+    return FM_OK;
+}
+
 // ---- token lists ------------------------------------------------------------------------------
 static fm_status check_layer_seq(FmCtx *ctx, const char *fn, int layer, int nlayers, const int *seq, int n) {
     if (layer < 0 || layer >= nlayers) return fail(ctx, FM_ERR_INVALID, "%s: layer index %d of %d", fn, layer, nlayers);
@@ -1108,6 +1128,10 @@ extern "C" fm_status fm_proj_forward(FmCtx *ctx, int count, const FmProjWeights 
     if (n == 0) return FM_OK;
     FM_CUDA(ctx, cudaSetDevice(ctx->cfg.device));
     const size_t K = (size_t)w[0].in_dim;
+    size_t need = staged(n * K * 4);
+    for (int i = 0; i < count; i++) need += staged((size_t)n * w[i].out_dim * 4);
+    fm_status st = stage_reserve(ctx, "fm_proj_forward", need);
+    if (st) return st;
     Stager sg(ctx);
     bool ok = true;
     Q4Params p = {};
@@ -1118,12 +1142,11 @@ extern "C" fm_status fm_proj_forward(FmCtx *ctx, int count, const FmProjWeights 
         p.out[i] = sg.out(y[i], (size_t)n * w[i].out_dim, &ok, &where[i]);
         p.mat[i] = Q4View{(const unsigned char *)w[i].w, (const unsigned char *)w[i].scales, (const unsigned char *)w[i].biases, 0, 0, w[i].out_dim};
     }
-    if (!ok) return fail(ctx, FM_ERR_INVALID, "fm_proj_forward: staging buffer too small (raise max_batch_tokens)");
+    if (!ok) return fail(ctx, FM_ERR_NOMEM, "fm_proj_forward: staging buffer too small");
     if (!aligned16(p.x)) return fail(ctx, FM_ERR_INVALID, "fm_proj_forward: x is not 16-byte aligned");
     const bool gemm = !proj_streams(w, count, n, ctx->sm_count);
     void *xs = nullptr;
     float *tscale = nullptr;
-    fm_status st;
     if (gemm) {
         auto carve = [&](Carver cv) {
             xs = cv.take<uint16_t>((size_t)n * 2 * q4_split_columns(p.in_dim));
@@ -1177,6 +1200,8 @@ extern "C" fm_status fm_moe_route(FmCtx *ctx, const FmRouteConfig *rc, int n, co
     if (n == 0) return FM_OK;
     FM_CUDA(ctx, cudaSetDevice(ctx->cfg.device));
     const size_t cols = (size_t)rc->num_experts + rc->shared_expert, slots = (size_t)rc->top_k + rc->shared_expert;
+    fm_status st = stage_reserve(ctx, "fm_moe_route", staged(n * cols * 4) + staged((size_t)rc->num_experts * 4) + 2 * staged(n * slots * 4));
+    if (st) return st;
     Stager sg(ctx);
     bool ok = true;
     size_t w_ids = 0, w_w = 0;
@@ -1185,11 +1210,11 @@ extern "C" fm_status fm_moe_route(FmCtx *ctx, const FmRouteConfig *rc, int n, co
     p.bias = sg.in(bias, (size_t)rc->num_experts, &ok);
     p.ids = sg.out(expert_ids, n * slots, &ok, &w_ids);
     p.weights = sg.out(weights, n * slots, &ok, &w_w);
-    if (!ok) return fail(ctx, FM_ERR_INVALID, "fm_moe_route: staging buffer too small (raise max_batch_tokens)");
+    if (!ok) return fail(ctx, FM_ERR_NOMEM, "fm_moe_route: staging buffer too small");
     p.n = n; p.experts = rc->num_experts; p.top_k = rc->top_k; p.score = rc->score; p.groups = rc->num_groups; p.top_groups = rc->top_groups;
     p.group_best = rc->group_best; p.renormalize = rc->renormalize; p.shared = rc->shared_expert; p.scale = rc->scale;
     FM_CUDA(ctx, sg.push());
-    fm_status st = launched(ctx, launch_moe_route(p, ctx->stream), "moe_route");
+    st = launched(ctx, launch_moe_route(p, ctx->stream), "moe_route");
     if (st) return st;
     FM_CUDA(ctx, sg.pull(expert_ids, w_ids, n * slots));
     FM_CUDA(ctx, sg.pull(weights, w_w, n * slots));
@@ -1218,6 +1243,8 @@ extern "C" fm_status fm_moe_experts(FmCtx *ctx, const FmExpertWeights *w, int n,
     if (n == 0) return FM_OK;
     FM_CUDA(ctx, cudaSetDevice(ctx->cfg.device));
     const size_t H = (size_t)w->hidden, I = (size_t)w->inter, pairs = (size_t)n * top_k;
+    fm_status st = stage_reserve(ctx, "fm_moe_experts", 4 * staged(n * H * 4) + 2 * staged(pairs * 4) + staged(H * 2));
+    if (st) return st;
     Stager sg(ctx);
     bool ok = true;
     size_t w_out = 0, w_norm = 0;
@@ -1226,7 +1253,7 @@ extern "C" fm_status fm_moe_experts(FmCtx *ctx, const FmExpertWeights *w, int n,
     const float *d_w = sg.in(weights, pairs, &ok), *d_res = sg.in(residual, n * H, &ok);
     const uint16_t *d_nw = sg.in(h_norm ? norm_w : nullptr, H, &ok);
     float *d_out = sg.out(h_out, n * H, &ok, &w_out), *d_norm = sg.out(h_norm, n * H, &ok, &w_norm);
-    if (!ok) return fail(ctx, FM_ERR_INVALID, "fm_moe_experts: staging buffer too small (raise max_batch_tokens)");
+    if (!ok) return fail(ctx, FM_ERR_NOMEM, "fm_moe_experts: staging buffer too small");
     if (!aligned16(d_x) || !aligned16(d_res) || !aligned16(d_out) || !aligned16(d_norm) || ((uintptr_t)d_nw & 7))
         return fail(ctx, FM_ERR_INVALID, "fm_moe_experts: x, residual, h_out and h_norm have to be 16-byte aligned, norm_w 8-byte");
 
@@ -1250,7 +1277,7 @@ extern "C" fm_status fm_moe_experts(FmCtx *ctx, const FmExpertWeights *w, int n,
         return cv.off;
     };
     char *ws = nullptr;
-    fm_status st = moe_workspace(ctx, "fm_moe_experts", carve(Carver{nullptr}), &ws);
+    st = moe_workspace(ctx, "fm_moe_experts", carve(Carver{nullptr}), &ws);
     if (st) return st;
     carve(Carver{ws});
     FM_CUDA(ctx, sg.push());

@@ -380,3 +380,41 @@ def test_experts_of_the_longest_rows(pkg, n, hidden, inter):
     x, res, ids, w, nw = inputs(rng, n, hidden, 2, 2)
     check(run_experts(pkg, c, device_stacks(pkg, m), x, ids, w, res, nw), m, x, ids, w, res, nw)
     c.close()
+
+
+def test_host_pointers_of_a_context_with_few_heads(pkg):
+    """A context stages as many tokens as it was made for, however small its attention tensors are."""
+    rng = np.random.default_rng(720)
+    n, hidden = 512, 2048
+    few = dict(num_attn_heads=4, num_kv_heads=1, linear_num_v_heads=1, linear_num_k_heads=1)
+    c = context(pkg, host=True, max_batch=n, **few)
+    m, mat = stacks(rng, 3, hidden, 64), moe_ref.weights(rng, 9000, 128)
+    dev, d = device_stacks(pkg, m), on_device(pkg, mat)
+    rcd = dict(num_experts=1024, top_k=30, score=1, num_groups=1, top_groups=1, group_best=1, renormalize=1, scale=1.0, shared_expert=1)
+
+    def project():
+        x, y = rng.standard_normal((n, 128)).astype(np.float32), np.empty((n, 9000), np.float32)
+        c.proj_forward([d], n, x, [y])
+        moe_ref.close(y, *moe_ref.product(x, mat))
+
+    def route():
+        logits = rng.standard_normal((n, 1025)).astype(np.float32)
+        ids, w = np.empty((n, 31), np.int32), np.empty((n, 31), np.float32)
+        c.moe_route(pkg.route_config(**rcd), n, logits, None, ids, w)
+        want = moe_ref.route(logits, None, rcd)
+        assert np.array_equal(ids, want[0]) and np.abs(w - want[1]).max() < 1e-6
+
+    def experts():
+        x, res, ids, w, nw = inputs(rng, n, hidden, 3, 2)
+        out, nrm = np.empty_like(x), np.empty_like(x)
+        c.moe_experts(dev, n, 2, x, ids, w, res, nw, out, nrm)
+        check((out, nrm), m, x, ids, w, res, nw)
+    route()
+    experts()
+    project()
+    experts()
+    route()
+    c.close()
+    c = context(pkg, host=True, max_batch=n, **few)
+    project()
+    c.close()
