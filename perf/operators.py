@@ -214,7 +214,7 @@ def _call(s):
                               group_best=c["group_best"], renormalize=int(c["renorm"]), scale=c["scale"], shared_expert=int(c["shared"]))
         call, out = ctx.prepared_moe_route(rc, n, s["logits"], s["bias"], s["ids"], s["weights"]), (s["ids"], s["weights"])
     else:
-        w = pkg.expert_weights(s["gate"], s["up"], s["down"], first_expert=c["first"])
+        w = pkg.expert_weights(s["gate"], s["up"], s["down"], first_expert=c["first"], total_experts=c["experts"])
         call = ctx.prepared_moe_experts(w, n, c["top"], s["x"], s["ids"], s["weights"], s["residual"], s["norm_w"], s["h_out"], s["h_norm"])
         out = (s["h_out"], s["h_norm"])
 
