@@ -1118,8 +1118,8 @@ extern "C" fm_status fm_proj_forward(FmCtx *ctx, int count, const FmProjWeights 
     if (n < 0 || n > ctx->cfg.max_batch_tokens) return fail(ctx, FM_ERR_INVALID, "fm_proj_forward: n=%d exceeds max_batch_tokens=%d", n, ctx->cfg.max_batch_tokens);
     for (int i = 0; i < count; i++) {
         if (!w[i].w || !w[i].scales || !w[i].biases || !y[i]) return fail(ctx, FM_ERR_INVALID, "fm_proj_forward: null argument (matrix %d)", i);
-        if (w[i].format != FM_W_Q4_AFFINE || w[i].group_size != 64 || w[i].out_dim < 1 || w[i].in_dim < 64 || w[i].in_dim % 64 || w[i].in_dim > 65536)
-            return fail(ctx, FM_ERR_UNSUPPORTED, "fm_proj_forward: matrix %d: format %d, group size %d, %d x %d (in a multiple of 64 up to 65536)", i,
+        if (w[i].format != FM_W_Q4_AFFINE || w[i].group_size != 64 || w[i].out_dim < 1 || w[i].out_dim > (1 << 30) || w[i].in_dim < 64 || w[i].in_dim % 64 || w[i].in_dim > 65536)
+            return fail(ctx, FM_ERR_UNSUPPORTED, "fm_proj_forward: matrix %d: format %d, group size %d, %d x %d (in a multiple of 64 up to 65536, out up to 2^30)", i,
                         w[i].format, w[i].group_size, w[i].out_dim, w[i].in_dim);
         if (w[i].in_dim != w[0].in_dim) return fail(ctx, FM_ERR_INVALID, "fm_proj_forward: matrix %d reads %d inputs, matrix 0 reads %d", i, w[i].in_dim, w[0].in_dim);
         if (!aligned16(w[i].w) || !aligned2(w[i].scales, w[i].biases) || !aligned4(y[i]))

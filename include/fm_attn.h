@@ -306,7 +306,7 @@ fm_status fm_out_proj_norm(FmCtx *ctx, const FmProjWeights *w, int n, const floa
  * size, dequant_gemm_4bit_batch (metal_infer/shaders.metal); CPU cpu_dequant_matvec (metal_infer/cpu_kernels.h:199-232).
  * x [n][in_dim], y[i] [n][out_dim_i] follow the pointer mode; the array y itself is a host array; weights are device
  * pointers in either mode.  Words and x 16-byte aligned, the rest as its type; in_dim a multiple of 64 (up to 65536) and the
- * same for all, out_dim any; n up to max_batch_tokens.  Up to 8 tokens nothing is allocated; the first call of a size
+ * same for all, out_dim up to 2^30; n up to max_batch_tokens.  Up to 8 tokens nothing is allocated; the first call of a size
  * with more may allocate workspace (so make it before a stream capture: FM_ERR_CAPACITY otherwise); graphs captured on one
  * context share that workspace and must not run at the same time.
  * Accuracy is fp32's: the nibbles are exact on the tensor cores, an activation enters them as 22 bits or more, the scale and

@@ -192,6 +192,21 @@ def test_two_contexts_at_once(pkg):
         c.close()
 
 
+def test_more_rows_than_32_bit_row_numbers_take_are_refused(pkg):
+    """The kernels count rows in int, past the last one by up to a unit."""
+    c = context(pkg, max_batch=128)
+    a = on_device(pkg, moe_ref.weights(np.random.default_rng(2), 16, 128))
+    x, y = torch.zeros((100, 128), device="cuda"), torch.zeros((100, 16), device="cuda")
+    for rows in (2 ** 30 + 1, 2 ** 31 - 1):
+        big = pkg.binding.FmProjWeights.from_buffer_copy(a)
+        big.out_dim = rows
+        for n in (1, 100):
+            with pytest.raises(pkg.FmError) as e:
+                c.proj_forward([big], n, x, [y])
+            assert e.value.status == pkg.binding.FM_ERR_UNSUPPORTED
+    c.close()
+
+
 def test_refusals(pkg):
     rng = np.random.default_rng(2)
     c = context(pkg, max_batch=8)
