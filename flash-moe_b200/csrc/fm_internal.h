@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <string>
 #include <vector>
 
@@ -377,6 +378,18 @@ inline cudaError_t launch_dependent(void (*kernel)(P...), dim3 grid, dim3 block,
     at[0].val.programmaticStreamSerializationAllowed = 1;
     lc.attrs = at; lc.numAttrs = 1;
     return cudaLaunchKernelEx(&lc, kernel, static_cast<P>(args)...);
+}
+
+// Raises a kernel's dynamic shared memory limit on the current device, once.  Contexts of several threads may come here at the
+// same time: a device counts as done only when its limit is raised, and a second raise of the same limit changes nothing.
+inline bool raise_smem_limit(const void *kernel, int bytes, std::atomic<unsigned long long> *done) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return false;
+    const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+    if (done->load(std::memory_order_acquire) & bit) return true;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+    done->fetch_or(bit, std::memory_order_release);
+    return true;
 }
 
 // True the first time it is called for the current device with a given per-call-site flag word: function

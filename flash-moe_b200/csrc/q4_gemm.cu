@@ -888,10 +888,8 @@ int launch_gemm(const GemmMaps &maps, GemmParams &g, long long jobs, int sm_coun
         g.m_units[i] = (g.p.mat[i].rows + kRows - 1) / kRows;
         g.units_per_job += g.m_units[i];
     }
-    static unsigned long long configured = 0;
-    if (first_use_on_device(&configured) &&
-        cudaFuncSetAttribute(q4_gemm_kernel<MODE, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem) != cudaSuccess)
-        return -1;
+    static std::atomic<unsigned long long> configured{0};
+    if (!raise_smem_limit(reinterpret_cast<const void *>(q4_gemm_kernel<MODE, WIDE>), kGemmSmem, &configured)) return -1;
     // (fewer units than SMs: as many CTAs as there are units or, cut, tiles; idle ones would crowd the others onto half of the GPU)
     const long long units = jobs * g.units_per_job;
     const int grid = (int)std::min<long long>(MODE == kProj && 2 * units <= sm_count ? 2 * units : units, sm_count);

@@ -495,10 +495,8 @@ int launch_one(const Q4Params &p, int jobs, int sm_count, cudaStream_t st) {
     int chunk = (G + S - 1) / S * S;  // whole steps
     while (smem_bytes(NTL, chunk) > kMaxSmem) chunk = (chunk / 2 + S - 1) / S * S;
     const size_t smem = smem_bytes(NTL, chunk);
-    static unsigned long long configured = 0;
-    if (first_use_on_device(&configured) &&
-        cudaFuncSetAttribute(q4_stream_kernel<MODE, NTL, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem) != cudaSuccess)
-        return -1;
+    static std::atomic<unsigned long long> configured{0};
+    if (!raise_smem_limit(reinterpret_cast<const void *>(q4_stream_kernel<MODE, NTL, WIDE>), kMaxSmem, &configured)) return -1;
     const int grid_max = sm_count * std::max(1, std::min(NTL == 4 ? 1 : 2, (int)((220 * 1024) / (smem + 1024))));
     // Warps along a row, the others side by side on more rows.  An SM's time is its units' steps, plus a unit's end worth about
     // 0.6 of a step (the warps meet, the next unit's addresses), and it takes whole units: the cheapest split.  (One token x 4096

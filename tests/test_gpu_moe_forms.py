@@ -1,4 +1,8 @@
 """fm_proj_forward and fm_moe_experts choose among kernels by size: each choice, at the places where it can go wrong."""
+import subprocess
+import sys
+from pathlib import Path
+
 import numpy as np
 import pytest
 import torch
@@ -418,3 +422,55 @@ def test_host_pointers_of_a_context_with_few_heads(pkg):
     c = context(pkg, host=True, max_batch=n, **few)
     project()
     c.close()
+
+
+THREADS = """
+import sys, threading
+sys.path[:0] = {path!r}
+import numpy as np, torch
+import moe_ref
+from __graft_entry__ import load_package
+from test_gpu_moe_experts import check, cuda, device_stacks, inputs, stacks
+from test_gpu_proj_forward import context, on_device
+pkg = load_package()
+rng = np.random.default_rng(730)
+mat, m = moe_ref.weights(rng, 1100, 512), stacks(rng, 6, 512, 320)
+d, dev = on_device(pkg, mat), device_stacks(pkg, m)
+sizes = [1, 2, 4, 8, 300, 700]
+work = [(n, inputs(rng, n, 512, 6, 3)) for n in sizes]
+contexts = [context(pkg, max_batch=1024) for _ in range(4)]
+buffers = [[([cuda(a) for a in v], torch.empty((n, 1100), device="cuda"), torch.empty((n, 512), device="cuda"), torch.empty((n, 512), device="cuda")) for n, v in work]
+           for _ in contexts]
+streams = [torch.cuda.Stream() for _ in contexts]
+torch.cuda.synchronize()
+gate, failed = threading.Barrier(len(contexts)), []
+
+def body(c, st, bufs):
+    try:
+        c.set_stream(st.cuda_stream)
+        gate.wait()
+        for (n, _), ((x, res, ids, w, nw), y, h, hn) in zip(work, bufs):  # every kernel's first launch falls on all threads at once
+            c.proj_forward([d], n, x, [y])
+            c.moe_experts(dev, n, 3, x, ids, w, res, nw, h, hn)
+        c.synchronize()
+    except Exception as e:
+        failed.append(e)
+
+threads = [threading.Thread(target=body, args=a) for a in zip(contexts, streams, buffers)]
+[t.start() for t in threads]
+[t.join() for t in threads]
+assert not failed, failed
+for bufs in buffers:
+    for (n, v), (_, y, h, hn) in zip(work, bufs):
+        moe_ref.close(y.cpu().numpy(), *moe_ref.product(v[0], mat))
+        check((h.cpu().numpy(), hn.cpu().numpy()), m, v[0], v[2], v[3], v[1], v[4])
+[c.close() for c in contexts]
+print("threads ok")
+"""
+
+
+def test_contexts_of_several_threads_begin_at_once():
+    """A process of its own, so that the first launch of every kernel falls on four threads with a context each."""
+    here = Path(__file__).resolve().parent
+    r = subprocess.run([sys.executable, "-c", THREADS.format(path=[str(here), str(here.parent)])], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "threads ok" in r.stdout, r.stdout[-2000:] + r.stderr[-2000:]
