@@ -1095,7 +1095,10 @@ static bool proj_streams(const FmProjWeights *w, int count, int n, int sm_count)
 // read again for each of its pairs.  Tokens are taken to choose evenly among the model's experts.
 // Measured, straight, stream and prompt form: 512 experts of 4096 x 1024, 10 per token, 1 token 29, 38 and 118 us, 48 tokens -,
 // 447 and 773, 208 tokens -, 1170 and 1298, 320 tokens -, 1687 and 1428; 16 experts of 1024 x 512, one per token, 16 tokens 11,
-// 17 and 34, 128 tokens 31, 25 and 41.  Over 110 sizes the choice costs 2 % against always the best one.
+// 17 and 34, 128 tokens 31, 25 and 41.  Over 110 sizes the choice costs 2 % against always the best one.  The price of a tile (11 ns
+// per input) is that of the kernel for scales in 16-byte pieces; the other one takes up to 1.8 times that, and the choice stands
+// there because the stream form takes longer still (596 tokens through 10 of 344 experts of 1792 x 384: 400 us, expected 232).
+// Where all tokens go to the same few experts, the jobs are fewer than expected.
 enum class ExpertForm { kStraight, kStream, kPrompt };
 static ExpertForm expert_form(const FmExpertWeights *w, int n, int top_k, int sm_count) {
     const double all = std::max(w->total_experts, w->num_experts), held = w->num_experts, pairs = (double)n * top_k, here = pairs * held / all;

@@ -31,9 +31,10 @@
 // Why 96: sums, steps and operands share 512 columns, token tiles 144 KB; at 64 tokens a weight is widened half as often again
 // and the MMA's start-up counts more, at 128 the steps could not be double-buffered.
 //
-// Measured (B200, 1.9 GHz; the tensor work is twice the product's, because of the two terms): 4096 tokens x 4096 x 8192 in
-// 514 us, 535 TFLOP/s of products (the tensor core is busy 73 % of the time in MMAs of 57 cycles, ideal 48); 300 tokens through
-// qkv + z + beta + alpha of 4096 in 120 us; 4096 tokens through 10 of 512 experts of 4096 x 1024: gate / up 1.72 ms, down 0.96 ms.
+// Measured (B200; the tensor work is twice the product's, because of the two terms): 4096 tokens x 4096 x 8192 in 520 us as a
+// replayed graph, 528 TFLOP/s of products (the tensor core is busy 72 % of the time in MMAs of 57 cycles, ideal 48), 610 us in calls
+// on fresh inputs (450 TFLOP/s, under the power cap); 300 tokens through qkv + z + beta + alpha of 4096 in 117 and 132 us; 4096
+// tokens through 10 of 512 experts of 4096 x 1024: gate / up 1.77 ms, down 0.98 ms.
 // What bounds it: the issue slots.  Widening, the epilogue and the hand-overs between the roles take 2000 to 2300 instructions
 // per operand slot of 915 tensor cycles; below 64 tokens a unit takes about 950 cycles per slot whatever its tokens.
 // Tried and not kept: 16 widening warps (the same time), the two issuing warps as one (+10 %), operand slots of one group
@@ -180,7 +181,7 @@ __device__ __forceinline__ uint2 chunk_scales(const unsigned char *row, int c) {
 }
 // Where they are not, a row begins at any even address.  It is read in aligned windows, each once, and its pieces are cut out
 // of two of them.  Read 2 bytes at a time (a sector of 32 per load and row, next to no L1 beside the tiles) 4160 inputs took
-// 2.4 times as long as 4096 (4096 rows, 20 tokens: 89 and 36 us), so they take 49.  A window that reaches beyond the matrix is
+// 2.4 times as long as 4096 (4096 rows, 20 tokens), in windows 1.35 times (28 and 21 us as a replayed graph).  A window that reaches beyond the matrix is
 // read by the 2 bytes that belong to it.
 struct Bytes { const unsigned char *begin, *end; };
 __device__ __forceinline__ uint2 window8(const unsigned char *at, Bytes m) {

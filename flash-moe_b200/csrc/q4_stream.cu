@@ -21,9 +21,9 @@
 // activations are widened once per CTA and not once per unit, and the next unit's weights are fetched while this one's sums
 // meet.
 //
-// Measured (B200): one token x 4096 x 17408 in 11.2 us (40 MB: 3.6 TB/s; 5.3 TB/s in the long run, 4.5 us go into the start and
-// the end), x 8192 x 4096 in 9 us; one token through 10 of 512 experts of 4096 x 1024 in 29 us with the weighted sum; 48 tokens
-// through them (2.2 GB) in 450 us, 4.9 TB/s.  In the long run it is bound by the L1 cache's wavefronts (72 % of their peak): a
+// Measured (B200, as replayed graphs): one token x 4096 x 17408 in 11 us (40 MB: 3.6 TB/s; 5.3 TB/s in the long run, 4.5 us go into
+// the start and the end), x 8192 x 4096 in 9 us; one token through 10 of 512 experts of 4096 x 1024 in 28 us with the weighted sum; 48
+// tokens through them (2.2 GB) in 450 us, 4.9 TB/s.  Calls on fresh inputs take 14.5, 32 and 480 us.  In the long run it is bound by the L1 cache's wavefronts (72 % of their peak): a
 // request of a warp touches 8 rows, 64 or 32 bytes of each, and the scales and biases cost as many as the words.
 // One token in the two-token form: 12.5 and 35 us; the one-token form for 3 or more tokens takes 1.3 to 1.8 times as long.
 // Rows read 64 bytes at a time for more tokens too, a group's share of the columns zero in the lanes of the other, doubles the

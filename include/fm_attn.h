@@ -307,11 +307,21 @@ fm_status fm_out_proj_norm(FmCtx *ctx, const FmProjWeights *w, int n, const floa
  * x [n][in_dim], y[i] [n][out_dim_i] follow the pointer mode; the array y itself is a host array; weights are device
  * pointers in either mode.  Words and x 16-byte aligned, the rest as its type; in_dim a multiple of 64 (up to 65536) and the
  * same for all, out_dim up to 2^30; n up to max_batch_tokens.  Up to 8 tokens nothing is allocated; the first call of a size
- * with more may allocate workspace (so make it before a stream capture: FM_ERR_CAPACITY otherwise); graphs captured on one
- * context share that workspace and must not run at the same time.
- * Accuracy is fp32's: the nibbles are exact on the tensor cores, an activation enters them as 22 bits or more, the scale and
- * bias of a group meet its sum in fp32.  A token with an infinity or a NaN among its inputs gets NaN outputs.
- * The outputs must not overlap each other or the inputs. */
+ * with more may allocate workspace (so make it before a stream capture: FM_ERR_CAPACITY otherwise), 4 n (in_dim + in_dim / 64,
+ * that rounded up to a multiple of 64) bytes.  One workspace serves this call and fm_moe_experts.  It grows by a quarter at the least;
+ * outgrown blocks stay until fm_destroy, since captured graphs may hold their addresses, so begin with the largest call (sizes
+ * that creep up leave a context with up to five times the last one).  Graphs captured on one context, and calls queued on
+ * different streams of it, share the workspace and must not run at the same time.  In host-pointer mode the staging buffers
+ * grow with the call.
+ * Accuracy is fp32's: an output is off by at most (in_dim / 64 + 64) 2^-24 of the sum of |nibble scale x| + |bias x| over its
+ * inputs, within these limits.  The kernel for few tokens (always up to 8): scale and bias of a group meet its sum in fp32, an input
+ * has 30 bits below the largest of its group of 64, and an absolute error of 2^-127 at the least.  The kernel for many tokens:
+ * an input has 22 bits down to 2^-16 of the largest of its token, and below that an absolute error of 2^-39 of it (2^-33 the sum of
+ * 64 inputs that meets the bias); scales are exact down to 2^-23 of the largest of their row's 256 inputs (groups 4 i to
+ * 4 i + 3), and below that leave each weight an absolute error of 2^-31 of that scale; bias + 8 scale has 22 bits down to 2^-16
+ * of the largest of its row's 4096 inputs, and below that 2^-39 of it; scales lie below 2^117.  Which kernel runs follows from
+ * the sizes, so a token's last bits may change with the number of tokens beside it; the same call gives the same bits.
+ * A token with an infinity or a NaN among its inputs gets NaN outputs.  The outputs must not overlap each other or the inputs. */
 fm_status fm_proj_forward(FmCtx *ctx, int count, const FmProjWeights *w, int n, const float *x, float *const *y);
 
 /* Routing: which experts a token goes to, and with what weights.  The reference takes the softmax of the gate's logits, the
@@ -362,10 +372,11 @@ fm_status fm_moe_route(FmCtx *ctx, const FmRouteConfig *rc, int n, const float *
  * token counts twice.  x [n][hidden], expert_ids and weights [n][top_k] (top_k <= 32), residual, h_out and h_norm [n][hidden]
  * follow the pointer mode; h_out may be the residual itself, and x may be h_out or h_norm.  hidden and inter multiples of 64
  * (up to 65536), num_experts <= 1024, n up to max_batch_tokens.  Words, x, residual, h_out and h_norm 16-byte aligned, norm_w
- * 8-byte, the rest as its type.  Accuracy as for fm_proj_forward; the same call gives the same bits, whichever order the
- * launches' blocks take.
- * The first call of a size allocates workspace (so make it before a stream capture: FM_ERR_CAPACITY otherwise); graphs
- * captured on one context share that workspace and must not run at the same time. */
+ * 8-byte, the rest as its type; n * top_k up to 2^24.  Accuracy as for fm_proj_forward, product by product; the same call gives
+ * the same bits, whichever order the launches' blocks take.  h_norm's sum of squares is fp32's.
+ * The first call of a size allocates workspace (so make it before a stream capture: FM_ERR_CAPACITY otherwise), the one of
+ * fm_proj_forward and under its terms: per token and slot 4 (hidden + inter) bytes, with many tokens about twice that (4096 tokens
+ * with 10 slots of 4096 x 1024: 1.7 GB). */
 typedef struct FmExpertWeights {
     int format;                  /* FM_W_Q4_AFFINE */
     int num_experts, first_expert;
